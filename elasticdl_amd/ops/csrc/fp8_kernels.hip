@@ -1,0 +1,880 @@
+// Dense layers in 8-bit floating point for MI355X (gfx950, CDNA4).
+//
+// Numbers. A block of 128 values shares one power of two s = 2^e, the
+// smallest with max|v| <= 448 s (e >= -126), and each value is stored as
+// e4m3(v / s), rounded to nearest, ties to even. s is stored as the byte
+// e + 127. A power of two divides exactly, so the one rounding is e4m3's
+// (half a step is 2^-4 of the value), and the matrix instruction takes the
+// byte as it is: v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 128-long
+// rows, scales each product of blocks and adds in 32 bits, so that a block
+// of 128 costs no vector instruction at all. Values that are not finite are
+// stored as e4m3's NaN and leave their block's scale alone.
+//
+// Two ways to multiply. The 8-bit matrix instructions of this chip add eight
+// neighbouring products with about 16 bits below the largest of them (32
+// only between such groups): 1.6e-5 of a result's norm, measured over random
+// e4m3. That is far below e4m3's and a 16-bit result's own rounding, but not
+// 32 bits. So where a result is returned in 32 bits, and where the sign of
+// a sum decides a relu's gradient, the bytes are widened to bf16 in
+// registers on the way (exactly, scale included) and multiplied by the bf16
+// instruction, whose sums hold 24 bits (8e-9 measured), at half the rate.
+//
+// Layout. A matrix [R, C] that is contracted over C is stored as bytes
+// [R, Cp], Cp = C rounded up to 128 (zeros behind C), with scales
+// [Cp/128, Rp], Rp = R rounded up to 256. Within each 64 rows the scale
+// bytes are permuted (scale_slot below) so that a lane finds the bytes of
+// the four fragments that it multiplies in one 32-bit word.
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "fp8_kernels.h"
+
+typedef __attribute__((ext_vector_type(8))) int i32x8;
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef __attribute__((ext_vector_type(2))) int i32x2;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+
+namespace {
+
+constexpr int kBlk = EDL_FP8_BLOCK;
+
+// ------------------------------ small pieces ------------------------------
+__device__ inline float as_f32(float v) { return v; }
+__device__ inline float as_f32(__bf16 v) { return (float)v; }
+__device__ inline float as_f32(_Float16 v) { return (float)v; }
+
+__device__ inline float load_any(const void* p, int64_t i, int type) {
+  if (type == EDL_T_F32) return static_cast<const float*>(p)[i];
+  if (type == EDL_T_BF16) return (float)static_cast<const __bf16*>(p)[i];
+  return (float)static_cast<const _Float16*>(p)[i];
+}
+
+__device__ inline void store_any(void* p, int64_t i, float v, int type) {
+  if (type == EDL_T_F32)
+    static_cast<float*>(p)[i] = v;
+  else if (type == EDL_T_BF16)
+    static_cast<__bf16*>(p)[i] = (__bf16)v;
+  else
+    static_cast<_Float16*>(p)[i] = (_Float16)v;
+}
+
+__device__ inline float activate(float z, int act) {
+  if (act == EDL_ACT_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
+  if (act == EDL_ACT_SIGMOID) return 1.f / (1.f + __expf(-z));
+  return z;
+}
+
+// |v|'s bits, 0 where v is infinite or NaN; as integers they order like |v|
+__device__ inline uint32_t finite_abs(float v) {
+  uint32_t b = __float_as_uint(v) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+
+// The byte e + 127 of the smallest 2^e with amax <= 448 * 2^e:
+// 448 = 1.75 * 2^8, so e is amax's exponent - 8, and one more where amax's
+// mantissa is over 1.75. At least 1 (2^-126), so that 2^-e is normal.
+__device__ inline int scale_byte(uint32_t amax) {
+  int b = (int)(amax >> 23) - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return b < 1 ? 1 : b;
+}
+
+__device__ inline float inverse_of(int byte) {  // 2^(127 - byte), exact
+  return __uint_as_float((uint32_t)(254 - byte) << 23);
+}
+
+// x / s, and NaN where x is not finite (infinity * 0), which the conversion
+// stores as 0xff; it would take infinity for a large number
+__device__ inline float scaled(float x, float inv) {
+  return __builtin_fmaf(x, 0.f, x * inv);
+}
+
+__device__ inline uint32_t pack4(float a, float b, float c, float d,
+                                 float inv) {
+  int v = 0;
+  v = __builtin_amdgcn_cvt_pk_fp8_f32(scaled(a, inv), scaled(b, inv), v, false);
+  v = __builtin_amdgcn_cvt_pk_fp8_f32(scaled(c, inv), scaled(d, inv), v, true);
+  return (uint32_t)v;
+}
+
+// where row r's scale byte lies within its column of Rp bytes
+__device__ inline int64_t scale_slot(int64_t r) {
+  int n = (int)(r & 63);
+  return (r & ~(int64_t)63) + (n >> 4) * 16 + (n & 3) * 4 + ((n >> 2) & 3);
+}
+
+// largest over the 16 lanes of a row of lanes
+template <int CTRL>
+__device__ inline uint32_t max_ror(uint32_t v) {
+  uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf,
+                                                     false);
+  return v > o ? v : o;
+}
+__device__ inline uint32_t max16(uint32_t v) {
+  v = max_ror<0x128>(v);  // row_ror:8, 4, 2, 1
+  v = max_ror<0x124>(v);
+  v = max_ror<0x122>(v);
+  return max_ror<0x121>(v);
+}
+
+// --------------------------------- quantise -------------------------------
+// One workgroup takes a tile of 128 x 128 and each thread 8 x 8 of it, so
+// that a block's maximum lies in one 16-lane row of lanes (rows) or in the
+// four waves (columns), and both forms are written from one read of x.
+// Bound by memory.
+//
+// DERIV: x is the gradient at an activation's output, which is turned into
+// the gradient at its input on the way (relu: one kept bit; sigmoid: the
+// kept output), and its column sums are the bias's gradient.
+template <typename T>
+__device__ inline void load8(const T* p, float* v);
+template <>
+__device__ inline void load8<float>(const float* p, float* v) {
+  f32x4 a = *reinterpret_cast<const f32x4*>(p);
+  f32x4 b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    v[c] = a[c];
+    v[4 + c] = b[c];
+  }
+}
+template <>
+__device__ inline void load8<__bf16>(const __bf16* p, float* v) {
+  bf16x8 a = *reinterpret_cast<const bf16x8*>(p);
+#pragma unroll
+  for (int c = 0; c < 8; ++c) v[c] = (float)a[c];
+}
+template <>
+__device__ inline void load8<_Float16>(const _Float16* p, float* v) {
+  f16x8 a = *reinterpret_cast<const f16x8*>(p);
+#pragma unroll
+  for (int c = 0; c < 8; ++c) v[c] = (float)a[c];
+}
+
+// 8 values of row r from column c; zeros outside the matrix
+template <typename T>
+__device__ inline void load_row8(const T* x, int64_t ld, int64_t R, int64_t C,
+                                 int64_t r, int64_t c, bool wide, float* v) {
+  const T* p = x + r * ld + c;
+  if (r < R && c + 8 <= C && wide) {
+    load8<T>(p, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      v[k] = (r < R && c + k < C) ? as_f32(p[k]) : 0.f;
+  }
+}
+
+constexpr int kLdsRow = 144;  // a transposed row: 128 bytes and 16 of padding
+
+template <typename T, bool COLS, bool TILE, bool DERIV>
+__global__ __launch_bounds__(256) void quantize_kernel(edl_fp8_quant a) {
+  __shared__ uint32_t s_max[4][kBlk];
+  __shared__ float s_sum[4][kBlk];
+  __shared__ __align__(16) uint8_t s_t[COLS ? kBlk * kLdsRow : 16];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int j = tid & 15;  // columns j*8 .. j*8+7
+  const int i = tid >> 4;  // rows    i*8 .. i*8+7
+  const int64_t ncb = (a.C + kBlk - 1) / kBlk;
+  const int64_t rb = blockIdx.x / ncb, cb = blockIdx.x % ncb;
+  const int64_t r0 = rb * kBlk + i * 8, c0 = cb * kBlk + j * 8;
+
+  float v[8][8];
+#pragma unroll
+  for (int r = 0; r < 8; ++r)
+    load_row8<T>(static_cast<const T*>(a.x), a.ld, a.R, a.C, r0 + r, c0,
+                 a.wide, v[r]);
+
+  if (DERIV) {
+    if (a.act == EDL_ACT_RELU) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        uint32_t bits = 0;
+        if (r0 + r < a.R && c0 < a.C)
+          bits = a.mask[(r0 + r) * a.mask_ld + (c0 >> 3)];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[r][c] = (bits >> c) & 1 ? v[r][c] : 0.f;
+      }
+    } else if (a.act == EDL_ACT_SIGMOID) {
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        float o[8];
+        load_row8<T>(static_cast<const T*>(a.y), a.y_ld, a.R, a.C, r0 + r, c0,
+                     a.y_wide, o);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[r][c] = v[r][c] * o[c] * (1.f - o[c]);
+      }
+    }
+    if (a.sums) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        float s = 0.f;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) s += v[r][c];
+        s += __shfl_xor(s, 16);
+        s += __shfl_xor(s, 32);
+        if (lane < 16) s_sum[wave][j * 8 + c] = s;
+      }
+    }
+  }
+
+  uint32_t rmax[8], cmax[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) rmax[k] = cmax[k] = 0;
+#pragma unroll
+  for (int r = 0; r < 8; ++r)
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      uint32_t m = finite_abs(v[r][c]);
+      rmax[r] = max(rmax[r], m);
+      cmax[c] = max(cmax[c], m);
+    }
+  if (!TILE) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) rmax[r] = max16(rmax[r]);
+  }
+  if (COLS || TILE) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      uint32_t m = cmax[c];
+      m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+      m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+      if (lane < 16) s_max[wave][j * 8 + c] = m;
+    }
+  }
+  if (COLS || TILE || (DERIV && a.sums)) __syncthreads();
+
+  if (COLS || TILE) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      int col = j * 8 + c;
+      cmax[c] = max(max(s_max[0][col], s_max[1][col]),
+                    max(s_max[2][col], s_max[3][col]));
+    }
+  }
+  if (TILE) {  // one scale for all of it
+    uint32_t m = cmax[0];
+#pragma unroll
+    for (int c = 1; c < 8; ++c) m = max(m, cmax[c]);
+    m = max16(m);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) rmax[k] = cmax[k] = m;
+  }
+  if (DERIV && a.sums && tid < kBlk) {
+    int64_t c = cb * kBlk + tid;
+    if (c < a.C)
+      a.sums[rb * a.C + c] =
+          (s_sum[0][tid] + s_sum[1][tid]) + (s_sum[2][tid] + s_sum[3][tid]);
+  }
+
+  if (a.rows) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      int b = scale_byte(rmax[r]);
+      float inv = inverse_of(b);
+      if (j == 0) a.rows_scale[cb * a.rows_rp + scale_slot(r0 + r)] = b;
+      if (r0 + r < a.R) {
+        i32x2 q;
+        q[0] = pack4(v[r][0], v[r][1], v[r][2], v[r][3], inv);
+        q[1] = pack4(v[r][4], v[r][5], v[r][6], v[r][7], inv);
+        *reinterpret_cast<i32x2*>(a.rows + (r0 + r) * a.rows_ld + c0) = q;
+      }
+    }
+  }
+  if (COLS) {
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      int b = scale_byte(cmax[c]);
+      float inv = inverse_of(b);
+      if (i == 0) a.cols_scale[rb * a.cols_rp + scale_slot(c0 + c)] = b;
+      i32x2 q;
+      q[0] = pack4(v[0][c], v[1][c], v[2][c], v[3][c], inv);
+      q[1] = pack4(v[4][c], v[5][c], v[6][c], v[7][c], inv);
+      *reinterpret_cast<i32x2*>(s_t + (j * 8 + c) * kLdsRow + i * 8) = q;
+    }
+    __syncthreads();
+    // 8 lanes write a transposed row's 128 bytes together
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      int col = s * 32 + (tid >> 3), part = (tid & 7) * 16;
+      int64_t c = cb * kBlk + col;
+      if (c < a.C)
+        *reinterpret_cast<i32x4*>(a.cols + c * a.cols_ld + rb * kBlk + part) =
+            *reinterpret_cast<const i32x4*>(s_t + col * kLdsRow + part);
+    }
+  }
+}
+
+// out[c] = sum over the tiles of sums[t][c], in order of t within each of 16
+// lanes' share, the shares then in order
+__global__ __launch_bounds__(256) void column_sums_kernel(
+    const float* __restrict__ sums, int64_t tiles, int64_t C, void* out,
+    int type) {
+  __shared__ float s[16][17];
+  const int c = threadIdx.x & 15, k = threadIdx.x >> 4;
+  const int64_t col = (int64_t)blockIdx.x * 16 + c;
+  float t = 0.f;
+  if (col < C)
+    for (int64_t r = k; r < tiles; r += 16) t += sums[r * C + col];
+  s[k][c] = t;
+  __syncthreads();
+  if (k == 0 && col < C) {
+    float u = 0.f;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) u += s[q][c];
+    store_any(out, col, u, type);
+  }
+}
+
+// --------------------------------- product --------------------------------
+// C[m, n] = act(sum over blocks of 128 of sa[m] sb[n] sum_k A[m, k] B[n, k]
+//               + bias[n])
+//
+// A workgroup takes WM*FM*16 x WN*FN*16 of C and a wave FM*16 x FN*16; a
+// step is one block of 128. Both tiles pass through two buffers of LDS,
+// filled by global_load_lds. A row's 128 bytes are eight 16-byte chunks,
+// and chunk c of row r lies at slot c ^ swz(r), which is free of bank
+// conflicts both ways.
+//
+// A fragment's 16 rows are not neighbours: row rr of fragment f is row
+// (rr>>2)*16 + f*4 + (rr&3) of its 64. B goes in as the instruction's first
+// operand, so that a lane's results are one row of C and, over the four
+// fragments, 16 neighbours of it: one or two wide stores, and one 16-bit
+// word of the relu mask.
+//
+// In a step each wave reads its fragments of A two ahead of the
+// instructions that use them. Once a wave has read its last fragment and
+// the next tile has landed, one barrier hands the buffer over; the
+// instructions on the last two fragments cover the first reads of the next
+// step.
+__device__ inline int swz(int r) { return (r & 3) | ((r >> 2) & 4); }
+
+__device__ inline int xcd_order(int bid, int n) {
+  // workgroups go to the 8 XCDs in turn; give each XCD a run of neighbours
+  if (n < 8) return bid;
+  int xcd = bid & 7, idx = bid >> 3, q = n >> 3, r = n & 7;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+}
+
+// Memory to LDS without registers: lane l's bytes land at m0 + l * size. The
+// address is a buffer's base + the lane's offset + a scalar, so the loop over
+// the blocks keeps no 64-bit addresses. Written as assembly because the
+// compiler would wait for these loads before any read of LDS that it cannot
+// tell from their target, and the two buffers differ at run time only; there
+// is no output register, and the loop waits (vmcnt) before each barrier.
+__device__ inline i32x4 buffer_of(const uint8_t* p, int64_t bytes) {
+  const uint64_t base = (uint64_t)p;
+  const int64_t most = 0xffffffffll;
+  return (i32x4){(int)(uint32_t)base, (int)(uint32_t)(base >> 32),
+                 (int)(uint32_t)(bytes < most ? bytes : most), 0x00027000};
+}
+__device__ inline void dma16(i32x4 src, uint32_t lane_off, uint32_t off,
+                             uint32_t dst) {
+  asm volatile(
+      "s_mov_b32 m0, %3\n\ts_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %0, %2 offen lds" ::"s"(src),
+      "v"(lane_off), "s"(off), "s"(dst)
+      : "memory", "m0");
+}
+__device__ inline void dma4(i32x4 src, uint32_t lane_off, uint32_t off,
+                            uint32_t dst) {
+  asm volatile(
+      "s_mov_b32 m0, %3\n\ts_nop 0\n\t"
+      "buffer_load_dword %1, %0, %2 offen lds" ::"s"(src),
+      "v"(lane_off), "s"(off), "s"(dst)
+      : "memory", "m0");
+}
+
+template <int OPA, int OPB>
+__device__ inline f32x4 mfma(i32x8 a, i32x8 b, f32x4 c, int sa, int sb) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, OPA,
+                                                          sa, OPB, sb);
+}
+// f: which byte of the scale words; all calls are unrolled to constants
+__device__ inline f32x4 mfma_sel(int fa, int fb, i32x8 a, i32x8 b, f32x4 c,
+                                 int sa, int sb) {
+#define EDL_SEL(X, Y) \
+  if (fa == X && fb == Y) return mfma<X, Y>(a, b, c, sa, sb);
+  EDL_SEL(0, 0) EDL_SEL(0, 1) EDL_SEL(0, 2) EDL_SEL(0, 3)
+  EDL_SEL(1, 0) EDL_SEL(1, 1) EDL_SEL(1, 2) EDL_SEL(1, 3)
+  EDL_SEL(2, 0) EDL_SEL(2, 1) EDL_SEL(2, 2) EDL_SEL(2, 3)
+  EDL_SEL(3, 0) EDL_SEL(3, 1) EDL_SEL(3, 2)
+  return mfma<3, 3>(a, b, c, sa, sb);
+#undef EDL_SEL
+}
+
+// ---- in 32 bits: a fragment's 32 bytes as four of 8 bf16, times its scale
+struct Wide {
+  bf16x8 v[4];
+};
+__device__ inline float scale_value(int word, int f) {
+  return __uint_as_float((((uint32_t)word >> (8 * f)) & 0xffu) << 23);
+}
+__device__ inline Wide widen(i32x8 q, float s) {
+  Wide w;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    bf16x2 lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[k], s, false);
+    bf16x2 hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[k], s, true);
+    const int o = (k & 1) * 4;
+    w.v[k >> 1][o] = lo[0];
+    w.v[k >> 1][o + 1] = lo[1];
+    w.v[k >> 1][o + 2] = hi[0];
+    w.v[k >> 1][o + 3] = hi[1];
+  }
+  return w;
+}
+__device__ inline f32x4 mfma_wide(const Wide& a, const Wide& b, f32x4 c) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[k], b.v[k], c, 0, 0, 0);
+  return c;
+}
+
+// 16 neighbours of a row of C, from column n
+__device__ inline void epilogue16(const edl_fp8_gemm& g, int64_t m, int64_t n,
+                                  float* v) {
+  const int type = g.c_type;
+  if (g.bias) {
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (n + k < g.N) v[k] += load_any(g.bias, n + k, g.bias_type);
+  }
+  uint32_t bits = 0;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    bits |= (v[k] > 0.f ? 1u : 0u) << k;
+    v[k] = activate(v[k], g.act);
+  }
+  if (g.mask)
+    *reinterpret_cast<uint16_t*>(g.mask + m * g.mask_ld + (n >> 3)) = bits;
+  const int64_t at = m * g.N + n;
+  if (n + 16 <= g.N && g.c_wide) {
+    if (type == EDL_T_F32) {
+      float* p = static_cast<float*>(g.c) + at;
+#pragma unroll
+      for (int k = 0; k < 16; k += 4)
+        *reinterpret_cast<f32x4*>(p + k) =
+            (f32x4){v[k], v[k + 1], v[k + 2], v[k + 3]};
+    } else if (type == EDL_T_BF16) {
+      __bf16* p = static_cast<__bf16*>(g.c) + at;
+#pragma unroll
+      for (int k = 0; k < 16; k += 8) {
+        bf16x8 o;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) o[q] = (__bf16)v[k + q];
+        *reinterpret_cast<bf16x8*>(p + k) = o;
+      }
+    } else {
+      _Float16* p = static_cast<_Float16*>(g.c) + at;
+#pragma unroll
+      for (int k = 0; k < 16; k += 8) {
+        f16x8 o;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) o[q] = (_Float16)v[k + q];
+        *reinterpret_cast<f16x8*>(p + k) = o;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (n + k < g.N) store_any(g.c, at + k, v[k], type);
+  }
+}
+
+template <int WM, int WN, int FM, int FN, bool WIDE>
+__global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(
+    edl_fp8_gemm g) {
+  constexpr int BM = WM * FM * 16, BN = WN * FN * 16, NW = WM * WN;
+  static_assert(FN == 4 && FM % 4 == 0, "scale words hold four fragments");
+  static_assert(BM == BN && (BM == 128 || BM == 256), "buffers' toggle");
+  constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW;  // 1 KB loads a wave
+  // two buffers each: A's, B's, and the scales (256 of A's, 256 of B's)
+  constexpr uint32_t kTile = BM * kBlk, kB = 2 * kTile, kS = 4 * kTile;
+  __shared__ __align__(1024) uint8_t smem[4 * kTile + 1024];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+
+  // tiles in groups of 4 rows of tiles, column by column
+  const int ntm = (g.M + BM - 1) / BM, ntn = (g.N + BN - 1) / BN;
+  int bid = xcd_order(blockIdx.x, ntm * ntn);
+  const int per = 4 * ntn, grp = bid / per, in = bid % per;
+  const int tall = min(4, ntm - grp * 4);
+  const int64_t m0 = (int64_t)(grp * 4 + in % tall) * BM;
+  const int64_t n0 = (int64_t)(in / tall) * BN;
+
+  // this split's share of the steps
+  const int kb_all = (int)(g.ld / kBlk);
+  const int split = blockIdx.y;
+  const int kb0 = (int)((int64_t)kb_all * split / g.splits);
+  const int T = (int)((int64_t)kb_all * (split + 1) / g.splits) - kb0;
+
+  // one load fills 8 rows: lane -> row lane>>3, slot lane&7
+  const uint8_t* pa = g.a + m0 * g.ld + (int64_t)kb0 * kBlk;
+  const uint8_t* pb = g.b + n0 * g.ld + (int64_t)kb0 * kBlk;
+  const i32x4 bufA = buffer_of(pa, g.a + g.M * g.ld - pa);
+  const i32x4 bufB = buffer_of(pb, g.b + g.N * g.ld - pb);
+  uint32_t offA[LA], offB[LB];
+  const uint32_t lastA = (uint32_t)min(g.M - 1 - m0, (int64_t)BM);
+  const uint32_t lastB = (uint32_t)min(g.N - 1 - n0, (int64_t)BN);
+#pragma unroll
+  for (int q = 0; q < LA; ++q) {
+    uint32_t r = (wave * LA + q) * 8 + (lane >> 3);
+    offA[q] = min(r, lastA) * (uint32_t)g.ld + (((lane & 7) ^ swz(r)) << 4);
+  }
+#pragma unroll
+  for (int q = 0; q < LB; ++q) {
+    uint32_t r = (wave * LB + q) * 8 + (lane >> 3);
+    offB[q] = min(r, lastB) * (uint32_t)g.ld + (((lane & 7) ^ swz(r)) << 4);
+  }
+  // scales: 256 bytes a load, A's by even waves and B's by odd ones (several
+  // fetch the same; a branch would cost more)
+  const bool odd = wave & 1;
+  const int64_t rp = odd ? g.b_rp : g.a_rp;
+  const uint8_t* ps = (odd ? g.sb + n0 : g.sa + m0) + kb0 * rp;
+  const i32x4 bufS =
+      buffer_of(ps, (odd ? g.sb : g.sa) + (int64_t)kb_all * rp - ps);
+  const uint32_t lds0 =
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+  uint32_t at = 0, atS = 0;
+  auto stage = [&](uint32_t buf) {  // the next block
+#pragma unroll
+    for (int q = 0; q < LA; ++q)
+      dma16(bufA, offA[q], at, lds0 + buf * kTile + (wave * LA + q) * 1024);
+#pragma unroll
+    for (int q = 0; q < LB; ++q)
+      dma16(bufB, offB[q], at,
+            lds0 + kB + buf * kTile + (wave * LB + q) * 1024);
+    dma4(bufS, lane * 4, atS, lds0 + kS + buf * 512 + odd * 256);
+    at += kBlk;
+    atS += (uint32_t)rp;
+  };
+
+  // fragment f of a wave's rows: 32 bytes of row rr, in chunks q4 and 4 + q4.
+  // Which bytes of a block meet is the same for A and B, and a block has one
+  // scale, so the order within it does not matter. f*4 leaves swz as it is.
+  const int rr = ((lane & 15) >> 2) * 16 + (lane & 3), q4 = lane >> 4;
+  const uint32_t lo = rr * kBlk + ((q4 ^ swz(rr)) << 4);
+  const uint32_t hi = rr * kBlk + (((q4 + 4) ^ swz(rr)) << 4);
+  const int wA = wm * FM * 16, wB = wn * FN * 16;
+  // these move to the other buffer and back with a step
+  uint32_t aLo = wA * kBlk + lo, aHi = wA * kBlk + hi;
+  uint32_t bLo = kB + wB * kBlk + lo, bHi = kB + wB * kBlk + hi;
+  uint32_t sAt = kS + (lane & 15) * 4;
+  auto frag = [&](uint32_t x, uint32_t y, int f) -> i32x8 {
+    const int o = ((f >> 2) * 64 + (f & 3) * 4) * kBlk;
+    i32x4 u = *reinterpret_cast<const i32x4*>(smem + x + o);
+    i32x4 v = *reinterpret_cast<const i32x4*>(smem + y + o);
+    return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+
+  f32x4 acc[FM][FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int k = 0; k < FN; ++k) acc[i][k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+  i32x8 a[FM], b[FN];
+  int sa[FM / 4], sb, na[FM / 4], nb;
+  auto read_scales = [&]() {
+#pragma unroll
+    for (int k = 0; k < FM / 4; ++k)
+      na[k] = *reinterpret_cast<const int*>(smem + sAt + wA + k * 64);
+    nb = *reinterpret_cast<const int*>(smem + sAt + 256 + wB);
+  };
+  Wide bw[WIDE ? FN : 1];
+  auto widen_b = [&]() {
+#pragma unroll
+    for (int k = 0; k < FN; ++k) bw[k] = widen(b[k], scale_value(sb, k));
+  };
+  auto rows_of = [&](int i) {  // fragment i of A against all of B
+    if (WIDE) {
+      const Wide aw = widen(a[i], scale_value(sa[i >> 2], i & 3));
+#pragma unroll
+      for (int k = 0; k < FN; ++k) acc[i][k] = mfma_wide(bw[k], aw, acc[i][k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < FN; ++k)
+        acc[i][k] =
+            mfma_sel(k, i & 3, b[k], a[i], acc[i][k], sb, sa[i >> 2]);
+    }
+  };
+  auto step = [&](uint32_t buf, bool more) {
+    if (WIDE) widen_b();
+#pragma unroll
+    for (int i = 0; i < FM - 2; ++i) {
+      a[i + 2] = frag(aLo, aHi, i + 2);
+      rows_of(i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    if (more) stage(buf);
+    aLo ^= kTile;
+    aHi ^= kTile;
+    bLo ^= kTile;
+    bHi ^= kTile;
+    sAt ^= 512;
+    // after the last step these read a buffer that nobody writes any more
+    read_scales();
+    a[0] = frag(aLo, aHi, 0);
+    a[1] = frag(aLo, aHi, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    if (WIDE) {
+#pragma unroll
+      for (int k = 0; k < FN; ++k) b[k] = frag(bLo, bHi, k);
+      __builtin_amdgcn_sched_barrier(0);
+      rows_of(FM - 2);
+      rows_of(FM - 1);
+    } else {
+#pragma unroll
+      for (int k = 0; k < FN; ++k) {
+#pragma unroll
+        for (int i = FM - 2; i < FM; ++i)
+          acc[i][k] =
+              mfma_sel(k, i & 3, b[k], a[i], acc[i][k], sb, sa[i >> 2]);
+        __builtin_amdgcn_sched_barrier(0);
+        b[k] = frag(bLo, bHi, k);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < FM / 4; ++k) sa[k] = na[k];
+    sb = nb;
+  };
+
+  stage(0);
+  if (T > 1) stage(1);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  read_scales();
+#pragma unroll
+  for (int k = 0; k < FM / 4; ++k) sa[k] = na[k];
+  sb = nb;
+  a[0] = frag(aLo, aHi, 0);
+  a[1] = frag(aLo, aHi, 1);
+#pragma unroll
+  for (int k = 0; k < FN; ++k) b[k] = frag(bLo, bHi, k);
+  // the last two steps fetch no more; a branch in the loop's body would let
+  // the compiler move matrix instructions behind the barrier
+  int t = 0;
+  for (; t + 2 < T; ++t) step(t & 1, true);
+  for (; t < T; ++t) step(t & 1, false);
+
+  // lane: row rr + 4 i of C's 64, columns q4*16 + k*4 + 0..3
+  const int64_t n = n0 + wn * FN * 16 + q4 * 16;
+  if (n >= g.N) return;
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    int64_t m = m0 + wm * FM * 16 + (i >> 2) * 64 + rr + (i & 3) * 4;
+    if (m >= g.M) continue;
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = acc[i][k >> 2][k & 3];
+    if (g.splits > 1) {
+      float* p = g.part + ((int64_t)split * g.M + m) * g.part_ld + n;
+#pragma unroll
+      for (int k = 0; k < 16; k += 4)
+        *reinterpret_cast<f32x4*>(p + k) =
+            (f32x4){v[k], v[k + 1], v[k + 2], v[k + 3]};
+    } else {
+      epilogue16(g, m, n, v);
+    }
+  }
+}
+
+// joins the splits in order; a thread takes 16 neighbours of a row
+__global__ __launch_bounds__(256) void gemm_join_kernel(edl_fp8_gemm g) {
+  const int64_t each = g.part_ld / 16;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= g.M * each) return;
+  const int64_t m = id / each, n = (id % each) * 16;
+  float v[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) v[k] = 0.f;
+  for (int s = 0; s < g.splits; ++s) {
+    const float* p = g.part + ((int64_t)s * g.M + m) * g.part_ld + n;
+#pragma unroll
+    for (int k = 0; k < 16; k += 4) {
+      f32x4 u = *reinterpret_cast<const f32x4*>(p + k);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[k + q] += u[q];
+    }
+  }
+  epilogue16(g, m, n, v);
+}
+
+// ------------------------------- few rows ---------------------------------
+// At most 16 rows of x, as served requests come: x is quantised in the
+// registers of the wave that multiplies it and the weights go from memory
+// straight to the matrix instruction, so that a layer is one launch. A
+// workgroup takes 16 columns; its 8 waves share the blocks of 128 between
+// them and join through LDS in order. Bound by the read of the weights.
+constexpr int kFewWaves = 8;
+
+template <typename T>
+__global__ __launch_bounds__(kFewWaves * 64) void few_rows_kernel(
+    edl_fp8_gemm g, const T* __restrict__ x, int64_t x_ld, int K, bool wide) {
+  __shared__ f32x4 s[kFewWaves][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row = lane & 15, q4 = lane >> 4;
+  const int64_t n0 = (int64_t)blockIdx.x * 16;
+  const int64_t n = n0 + row < g.N ? n0 + row : g.N - 1;
+  const int kbs = (int)(g.ld / kBlk);
+  const uint8_t* pb = g.b + n * g.ld + q4 * 32;
+  const uint8_t* ps = g.sb + scale_slot(n);
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+  for (int kb = wave; kb < kbs; kb += kFewWaves) {
+    i32x8 b = *reinterpret_cast<const i32x8*>(pb + (int64_t)kb * kBlk);
+    int sb = ps[(int64_t)kb * g.b_rp];
+    float v[32];
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 32; k += 8)
+      load_row8<T>(x, x_ld, g.M, K, row, (int64_t)kb * kBlk + q4 * 32 + k,
+                   wide, v + k);
+#pragma unroll
+    for (int k = 0; k < 32; ++k) m = max(m, finite_abs(v[k]));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+    const int sa = scale_byte(m);
+    const float inv = inverse_of(sa);
+    i32x8 a;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      a[k] = pack4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3], inv);
+    if (sizeof(T) == 4)  // the result is in 32 bits
+      acc = mfma_wide(widen(b, scale_value(sb, 0)),
+                      widen(a, scale_value(sa, 0)), acc);
+    else
+      acc = mfma<0, 0>(b, a, acc, sb, sa);
+  }
+  s[wave][lane] = acc;
+  __syncthreads();
+  if (wave != 0) return;
+  // lane: row `row` of C, columns n0 + q4*4 + 0..3
+  f32x4 t = s[0][lane];
+#pragma unroll
+  for (int w = 1; w < kFewWaves; ++w) {
+    f32x4 u = s[w][lane];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) t[q] += u[q];
+  }
+  if (row >= g.M) return;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    int64_t c = n0 + q4 * 4 + q;
+    if (c >= g.N) continue;
+    float z = t[q];
+    if (g.bias) z += load_any(g.bias, c, g.bias_type);
+    store_any(g.c, row * g.N + c, activate(z, g.act), g.c_type);
+  }
+}
+
+template <typename T>
+void launch_quantize(const edl_fp8_quant& a, hipStream_t st) {
+  const int64_t tiles =
+      ((a.R + kBlk - 1) / kBlk) * ((a.C + kBlk - 1) / kBlk);
+  dim3 grid((unsigned)tiles), block(256);
+  const bool cols = a.cols != nullptr;
+  if (a.tile) {
+    if (cols)
+      quantize_kernel<T, true, true, false><<<grid, block, 0, st>>>(a);
+    else
+      quantize_kernel<T, false, true, false><<<grid, block, 0, st>>>(a);
+  } else if (a.deriv) {
+    if (cols)
+      quantize_kernel<T, true, false, true><<<grid, block, 0, st>>>(a);
+    else
+      quantize_kernel<T, false, false, true><<<grid, block, 0, st>>>(a);
+  } else {
+    if (cols)
+      quantize_kernel<T, true, false, false><<<grid, block, 0, st>>>(a);
+    else
+      quantize_kernel<T, false, false, false><<<grid, block, 0, st>>>(a);
+  }
+}
+
+}  // namespace
+
+extern "C" int edl_fp8_quantize(const edl_fp8_quant* a, hipStream_t st) {
+  if (a->type == EDL_T_F32)
+    launch_quantize<float>(*a, st);
+  else if (a->type == EDL_T_BF16)
+    launch_quantize<__bf16>(*a, st);
+  else
+    launch_quantize<_Float16>(*a, st);
+  return (int)hipGetLastError();
+}
+
+extern "C" int edl_fp8_column_sums(const float* sums, int64_t tiles, int64_t C,
+                                   void* out, int type, hipStream_t st) {
+  column_sums_kernel<<<dim3((unsigned)((C + 15) / 16)), dim3(256), 0, st>>>(
+      sums, tiles, C, out, type);
+  return (int)hipGetLastError();
+}
+
+// Which tile, and how many splits. 256 x 256 reads each operand half as
+// often but runs one workgroup a CU, so it takes the products that give each
+// of the 256 CUs one; 128 x 128 takes the rest, split over the contraction
+// until there are 512 workgroups (two a CU) or four blocks are left to each.
+// In 32 bits a wave's fragments take twice the registers: always 128 x 128.
+static bool in_32_bits(const edl_fp8_gemm* g) {
+  return g->c_type == EDL_T_F32 || g->mask != nullptr;
+}
+static bool takes_256(const edl_fp8_gemm* g) {
+  return !in_32_bits(g) && ((g->M + 255) / 256) * ((g->N + 255) / 256) >= 256;
+}
+
+extern "C" int edl_fp8_gemm_splits(const edl_fp8_gemm* g) {
+  if (takes_256(g)) return 1;
+  const int64_t tiles = ((g->M + 127) / 128) * ((g->N + 127) / 128);
+  int64_t s = 512 / tiles, most = g->ld / kBlk / 4;
+  if (s > most) s = most;
+  if (s > 64) s = 64;
+  return s < 1 ? 1 : (int)s;
+}
+
+extern "C" int edl_fp8_gemm_run(const edl_fp8_gemm* g, hipStream_t st) {
+  if (takes_256(g)) {
+    const int64_t big = ((g->M + 255) / 256) * ((g->N + 255) / 256);
+    gemm_kernel<2, 4, 8, 4, false>
+        <<<dim3((unsigned)big, 1), dim3(512), 0, st>>>(*g);
+    return (int)hipGetLastError();
+  }
+  const int64_t tiles = ((g->M + 127) / 128) * ((g->N + 127) / 128);
+  dim3 grid((unsigned)tiles, g->splits), block(256);
+  if (in_32_bits(g))
+    gemm_kernel<2, 2, 4, 4, true><<<grid, block, 0, st>>>(*g);
+  else
+    gemm_kernel<2, 2, 4, 4, false><<<grid, block, 0, st>>>(*g);
+  int rc = (int)hipGetLastError();
+  if (rc != 0 || g->splits == 1) return rc;
+  const int64_t n = g->M * (g->part_ld / 16);
+  gemm_join_kernel<<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st>>>(
+      *g);
+  return (int)hipGetLastError();
+}
+
+extern "C" int edl_fp8_few_rows(const edl_fp8_gemm* g, const void* x,
+                                int64_t x_ld, int K, int x_type, int wide,
+                                hipStream_t st) {
+  dim3 grid((unsigned)((g->N + 15) / 16)), block(kFewWaves * 64);
+  if (x_type == EDL_T_F32)
+    few_rows_kernel<float><<<grid, block, 0, st>>>(
+        *g, static_cast<const float*>(x), x_ld, K, wide);
+  else if (x_type == EDL_T_BF16)
+    few_rows_kernel<__bf16><<<grid, block, 0, st>>>(
+        *g, static_cast<const __bf16*>(x), x_ld, K, wide);
+  else
+    few_rows_kernel<_Float16><<<grid, block, 0, st>>>(
+        *g, static_cast<const _Float16*>(x), x_ld, K, wide);
+  return (int)hipGetLastError();
+}

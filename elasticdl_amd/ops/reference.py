@@ -287,3 +287,97 @@ def gather_rows(arena: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
 
 def scatter_rows(arena: torch.Tensor, slots: torch.Tensor, rows: torch.Tensor):
     arena.index_copy_(0, slots.long(), rows)
+
+
+# ------------------------ 8-bit dense layers ------------------------------
+# e4m3 with a power-of-two scale for each block of 128; bytes and scales are
+# laid out as by quantize_kernel in fp8_kernels.hip, bit for bit.
+FP8_BLOCK = 128
+
+
+def fp8_scale_slots(rows: int, device=None) -> torch.Tensor:
+    """Where each row's scale byte lies within its block's row of bytes."""
+    r = torch.arange(rows, device=device)
+    n = r & 63
+    return (r & ~63) + (n >> 4) * 16 + (n & 3) * 4 + ((n >> 2) & 3)
+
+
+def _fp8_blocks(x: torch.Tensor, tile: bool):
+    """(x padded to whole blocks, in f32, as [blocks down, 128 or 1, blocks
+    across, 128]; each block's exponent: the smallest e with
+    max|finite x| <= 448 * 2^e, at least -126)."""
+    r, c = x.shape
+    down = -r % FP8_BLOCK if tile else 0
+    v = torch.nn.functional.pad(x.float(), (0, -c % FP8_BLOCK, 0, down))
+    h = FP8_BLOCK if tile else 1
+    v = v.reshape(v.shape[0] // h, h, v.shape[1] // FP8_BLOCK, FP8_BLOCK)
+    finite = torch.where(torch.isfinite(v), v.abs(), torch.zeros_like(v))
+    f, e = torch.frexp(finite.amax((1, 3), keepdim=True))
+    # amax = f * 2^e with f in [0.5, 1), and 448 = 0.875 * 2^9
+    e = torch.where(f <= 0.875, e - 9, e - 8).clamp_(min=-126)
+    return v, torch.where(f == 0, torch.full_like(e, -126), e)
+
+
+def fp8_quantize(x: torch.Tensor, tile: bool):
+    """(bytes [rows, cols up to 128], scales [blocks, rows up to 256])."""
+    r, c = x.shape
+    blocks = -(-c // FP8_BLOCK)
+    scale = torch.zeros(blocks, -(-r // 256) * 256, dtype=torch.uint8,
+                        device=x.device)
+    if r == 0:
+        return (torch.zeros(0, blocks * FP8_BLOCK, dtype=torch.uint8,
+                            device=x.device), scale)
+    v, e = _fp8_blocks(x, tile)
+    q = torch.ldexp(v, -e).to(torch.float8_e4m3fn).view(torch.uint8)
+    q = torch.where(torch.isfinite(v), q, torch.full_like(q, 0xff))  # a NaN
+    q = q.reshape(-1, blocks * FP8_BLOCK)
+    b = (e + 127).to(torch.uint8).expand(-1, v.shape[1], -1, -1)
+    scale[:, fp8_scale_slots(r, x.device)] = \
+        b.reshape(-1, blocks)[:r].t()
+    return q[:r].contiguous(), scale
+
+
+def fp8_values(data: torch.Tensor, scale: torch.Tensor, cols: int):
+    """What bytes and scales stand for, in f32."""
+    r = data.shape[0]
+    e = scale[:, fp8_scale_slots(r, data.device)].t().int() - 127
+    v = data.view(torch.float8_e4m3fn).float().view(
+        r, data.shape[1] // FP8_BLOCK, FP8_BLOCK)
+    return torch.ldexp(v, e.unsqueeze(2)).reshape(data.shape)[:, :cols]
+
+
+def fp8_dense_fwd(x, wq, ws, bias, act, keep_x, keep_mask):
+    """(y, x^T's bytes, its scales, relu's mask)."""
+    k = x.shape[1]
+    z = fp8_values(*fp8_quantize(x, False), k) @ fp8_values(wq, ws, k).t()
+    if bias is not None:
+        z = z + bias.float()
+    y = torch.relu(z) if act == 1 else torch.sigmoid(z) if act == 2 else z
+    xtq = xts = None
+    if keep_x:
+        xtq, xts = fp8_quantize(x.t(), False) if x.shape[0] else (
+            torch.zeros(k, 0, dtype=torch.uint8),
+            torch.zeros(0, -(-k // 256) * 256, dtype=torch.uint8))
+    return y.to(x.dtype), xtq, xts, (z > 0) if keep_mask else None
+
+
+def fp8_dense_bwd(dy, act, mask, y, wtq, wts, xtq, xts, k, need_dx, need_dw,
+                  need_db, w_dtype, b_dtype):
+    """(dx, dw, db), each where it is asked for."""
+    m, n = dy.shape
+    dz = dy.float()
+    if act == 1:
+        dz = torch.where(mask, dz, torch.zeros_like(dz))
+    elif act == 2:
+        dz = dz * y.float() * (1 - y.float())
+    dx = dw = None
+    if need_dx:
+        dx = (fp8_values(*fp8_quantize(dz, False), n)
+              @ fp8_values(wtq, wts, n).t()).to(dy.dtype)
+    if need_dw:
+        if m:
+            dw = (fp8_values(*fp8_quantize(dz.t(), False), m)
+                  @ fp8_values(xtq, xts, m).t()).to(w_dtype)
+        else:
+            dw = torch.zeros(n, k, dtype=w_dtype)
+    return dx, dw, dz.sum(0).to(b_dtype) if need_db else None
