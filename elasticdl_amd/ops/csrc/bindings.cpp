@@ -571,10 +571,12 @@ void fused_adamw_bf16(torch::Tensor p, torch::Tensor master, torch::Tensor m,
 }  // namespace
 
 void edl_bind_fp8(py::module& m);
+void edl_bind_embedding(py::module& m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "elasticdl_amd MI355X kernels";
   edl_bind_fp8(m);
+  edl_bind_embedding(m);
   m.def("dense_sgd", &dense_sgd);
   m.def("dense_momentum", &dense_momentum);
   m.def("dense_adam", &dense_adam);

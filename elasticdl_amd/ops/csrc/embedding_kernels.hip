@@ -1,0 +1,995 @@
+// Embedding lookup with scaling and pooling, and its gradient by sorted ids,
+// for MI355X (gfx950, CDNA4).
+//
+//   out[b]    = T(c[b] * sum over l of w[b,l] * table[ids[b,l]])
+//   dw[b,l]   = c[b] * <table[ids[b,l]], dy[b]>
+//   dtable[v] = T(sum over (b,l) with ids[b,l] = v of c[b] * w[b,l] * dy[b])
+//
+// with c[b] = scale / norm, norm 1, n or sqrt(n) for n ids in bag b. Ids
+// below zero are no tokens; ids past the table make their output NaN and
+// have no gradient. Sums are in 32 bits, in an order that the inputs alone
+// decide: no atomic adds to a sum.
+//
+// All of it moves rows, so it is bound by memory, or by launches where there
+// are few tokens.
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "embedding_kernels.h"
+
+namespace {
+
+constexpr uint32_t kNone = 0xffffffffu;
+
+__device__ inline float as_f32(float v) { return v; }
+__device__ inline float as_f32(__bf16 v) { return (float)v; }
+__device__ inline float as_f32(_Float16 v) { return (float)v; }
+
+__device__ inline float load_any(const void* p, int64_t i, int type) {
+  if (type == EDL_T_F32) return static_cast<const float*>(p)[i];
+  if (type == EDL_T_BF16) return (float)static_cast<const __bf16*>(p)[i];
+  return (float)static_cast<const _Float16*>(p)[i];
+}
+
+template <typename T, int N>
+struct Vec {
+  typedef T type __attribute__((ext_vector_type(N)));
+  type v;
+  __device__ float get(int i) const { return as_f32(v[i]); }
+  __device__ void set(int i, float x) { v[i] = (T)x; }
+};
+template <typename T>
+struct Vec<T, 1> {
+  T v;
+  __device__ float get(int) const { return as_f32(v); }
+  __device__ void set(int, float x) { v = (T)x; }
+};
+
+__device__ inline int64_t load_id(const void* ids, bool wide, int64_t i) {
+  return wide ? static_cast<const int64_t*>(ids)[i]
+              : (int64_t)static_cast<const int32_t*>(ids)[i];
+}
+
+// lanes that share a row: a power of two, at most a wave
+__host__ __device__ inline int lanes_of(int D, int vec) {
+  int n = (D + vec - 1) / vec, l = 1;
+  while (l < n && l < 64) l <<= 1;
+  return l;
+}
+// a row's pieces of lanes_of() loads
+__host__ __device__ inline int pieces_of(int D, int vec) {
+  const int each = lanes_of(D, vec) * vec;
+  return (D + each - 1) / each;
+}
+
+// --------------------------------- lookup ---------------------------------
+// A row is read by the few lanes that its width takes, 8 ids at a time so
+// that 8 rows are in flight. SPLIT: a wave to a bag, its groups of lanes
+// taking every so-many-th eight, for calls with too few bags to fill the
+// chip otherwise.
+template <typename T, int VEC, bool SPLIT>
+__global__ __launch_bounds__(256) void lookup_kernel(edl_bag a) {
+  typedef Vec<T, VEC> V;
+  constexpr int U = 8;
+  const int lanes = lanes_of(a.D, VEC), pieces = pieces_of(a.D, VEC);
+  const int lane = threadIdx.x & 63;
+  const int sub = SPLIT ? lane / lanes : 0, subs = SPLIT ? 64 / lanes : 1;
+  const int64_t id0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t unit = SPLIT ? id0 >> 6 : id0 / lanes;
+  const int64_t bag = unit / pieces;
+  const int col = ((int)(unit % pieces) * lanes + (lane & (lanes - 1))) * VEC;
+  if (bag >= a.B) return;  // whole groups, and whole waves where SPLIT
+  const bool mine = col < a.D;
+  const int at = mine ? col : 0;
+  const T* table = static_cast<const T*>(a.table) + at;
+
+  float acc[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+  int count = 0;
+  for (int l0 = sub * U; l0 < a.L; l0 += subs * U) {
+    int64_t id[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      id[u] = l0 + u < a.L ? load_id(a.ids, a.ids64, bag * a.L + l0 + u) : -1;
+    bool any = false;
+#pragma unroll
+    for (int u = 0; u < U; ++u) any |= id[u] >= 0;
+    if (!__any(any)) continue;  // behind the ends of short bags
+    V row[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      row[u].v = *reinterpret_cast<const decltype(row[u].v)*>(
+          table + ((uint64_t)id[u] < (uint64_t)a.V ? id[u] : 0) * a.ld);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (id[u] < 0) continue;
+      ++count;
+      const float w =
+          a.weights ? load_any(a.weights, bag * a.L + l0 + u, a.w_type) : 1.f;
+      const float bad = id[u] < a.V ? 0.f : __uint_as_float(0x7fc00000u);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        acc[k] += bad == 0.f ? w * row[u].get(k) : bad;
+    }
+  }
+  if (SPLIT) {
+    for (int o = lanes; o < 64; o <<= 1) {
+      count += __shfl_xor(count, o);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] += __shfl_xor(acc[k], o);
+    }
+    if (sub != 0) return;
+  }
+  const float n = (float)(count > 1 ? count : 1);
+  float c = a.scale;
+  if (a.combiner == EDL_BAG_MEAN) c = a.scale / n;
+  if (a.combiner == EDL_BAG_SQRTN) c = a.scale / sqrtf(n);
+  if (a.coef && col == 0) a.coef[bag] = c;
+  if (!mine) return;
+  V o;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) o.set(k, acc[k] * c);
+  *reinterpret_cast<decltype(o.v)*>(static_cast<T*>(a.out) + bag * a.D + col) =
+      o.v;
+}
+
+// the weights' gradient: a group of lanes keeps its bag's dy (its first
+// piece; wider rows read the rest again) and goes over the ids
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void weight_grad_kernel(edl_bag a) {
+  typedef Vec<T, VEC> V;
+  constexpr int U = 4;
+  const int lanes = lanes_of(a.D, VEC);
+  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
+  const int l_lane = threadIdx.x & (lanes - 1);
+  // eight ids of a bag to a unit, so that long bags spread
+  const int eights = (a.L + 7) / 8;
+  const int64_t bag = unit / eights;
+  const int l0 = (int)(unit % eights) * 8;
+  if (bag >= a.B) return;
+  const T* dy = static_cast<const T*>(a.dy) + bag * a.D;
+  const T* table = static_cast<const T*>(a.table);
+  const float c = a.coef[bag];
+  for (int l = l0; l < l0 + 8 && l < a.L; l += U) {
+    int64_t id[U];
+    float dot[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      id[u] = l + u < a.L ? load_id(a.ids, a.ids64, bag * a.L + l + u) : -1;
+      dot[u] = 0.f;
+    }
+    for (int col = l_lane * VEC; col < a.D; col += lanes * VEC) {
+      V g, row[U];
+      g.v = *reinterpret_cast<const decltype(g.v)*>(dy + col);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        row[u].v = *reinterpret_cast<const decltype(row[u].v)*>(
+            table + ((uint64_t)id[u] < (uint64_t)a.V ? id[u] : 0) * a.ld +
+            col);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) dot[u] += row[u].get(k) * g.get(k);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      for (int o = 1; o < lanes; o <<= 1) dot[u] += __shfl_xor(dot[u], o);
+      if (l_lane == 0 && l + u < a.L)
+        a.dw[bag * a.L + l + u] =
+            (uint64_t)id[u] < (uint64_t)a.V ? dot[u] * c : 0.f;
+    }
+  }
+}
+
+// ---------------------------------- sort ----------------------------------
+// Least significant digit first, stable, up to 9 bits a pass. A pass counts
+// each tile's digits, adds the counts up by digit, and moves each tile's
+// items: ranked by the wave (ballots find equal digits), brought in order in
+// LDS, and written in runs. The first pass makes the keys from the ids.
+struct Keys32 {  // an id of a table of V rows; V where it has none
+  typedef uint32_t K;
+  const void* ids;
+  bool wide;
+  int64_t V;
+  __device__ K operator()(int64_t i) const {
+    const int64_t v = load_id(ids, wide, i);
+    return (uint64_t)v < (uint64_t)V ? (K)v : (K)V;
+  }
+};
+struct Keys32From {  // an id less the smallest, within 32 bits
+  typedef uint32_t K;
+  const int64_t* ids;
+  int64_t base;
+  __device__ K operator()(int64_t i) const {
+    return (K)((uint64_t)ids[i] - (uint64_t)base);
+  }
+};
+struct Keys64 {  // any id; the sign bit turned, so that the order is theirs
+  typedef uint64_t K;
+  const int64_t* ids;
+  __device__ K operator()(int64_t i) const {
+    return (uint64_t)ids[i] ^ 0x8000000000000000ull;
+  }
+};
+template <typename K_>
+struct KeysOf {  // what the pass before wrote
+  typedef K_ K;
+  const K* keys;
+  __device__ K operator()(int64_t i) const { return keys[i]; }
+};
+
+constexpr int kTile = EDL_SORT_TILE, kBins = EDL_SORT_BINS;
+constexpr int kItems = kTile / 256;
+
+template <typename S>
+__global__ __launch_bounds__(256) void sort_count_kernel(S src, int64_t N,
+                                                         int shift, int bits,
+                                                         int tiles,
+                                                         uint32_t* counts) {
+  __shared__ uint32_t h[kBins];
+  const int bins = 1 << bits;
+  for (int d = threadIdx.x; d < bins; d += 256) h[d] = 0;
+  __syncthreads();
+  const int64_t base = (int64_t)blockIdx.x * kTile;
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int64_t i = base + k * 256 + threadIdx.x;
+    if (i < N) atomicAdd(&h[(uint32_t)(src(i) >> shift) & (bins - 1)], 1u);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < bins; d += 256)
+    counts[(int64_t)d * tiles + blockIdx.x] = h[d];
+}
+
+// exclusive sum over the 256 threads, and the total
+__device__ inline uint32_t block_scan(uint32_t v, uint32_t* s4,
+                                      uint32_t* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t x = v;
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 63) s4[wave] = x;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < wave) before += s4[w];
+    all += s4[w];
+  }
+  __syncthreads();
+  *total = all;
+  return before + x - v;
+}
+
+// one digit's counts to offsets within the digit, and its total
+__global__ __launch_bounds__(256) void sort_offsets_kernel(uint32_t* counts,
+                                                           int tiles,
+                                                           uint32_t* totals) {
+  __shared__ uint32_t s4[4];
+  uint32_t* row = counts + (int64_t)blockIdx.x * tiles;
+  uint32_t run = 0;
+  for (int t0 = 0; t0 < tiles; t0 += 256) {
+    const int t = t0 + threadIdx.x;
+    const uint32_t v = t < tiles ? row[t] : 0;
+    uint32_t all;
+    const uint32_t x = block_scan(v, s4, &all);
+    if (t < tiles) row[t] = run + x;
+    run += all;
+  }
+  if (threadIdx.x == 0) totals[blockIdx.x] = run;
+}
+
+template <typename S, bool FIRST>
+__global__ __launch_bounds__(256) void sort_move_kernel(
+    S src, const uint32_t* __restrict__ pos_in, int64_t N, int shift, int bits,
+    int tiles, const uint32_t* __restrict__ counts,
+    const uint32_t* __restrict__ totals, typename S::K* __restrict__ keys_out,
+    uint32_t* __restrict__ pos_out) {
+  typedef typename S::K K;
+  __shared__ K s_key[kTile];
+  __shared__ uint32_t s_pos[kTile];
+  __shared__ uint32_t cnt[4][kBins];
+  __shared__ uint32_t local[kBins];  // a digit's first place in the tile
+  __shared__ uint32_t goal[kBins];   // where it goes, less that place
+  __shared__ uint32_t s4[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int bins = 1 << bits;
+  const int64_t base = (int64_t)blockIdx.x * kTile;
+  for (int d = tid; d < 4 * kBins; d += 256) (&cnt[0][0])[d] = 0;
+  __syncthreads();
+
+  K key[kItems];
+  uint32_t pos[kItems], rank[kItems];
+  volatile uint32_t* mine = cnt[wave];
+  const uint64_t below = ((uint64_t)1 << lane) - 1;
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int64_t i = base + wave * (kTile / 4) + k * 64 + lane;
+    const bool in = i < N;
+    key[k] = in ? src(i) : 0;
+    pos[k] = in ? (FIRST ? (uint32_t)i : pos_in[i]) : 0;
+  }
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int64_t i = base + wave * (kTile / 4) + k * 64 + lane;
+    const bool in = i < N;
+    const uint32_t d = (uint32_t)(key[k] >> shift) & (bins - 1);
+    uint64_t same = __ballot(in);
+    for (int b = 0; b < bits; ++b) {
+      const uint64_t set = __ballot((d >> b) & 1);
+      same &= (d >> b) & 1 ? set : ~set;
+    }
+    const uint32_t lower = __popcll(same & below);
+    const uint32_t old = mine[d];  // read by all, then written by the first
+    rank[k] = old + lower;
+    __builtin_amdgcn_wave_barrier();
+    if (in && lower == 0) mine[d] = old + __popcll(same);
+    __builtin_amdgcn_wave_barrier();
+  }
+  __syncthreads();
+  // two neighbouring digits to a thread
+  uint32_t sum[2], tot[2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int d = tid * 2 + q;
+    uint32_t s = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t t = cnt[w][d];
+      cnt[w][d] = s;
+      s += t;
+    }
+    sum[q] = s;
+    tot[q] = d < bins ? totals[d] : 0;
+  }
+  uint32_t all;
+  const uint32_t l0 = block_scan(sum[0] + sum[1], s4, &all);
+  const uint32_t g0 = block_scan(tot[0] + tot[1], s4, &all);
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int d = tid * 2 + q;
+    const uint32_t at = l0 + (q ? sum[0] : 0);
+    local[d] = at;
+    if (d < bins)
+      goal[d] = g0 + (q ? tot[0] : 0) + counts[(int64_t)d * tiles + blockIdx.x] -
+                at;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int64_t i = base + wave * (kTile / 4) + k * 64 + lane;
+    if (i < N) {
+      const uint32_t d = (uint32_t)(key[k] >> shift) & (bins - 1);
+      const uint32_t at = local[d] + cnt[wave][d] + rank[k];
+      s_key[at] = key[k];
+      s_pos[at] = pos[k];
+    }
+  }
+  __syncthreads();
+  const int n = (int)(N - base < kTile ? N - base : kTile);
+  for (int at = tid; at < n; at += 256) {
+    const K key = s_key[at];
+    const uint32_t to =
+        goal[(uint32_t)(key >> shift) & (bins - 1)] + (uint32_t)at;
+    keys_out[to] = key;
+    pos_out[to] = s_pos[at];
+  }
+}
+
+// Up to EDL_SORT_SMALL items in one workgroup, all passes in LDS: one launch
+// in the place of three a pass. FROM: ids of any value, taken relative to
+// the smallest; *state is 1 where they do not fit 32 bits (and the output is
+// of no use), and the smallest goes to *low.
+constexpr int kSmallThreads = 1024;
+constexpr int kSmallItems = EDL_SORT_SMALL / kSmallThreads;
+constexpr int kSmallWaves = kSmallThreads / 64;
+
+template <typename S, bool FROM>
+__global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
+    S src, int N, int bits_all, uint32_t* keys_out, uint32_t* pos_out,
+    int64_t* low, uint32_t* state) {
+  __shared__ uint32_t s_key[EDL_SORT_SMALL];
+  __shared__ uint16_t s_pos[EDL_SORT_SMALL];
+  __shared__ uint16_t cnt[kSmallWaves][256];
+  __shared__ uint32_t local[256];
+  __shared__ int64_t s_min[kSmallWaves], s_max[kSmallWaves];
+  __shared__ uint32_t s4[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int i0 = wave * (EDL_SORT_SMALL / kSmallWaves) + lane;
+  uint32_t key[kSmallItems], pos[kSmallItems];
+  int bits = bits_all;
+  if constexpr (FROM) {
+    int64_t mn = INT64_MAX, mx = INT64_MIN;
+    int64_t v[kSmallItems];
+#pragma unroll
+    for (int k = 0; k < kSmallItems; ++k) {
+      const int i = i0 + k * 64;
+      v[k] = i < N ? src.ids[i] : 0;
+      if (i < N) {
+        mn = v[k] < mn ? v[k] : mn;
+        mx = v[k] > mx ? v[k] : mx;
+      }
+    }
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t a = __shfl_xor((long long)mn, o);
+      const int64_t b = __shfl_xor((long long)mx, o);
+      mn = a < mn ? a : mn;
+      mx = b > mx ? b : mx;
+    }
+    if (lane == 0) {
+      s_min[wave] = mn;
+      s_max[wave] = mx;
+    }
+    __syncthreads();
+    for (int w = 0; w < kSmallWaves; ++w) {
+      mn = s_min[w] < mn ? s_min[w] : mn;
+      mx = s_max[w] > mx ? s_max[w] : mx;
+    }
+    const uint64_t range = (uint64_t)mx - (uint64_t)mn;
+    const bool far = range >> 32 != 0;
+    if (tid == 0) {
+      *low = mn;
+      *state = far;
+    }
+    if (far) return;  // all threads alike
+    bits = range ? 64 - __clzll((long long)range) : 1;
+#pragma unroll
+    for (int k = 0; k < kSmallItems; ++k)
+      key[k] = (uint32_t)((uint64_t)v[k] - (uint64_t)mn);
+  } else {
+#pragma unroll
+    for (int k = 0; k < kSmallItems; ++k) {
+      const int i = i0 + k * 64;
+      key[k] = i < N ? (uint32_t)src(i) : 0;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kSmallItems; ++k) pos[k] = i0 + k * 64;
+
+  const uint64_t below = ((uint64_t)1 << lane) - 1;
+  volatile uint16_t* mine = cnt[wave];
+  for (int shift = 0; shift < bits; shift += 8) {
+    for (int d = tid; d < kSmallWaves * 256; d += kSmallThreads)
+      (&cnt[0][0])[d] = 0;
+    __syncthreads();
+    uint32_t rank[kSmallItems];
+#pragma unroll
+    for (int k = 0; k < kSmallItems; ++k) {
+      const bool in = i0 + k * 64 < N;
+      const uint32_t d = (key[k] >> shift) & 255;
+      uint64_t same = __ballot(in);
+#pragma unroll
+      for (int b = 0; b < 8; ++b) {
+        const uint64_t set = __ballot((d >> b) & 1);
+        same &= (d >> b) & 1 ? set : ~set;
+      }
+      const uint32_t lower = __popcll(same & below);
+      const uint32_t old = mine[d];
+      rank[k] = old + lower;
+      __builtin_amdgcn_wave_barrier();
+      if (in && lower == 0) mine[d] = (uint16_t)(old + __popcll(same));
+      __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    uint32_t total = 0;
+    if (tid < 256) {
+      for (int w = 0; w < kSmallWaves; ++w) {
+        const uint32_t t = cnt[w][tid];
+        cnt[w][tid] = (uint16_t)total;
+        total += t;
+      }
+    }
+    // exclusive sum over the 256 digits, by the first four waves
+    uint32_t x = total;
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t y = __shfl_up(x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 63 && wave < 4) s4[wave] = x;
+    __syncthreads();
+    if (tid < 256) {
+      uint32_t before = 0;
+      for (int w = 0; w < wave; ++w) before += s4[w];
+      local[tid] = before + x - total;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kSmallItems; ++k) {
+      if (i0 + k * 64 < N) {
+        const uint32_t d = (key[k] >> shift) & 255;
+        const uint32_t at = local[d] + cnt[wave][d] + rank[k];
+        s_key[at] = key[k];
+        s_pos[at] = (uint16_t)pos[k];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kSmallItems; ++k) {
+      const int i = i0 + k * 64;
+      if (i < N) {
+        key[k] = s_key[i];
+        pos[k] = s_pos[i];
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int k = 0; k < kSmallItems; ++k) {
+    const int i = i0 + k * 64;
+    if (i < N) {
+      keys_out[i] = key[k];
+      pos_out[i] = pos[k];
+    }
+  }
+}
+
+// smallest and largest of ids: range[0], range[1], which hold the extremes
+__global__ __launch_bounds__(256) void range_kernel(
+    const int64_t* __restrict__ ids, int64_t N, long long* range) {
+  long long mn = INT64_MAX, mx = INT64_MIN;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < N;
+       i += (int64_t)gridDim.x * 256) {
+    const long long v = ids[i];
+    mn = v < mn ? v : mn;
+    mx = v > mx ? v : mx;
+  }
+  for (int o = 1; o < 64; o <<= 1) {
+    const long long a = __shfl_xor(mn, o), b = __shfl_xor(mx, o);
+    mn = a < mn ? a : mn;
+    mx = b > mx ? b : mx;
+  }
+  if ((threadIdx.x & 63) == 0 && mn <= mx) {
+    atomicMin(&range[0], mn);
+    atomicMax(&range[1], mx);
+  }
+}
+__global__ void range_start_kernel(long long* range) {
+  range[0] = INT64_MAX;
+  range[1] = INT64_MIN;
+}
+
+// ------------------------------ unique ids --------------------------------
+// Each item's place among the unique keys: counts of first occurrences by
+// tile, their sums, then the places.
+template <typename K>
+__device__ inline bool first_of(const K* keys, int64_t i) {
+  return i == 0 || keys[i] != keys[i - 1];
+}
+
+template <typename K>
+__global__ __launch_bounds__(256) void unique_count_kernel(
+    const K* __restrict__ keys, int64_t N, uint32_t* counts) {
+  __shared__ uint32_t s4[4];
+  uint32_t n = 0;
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int64_t i = (int64_t)blockIdx.x * kTile + k * 256 + threadIdx.x;
+    if (i < N) n += first_of(keys, i);
+  }
+  uint32_t all;
+  block_scan(n, s4, &all);
+  if (threadIdx.x == 0) counts[blockIdx.x] = all;
+}
+
+template <typename K>
+__global__ __launch_bounds__(256) void unique_place_kernel(
+    const K* __restrict__ keys, int64_t N, const uint32_t* __restrict__ counts,
+    int64_t base, const int64_t* __restrict__ low, bool turned,
+    uint32_t* __restrict__ place, int64_t* __restrict__ unique) {
+  __shared__ uint32_t s4[4];
+  uint32_t run = counts[blockIdx.x];
+  const int64_t add = low ? *low : base;
+  for (int k = 0; k < kItems; ++k) {
+    const int64_t i = (int64_t)blockIdx.x * kTile + k * 256 + threadIdx.x;
+    const bool f = i < N && first_of(keys, i);
+    uint32_t all;
+    const uint32_t x = block_scan(f, s4, &all);
+    if (i < N) {
+      const uint32_t at = run + x + (f ? 1 : 0) - 1;
+      place[i] = at;
+      if (f)
+        unique[at] = turned ? (int64_t)((uint64_t)keys[i] ^
+                                        0x8000000000000000ull)
+                            : (int64_t)((uint64_t)keys[i] + (uint64_t)add);
+    }
+    run += all;
+  }
+}
+
+// ------------------------------ summed rows -------------------------------
+// The sorted tokens are cut into chunks of EDL_SEG_CHUNK, whatever the runs
+// of equal keys are, so that a frequent id costs no more than rare ones. A
+// group of lanes adds its chunk's rows in order, 8 in flight; a run that
+// begins and ends in the chunk is written at once. One that goes on past an
+// end of the chunk leaves its sum in the workspace, and the chunk in which
+// it begins collects the sums of those behind: short runs by a group, long
+// ones (over kShort chunks) by a whole workgroup each.
+constexpr int kChunk = EDL_SEG_CHUNK;
+constexpr int kShort = 8;
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void segment_kernel(edl_segments a) {
+  typedef Vec<T, VEC> V;
+  constexpr int U = 8;
+  const int lanes = lanes_of(a.D, VEC), pieces = pieces_of(a.D, VEC);
+  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
+  const int64_t c = unit / pieces;
+  const int col =
+      ((int)(unit % pieces) * lanes + (threadIdx.x & (lanes - 1))) * VEC;
+  const int64_t t0 = c * kChunk;
+  if (t0 >= a.N) return;
+  const int64_t t1 = t0 + kChunk < a.N ? t0 + kChunk : a.N;
+  const bool mine = col < a.D;
+  const T* src = static_cast<const T*>(a.src) + (mine ? col : 0);
+
+  float acc[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+  uint32_t cur = a.keys[t0];
+  bool open = t0 > 0 && a.keys[t0 - 1] == cur;  // begun in a chunk before
+  uint32_t head = kNone, tail = kNone;
+
+  auto keep = [&](int which) {
+    if (!mine) return;
+    float* p = a.part + (c * 2 + which) * a.D + col;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) p[k] = acc[k];
+  };
+  auto write = [&]() {
+    if (!mine) return;
+    V o;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) o.set(k, acc[k]);
+    *reinterpret_cast<decltype(o.v)*>(static_cast<T*>(a.out) +
+                                      (int64_t)cur * a.D + col) = o.v;
+  };
+
+  for (int64_t t = t0; t < t1; t += U) {
+    uint32_t key[U], row[U];
+    float w[U];
+    V v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t i = t + u < t1 ? t + u : t1 - 1;
+      key[u] = a.keys[i];
+      const uint32_t p = a.pos[i];
+      row[u] = a.L > 1 ? p / (uint32_t)a.L : p;
+      w[u] = a.weights ? load_any(a.weights, p, a.w_type) : 1.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      v[u].v = *reinterpret_cast<const decltype(v[u].v)*>(
+          src + (int64_t)row[u] * a.D);
+      w[u] *= a.coef ? a.coef[row[u]] : a.scale;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (t + u >= t1) break;
+      if (key[u] != cur) {
+        if (cur < a.limit) {
+          if (open) {
+            keep(0);
+            head = cur;
+          } else {
+            write();
+          }
+        }
+        cur = key[u];
+        open = false;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] += w[u] * v[u].get(k);
+    }
+  }
+  const bool goes_on = t1 < a.N && a.keys[t1] == cur;
+  if (cur < a.limit) {
+    if (open) {
+      keep(0);
+      head = cur;
+    } else if (goes_on) {
+      keep(1);
+      tail = cur;
+    } else {
+      write();
+    }
+  }
+  if (col == 0) {
+    a.head[c] = head;
+    a.tail[c] = tail;
+    if (c == 0) *a.listed = 0;
+  }
+}
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void segment_short_kernel(edl_segments a,
+                                                            int64_t chunks) {
+  typedef Vec<T, VEC> V;
+  const int lanes = lanes_of(a.D, VEC), pieces = pieces_of(a.D, VEC);
+  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
+  const int64_t c = unit / pieces;
+  const int col =
+      ((int)(unit % pieces) * lanes + (threadIdx.x & (lanes - 1))) * VEC;
+  if (c >= chunks) return;
+  const uint32_t key = a.tail[c];
+  if (key == kNone) return;
+  int n = 0;  // chunks behind that the run goes on into
+  while (n <= kShort && c + 1 + n < chunks && a.head[c + 1 + n] == key) ++n;
+  if (n > kShort) {
+    if (col == 0) a.list[atomicAdd(a.listed, 1u)] = (uint32_t)c;
+    return;
+  }
+  if (col >= a.D) return;
+  const float* p = a.part + (c * 2 + 1) * a.D + col;
+  float acc[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) acc[k] = p[k];
+  for (int q = 0; q < n; ++q) {
+    const float* h = a.part + (c + 1 + q) * 2 * a.D + col;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] += h[k];
+  }
+  V o;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) o.set(k, acc[k]);
+  *reinterpret_cast<decltype(o.v)*>(static_cast<T*>(a.out) +
+                                    (int64_t)key * a.D + col) = o.v;
+}
+
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void segment_long_kernel(edl_segments a,
+                                                           int64_t chunks) {
+  typedef Vec<T, VEC> V;
+  constexpr int U = 4;
+  __shared__ float s[256 * VEC];
+  const int lanes = lanes_of(a.D, VEC), pieces = pieces_of(a.D, VEC);
+  const int groups = 256 / lanes, g = threadIdx.x / lanes;
+  const uint32_t n = *a.listed;
+  for (uint32_t at = blockIdx.x; at < n * pieces; at += gridDim.x) {
+    const int64_t c = a.list[at / pieces];
+    const uint32_t key = a.tail[c];
+    const int col =
+        ((int)(at % pieces) * lanes + (threadIdx.x & (lanes - 1))) * VEC;
+    // the chunks behind that begin with this key: up to the first that does
+    // not, and they lie together
+    int64_t in = c + 1, out = chunks;
+    while (in < out) {
+      const int64_t mid = (in + out) / 2;
+      if (a.head[mid] == key)
+        in = mid + 1;
+      else
+        out = mid;
+    }
+    float acc[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+    const int64_t end = in;
+    if (col < a.D) {
+      for (int64_t q = c + 1 + g; q < end; q += (int64_t)groups * U) {
+        float v[U][VEC];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int64_t r = q + (int64_t)u * groups;
+          const float* h = a.part + (r < end ? r : q) * 2 * a.D + col;
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) v[u][k] = r < end ? h[k] : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) acc[k] += v[u][k];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) s[threadIdx.x * VEC + k] = acc[k];
+    __syncthreads();
+    for (int h = groups / 2; h > 0; h >>= 1) {
+      if (g < h) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k)
+          s[threadIdx.x * VEC + k] += s[(threadIdx.x + h * lanes) * VEC + k];
+      }
+      __syncthreads();
+    }
+    if (g == 0 && col < a.D) {
+      const float* p = a.part + (c * 2 + 1) * a.D + col;
+      V o;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        o.set(k, s[threadIdx.x * VEC + k] + p[k]);
+      *reinterpret_cast<decltype(o.v)*>(static_cast<T*>(a.out) +
+                                        (int64_t)key * a.D + col) = o.v;
+    }
+    __syncthreads();
+  }
+}
+
+// -------------------------------- launches --------------------------------
+unsigned blocks_for(int64_t threads) {
+  return (unsigned)((threads + 255) / 256);
+}
+
+template <typename T, int VEC>
+void launch_lookup(const edl_bag& a, hipStream_t st) {
+  const int64_t pieces = pieces_of(a.D, VEC), lanes = lanes_of(a.D, VEC);
+  // a wave to a bag where bags alone would leave most of the 256 CUs' 32
+  // waves empty
+  if (a.L > 8 && a.B * pieces * lanes < 256 * 8 * 64 && lanes < 64)
+    lookup_kernel<T, VEC, true>
+        <<<blocks_for(a.B * pieces * 64), 256, 0, st>>>(a);
+  else
+    lookup_kernel<T, VEC, false>
+        <<<blocks_for(a.B * pieces * lanes), 256, 0, st>>>(a);
+}
+template <typename T, int VEC>
+void launch_weight_grad(const edl_bag& a, hipStream_t st) {
+  const int64_t units = a.B * ((a.L + 7) / 8);
+  weight_grad_kernel<T, VEC>
+      <<<blocks_for(units * lanes_of(a.D, VEC)), 256, 0, st>>>(a);
+}
+template <typename T, int VEC>
+void launch_segments(const edl_segments& a, hipStream_t st) {
+  const int64_t chunks = (a.N + kChunk - 1) / kChunk;
+  const int64_t threads =
+      chunks * pieces_of(a.D, VEC) * lanes_of(a.D, VEC);
+  segment_kernel<T, VEC><<<blocks_for(threads), 256, 0, st>>>(a);
+  if (chunks == 1) return;
+  segment_short_kernel<T, VEC>
+      <<<blocks_for(threads), 256, 0, st>>>(a, chunks);
+  if (chunks <= kShort + 1) return;
+  segment_long_kernel<T, VEC><<<256, 256, 0, st>>>(a, chunks);
+}
+
+#define EDL_BY_TYPE(FN, A, ST)                       \
+  if ((A).type == EDL_T_F32) {                       \
+    if ((A).vec == 4) FN<float, 4>(A, ST);           \
+    else if ((A).vec == 2) FN<float, 2>(A, ST);      \
+    else FN<float, 1>(A, ST);                        \
+  } else if ((A).type == EDL_T_BF16) {               \
+    if ((A).vec == 8) FN<__bf16, 8>(A, ST);          \
+    else if ((A).vec == 4) FN<__bf16, 4>(A, ST);     \
+    else if ((A).vec == 2) FN<__bf16, 2>(A, ST);     \
+    else FN<__bf16, 1>(A, ST);                       \
+  } else {                                           \
+    if ((A).vec == 8) FN<_Float16, 8>(A, ST);        \
+    else if ((A).vec == 4) FN<_Float16, 4>(A, ST);   \
+    else if ((A).vec == 2) FN<_Float16, 2>(A, ST);   \
+    else FN<_Float16, 1>(A, ST);                     \
+  }
+
+template <typename S, bool FIRST>
+int sort_pass(S src, const uint32_t* pos_in, int64_t N, int shift, int bits,
+              uint32_t* counts, uint32_t* totals, typename S::K* keys_out,
+              uint32_t* pos_out, hipStream_t st) {
+  const int tiles = (int)((N + kTile - 1) / kTile), bins = 1 << bits;
+  sort_count_kernel<S>
+      <<<tiles, 256, 0, st>>>(src, N, shift, bits, tiles, counts);
+  sort_offsets_kernel<<<bins, 256, 0, st>>>(counts, tiles, totals);
+  sort_move_kernel<S, FIRST><<<tiles, 256, 0, st>>>(
+      src, pos_in, N, shift, bits, tiles, counts, totals, keys_out, pos_out);
+  return (int)hipGetLastError();
+}
+
+// sorts into keys[0], pos[0], or keys[1], pos[1]: which, or -1 - error
+template <typename S>
+int sort_all(S src, int64_t N, int bits, typename S::K* const* keys,
+             uint32_t* const* pos, uint32_t* counts, uint32_t* totals,
+             hipStream_t st) {
+  const int passes = (bits + 8) / 9;
+  int done = 0, at = 0;
+  for (int p = 0; p < passes; ++p) {
+    const int left = passes - p, b = (bits - done + left - 1) / left;
+    int rc;
+    if (p == 0)
+      rc = sort_pass<S, true>(src, nullptr, N, done, b, counts, totals,
+                              keys[0], pos[0], st);
+    else
+      rc = sort_pass<KeysOf<typename S::K>, false>(
+          KeysOf<typename S::K>{keys[at]}, pos[at], N, done, b, counts, totals,
+          keys[at ^ 1], pos[at ^ 1], st);
+    if (rc) return -1 - rc;
+    if (p) at ^= 1;
+    done += b;
+  }
+  return at;
+}
+
+template <typename K>
+int unique_all(const K* keys, int64_t N, uint32_t* counts, uint32_t* totals,
+               int64_t base, const int64_t* low, bool turned, uint32_t* place,
+               int64_t* unique, hipStream_t st) {
+  const int tiles = (int)((N + kTile - 1) / kTile);
+  unique_count_kernel<K><<<tiles, 256, 0, st>>>(keys, N, counts);
+  sort_offsets_kernel<<<1, 256, 0, st>>>(counts, tiles, totals);
+  unique_place_kernel<K><<<tiles, 256, 0, st>>>(keys, N, counts, base, low,
+                                                turned, place, unique);
+  return (int)hipGetLastError();
+}
+
+}  // namespace
+
+extern "C" int edl_lookup(const edl_bag* a, hipStream_t st) {
+  EDL_BY_TYPE(launch_lookup, *a, st)
+  return (int)hipGetLastError();
+}
+
+extern "C" int edl_lookup_weight_grad(const edl_bag* a, hipStream_t st) {
+  EDL_BY_TYPE(launch_weight_grad, *a, st)
+  return (int)hipGetLastError();
+}
+
+extern "C" int edl_segment_sums(const edl_segments* a, hipStream_t st) {
+  EDL_BY_TYPE(launch_segments, *a, st)
+  return (int)hipGetLastError();
+}
+
+// Sorts the ids of a table of V rows, those without a row behind the rest.
+// Returns which of the two buffers holds the result, or -1 - error.
+extern "C" int edl_sort_rows(const void* ids, int ids64, int64_t V, int64_t N,
+                             uint32_t* const* keys, uint32_t* const* pos,
+                             uint32_t* counts, uint32_t* totals,
+                             hipStream_t st) {
+  int bits = 1;
+  while (bits < 32 && (V >> bits) != 0) ++bits;
+  Keys32 src{ids, ids64 != 0, V};
+  if (N <= EDL_SORT_SMALL) {
+    sort_small_kernel<Keys32, false><<<1, kSmallThreads, 0, st>>>(
+        src, (int)N, bits, keys[0], pos[0], nullptr, nullptr);
+    const int rc = (int)hipGetLastError();
+    return rc ? -1 - rc : 0;
+  }
+  return sort_all(src, N, bits, keys, pos, counts, totals, st);
+}
+
+// the small sort of ids of any value; low and state as at the kernel
+extern "C" int edl_sort_ids_small(const int64_t* ids, int64_t N,
+                                  uint32_t* keys, uint32_t* pos, int64_t* low,
+                                  uint32_t* state, hipStream_t st) {
+  sort_small_kernel<Keys32From, true><<<1, kSmallThreads, 0, st>>>(
+      Keys32From{ids, 0}, (int)N, 0, keys, pos, low, state);
+  return (int)hipGetLastError();
+}
+
+extern "C" int edl_ids_range(const int64_t* ids, int64_t N, int64_t* range,
+                             hipStream_t st) {
+  long long* r = reinterpret_cast<long long*>(range);
+  range_start_kernel<<<1, 1, 0, st>>>(r);
+  int64_t b = (N + 2047) / 2048;
+  range_kernel<<<(unsigned)(b > 1024 ? 1024 : b), 256, 0, st>>>(ids, N, r);
+  return (int)hipGetLastError();
+}
+
+extern "C" int edl_sort_ids32(const int64_t* ids, int64_t base, int bits,
+                              int64_t N, uint32_t* const* keys,
+                              uint32_t* const* pos, uint32_t* counts,
+                              uint32_t* totals, hipStream_t st) {
+  return sort_all(Keys32From{ids, base}, N, bits, keys, pos, counts, totals,
+                  st);
+}
+
+extern "C" int edl_sort_ids64(const int64_t* ids, int64_t N,
+                              uint64_t* const* keys, uint32_t* const* pos,
+                              uint32_t* counts, uint32_t* totals,
+                              hipStream_t st) {
+  return sort_all(Keys64{ids}, N, 64, keys, pos, counts, totals, st);
+}
+
+extern "C" int edl_unique32(const uint32_t* keys, int64_t N, uint32_t* counts,
+                            uint32_t* totals, int64_t base, const int64_t* low,
+                            uint32_t* place, int64_t* unique, hipStream_t st) {
+  return unique_all(keys, N, counts, totals, base, low, false, place, unique,
+                    st);
+}
+
+extern "C" int edl_unique64(const uint64_t* keys, int64_t N, uint32_t* counts,
+                            uint32_t* totals, uint32_t* place, int64_t* unique,
+                            hipStream_t st) {
+  return unique_all(keys, N, counts, totals, 0, nullptr, true, place, unique,
+                    st);
+}

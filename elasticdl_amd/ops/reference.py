@@ -381,3 +381,23 @@ def fp8_dense_bwd(dy, act, mask, y, wtq, wts, xtq, xts, k, need_dx, need_dw,
         else:
             dw = torch.zeros(n, k, dtype=w_dtype)
     return dx, dw, dz.sum(0).to(b_dtype) if need_db else None
+
+
+# --------------------------- embedding lookup -----------------------------
+def embedding_lookup(table, ids, weights, combiner, scale):
+    """Rows, or pooled bags of rows, in f32, rounded once at the end."""
+    live = ids >= 0
+    at = ids.clamp(min=0).long()
+    # widened before the lookup, a gradient is summed in f32
+    rows = table.float()[at] if table.requires_grad else table[at].float()
+    rows = torch.where(live.unsqueeze(-1), rows, torch.zeros_like(rows))
+    if combiner is None:
+        return (rows * scale).to(table.dtype)
+    if weights is not None:
+        w = torch.where(live, weights.float(),
+                        torch.zeros_like(weights, dtype=torch.float32))
+        rows = rows * w.unsqueeze(-1)
+    n = live.sum(1).clamp(min=1).float()
+    coef = scale / (n if combiner == "mean" else
+                    n.sqrt() if combiner == "sqrtn" else torch.ones_like(n))
+    return (rows.sum(1) * coef.unsqueeze(1)).to(table.dtype)

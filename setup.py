@@ -26,6 +26,8 @@ ext = CUDAExtension(
         "elasticdl_amd/ops/csrc/bn_kernels.hip",
         "elasticdl_amd/ops/csrc/fp8_bindings.cpp",
         "elasticdl_amd/ops/csrc/fp8_kernels.hip",
+        "elasticdl_amd/ops/csrc/embedding_bindings.cpp",
+        "elasticdl_amd/ops/csrc/embedding_kernels.hip",
     ],
     extra_compile_args={
         "cxx": ["-O3", "-std=c++17"],
