@@ -171,17 +171,25 @@ __device__ inline void load_row8(const T* x, int64_t ld, int64_t R, int64_t C,
 
 constexpr int kLdsRow = 144;  // a transposed row: 128 bytes and 16 of padding
 
-template <typename T, bool COLS, bool TILE, bool DERIV>
-__global__ __launch_bounds__(256) void quantize_kernel(edl_fp8_quant a) {
-  __shared__ uint32_t s_max[4][kBlk];
-  __shared__ float s_sum[4][kBlk];
-  __shared__ __align__(16) uint8_t s_t[COLS ? kBlk * kLdsRow : 16];
+struct QuantLds {
+  uint32_t max[4][kBlk];
+  float sum[4][kBlk];
+  __align__(16) uint8_t t[kBlk * kLdsRow];
+};
+
+template <typename T, bool TILE, bool DERIV>
+__device__ inline void quantize_tile(const edl_fp8_quant& a, int64_t block,
+                                     QuantLds& lds) {
+  uint32_t(*s_max)[kBlk] = lds.max;
+  float(*s_sum)[kBlk] = lds.sum;
+  uint8_t* s_t = lds.t;
+  const bool cols = a.cols != nullptr;  // the transpose too
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int j = tid & 15;  // columns j*8 .. j*8+7
   const int i = tid >> 4;  // rows    i*8 .. i*8+7
   const int64_t ncb = (a.C + kBlk - 1) / kBlk;
-  const int64_t rb = blockIdx.x / ncb, cb = blockIdx.x % ncb;
+  const int64_t rb = block / ncb, cb = block % ncb;
   const int64_t r0 = rb * kBlk + i * 8, c0 = cb * kBlk + j * 8;
 
   float v[8][8];
@@ -238,7 +246,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(edl_fp8_quant a) {
 #pragma unroll
     for (int r = 0; r < 8; ++r) rmax[r] = max16(rmax[r]);
   }
-  if (COLS || TILE) {
+  if (cols || TILE) {
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
       uint32_t m = cmax[c];
@@ -247,9 +255,9 @@ __global__ __launch_bounds__(256) void quantize_kernel(edl_fp8_quant a) {
       if (lane < 16) s_max[wave][j * 8 + c] = m;
     }
   }
-  if (COLS || TILE || (DERIV && a.sums)) __syncthreads();
+  if (cols || TILE || (DERIV && a.sums)) __syncthreads();
 
-  if (COLS || TILE) {
+  if (cols || TILE) {
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
       int col = j * 8 + c;
@@ -286,7 +294,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(edl_fp8_quant a) {
       }
     }
   }
-  if (COLS) {
+  if (cols) {
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
       int b = scale_byte(cmax[c]);
@@ -310,14 +318,32 @@ __global__ __launch_bounds__(256) void quantize_kernel(edl_fp8_quant a) {
   }
 }
 
+template <typename T, bool TILE, bool DERIV>
+__global__ __launch_bounds__(256) void quantize_kernel(edl_fp8_quant a) {
+  __shared__ QuantLds lds;
+  quantize_tile<T, TILE, DERIV>(a, blockIdx.x, lds);
+}
+
+// a layer's input and its weight in one launch
+template <typename TX, typename TW>
+__global__ __launch_bounds__(256) void quantize_pair_kernel(edl_fp8_quant x,
+                                                            edl_fp8_quant w,
+                                                            int x_tiles) {
+  __shared__ QuantLds lds;
+  if ((int)blockIdx.x < x_tiles)
+    quantize_tile<TX, false, false>(x, blockIdx.x, lds);
+  else
+    quantize_tile<TW, true, false>(w, blockIdx.x - x_tiles, lds);
+}
+
 // out[c] = sum over the tiles of sums[t][c], in order of t within each of 16
 // lanes' share, the shares then in order
-__global__ __launch_bounds__(256) void column_sums_kernel(
-    const float* __restrict__ sums, int64_t tiles, int64_t C, void* out,
-    int type) {
+__device__ inline void column_sums(const float* __restrict__ sums,
+                                   int64_t tiles, int64_t C, void* out,
+                                   int type, int64_t block) {
   __shared__ float s[16][17];
   const int c = threadIdx.x & 15, k = threadIdx.x >> 4;
-  const int64_t col = (int64_t)blockIdx.x * 16 + c;
+  const int64_t col = block * 16 + c;
   float t = 0.f;
   if (col < C)
     for (int64_t r = k; r < tiles; r += 16) t += sums[r * C + col];
@@ -487,16 +513,19 @@ __device__ inline void epilogue16(const edl_fp8_gemm& g, int64_t m, int64_t n,
   }
 }
 
+template <int BM>
+struct GemmLds {  // two buffers each: A's, B's, scales (256 of A's and B's)
+  __align__(1024) uint8_t m[4 * BM * kBlk + 1024];
+};
+
 template <int WM, int WN, int FM, int FN, bool WIDE>
-__global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(
-    edl_fp8_gemm g) {
+__device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
+                                 uint8_t* smem) {
   constexpr int BM = WM * FM * 16, BN = WN * FN * 16, NW = WM * WN;
   static_assert(FN == 4 && FM % 4 == 0, "scale words hold four fragments");
   static_assert(BM == BN && (BM == 128 || BM == 256), "buffers' toggle");
   constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW;  // 1 KB loads a wave
-  // two buffers each: A's, B's, and the scales (256 of A's, 256 of B's)
   constexpr uint32_t kTile = BM * kBlk, kB = 2 * kTile, kS = 4 * kTile;
-  __shared__ __align__(1024) uint8_t smem[4 * kTile + 1024];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -504,7 +533,8 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(
 
   // tiles in groups of 4 rows of tiles, column by column
   const int ntm = (g.M + BM - 1) / BM, ntn = (g.N + BN - 1) / BN;
-  int bid = xcd_order(blockIdx.x, ntm * ntn);
+  const int order = xcd_order(block, blocks);
+  const int bid = order % (ntm * ntn), split = order / (ntm * ntn);
   const int per = 4 * ntn, grp = bid / per, in = bid % per;
   const int tall = min(4, ntm - grp * 4);
   const int64_t m0 = (int64_t)(grp * 4 + in % tall) * BM;
@@ -512,7 +542,6 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(
 
   // this split's share of the steps
   const int kb_all = (int)(g.ld / kBlk);
-  const int split = blockIdx.y;
   const int kb0 = (int)((int64_t)kb_all * split / g.splits);
   const int T = (int)((int64_t)kb_all * (split + 1) / g.splits) - kb0;
 
@@ -689,10 +718,30 @@ __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(
   }
 }
 
-// joins the splits in order; a thread takes 16 neighbours of a row
-__global__ __launch_bounds__(256) void gemm_join_kernel(edl_fp8_gemm g) {
+template <int WM, int WN, int FM, int FN, bool WIDE>
+__global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(
+    edl_fp8_gemm g) {
+  __shared__ GemmLds<WM * FM * 16> lds;
+  gemm_tile<WM, WN, FM, FN, WIDE>(g, blockIdx.x, gridDim.x, lds.m);
+}
+
+// the two products of a backward pass in one launch, each of 128 x 128
+template <bool WIDE0, bool WIDE1>
+__global__ __launch_bounds__(256, 2) void gemm_pair_kernel(edl_fp8_gemm g0,
+                                                           edl_fp8_gemm g1,
+                                                           int blocks0) {
+  __shared__ GemmLds<128> lds;
+  if ((int)blockIdx.x < blocks0)
+    gemm_tile<2, 2, 4, 4, WIDE0>(g0, blockIdx.x, blocks0, lds.m);
+  else
+    gemm_tile<2, 2, 4, 4, WIDE1>(g1, blockIdx.x - blocks0,
+                                 gridDim.x - blocks0, lds.m);
+}
+
+// joins a product's splits in order; a thread takes 16 neighbours of a row
+__device__ inline void gemm_join(const edl_fp8_gemm& g, int64_t block) {
   const int64_t each = g.part_ld / 16;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t id = block * 256 + threadIdx.x;
   if (id >= g.M * each) return;
   const int64_t m = id / each, n = (id % each) * 16;
   float v[16];
@@ -708,6 +757,17 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(edl_fp8_gemm g) {
     }
   }
   epilogue16(g, m, n, v);
+}
+
+// what is left when a pass's products are done: the joins of up to two of
+// them, and a bias's gradient; each takes the blocks that it needs
+__global__ __launch_bounds__(256) void finish_kernel(edl_fp8_finish f) {
+  int64_t b = blockIdx.x;
+  if (b < f.join_blocks[0]) return gemm_join(f.g[0], b);
+  b -= f.join_blocks[0];
+  if (b < f.join_blocks[1]) return gemm_join(f.g[1], b);
+  column_sums(f.sums, f.tiles, f.C, f.out, f.out_type,
+              b - f.join_blocks[1]);
 }
 
 // ------------------------------- few rows ---------------------------------
@@ -778,28 +838,47 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_rows_kernel(
   }
 }
 
+int64_t tiles_of(const edl_fp8_quant& a) {
+  return ((a.R + kBlk - 1) / kBlk) * ((a.C + kBlk - 1) / kBlk);
+}
+
 template <typename T>
 void launch_quantize(const edl_fp8_quant& a, hipStream_t st) {
-  const int64_t tiles =
-      ((a.R + kBlk - 1) / kBlk) * ((a.C + kBlk - 1) / kBlk);
-  dim3 grid((unsigned)tiles), block(256);
-  const bool cols = a.cols != nullptr;
-  if (a.tile) {
-    if (cols)
-      quantize_kernel<T, true, true, false><<<grid, block, 0, st>>>(a);
-    else
-      quantize_kernel<T, false, true, false><<<grid, block, 0, st>>>(a);
-  } else if (a.deriv) {
-    if (cols)
-      quantize_kernel<T, true, false, true><<<grid, block, 0, st>>>(a);
-    else
-      quantize_kernel<T, false, false, true><<<grid, block, 0, st>>>(a);
-  } else {
-    if (cols)
-      quantize_kernel<T, true, false, false><<<grid, block, 0, st>>>(a);
-    else
-      quantize_kernel<T, false, false, false><<<grid, block, 0, st>>>(a);
-  }
+  dim3 grid((unsigned)tiles_of(a)), block(256);
+  if (a.tile)
+    quantize_kernel<T, true, false><<<grid, block, 0, st>>>(a);
+  else if (a.deriv)
+    quantize_kernel<T, false, true><<<grid, block, 0, st>>>(a);
+  else
+    quantize_kernel<T, false, false><<<grid, block, 0, st>>>(a);
+}
+
+template <typename TX>
+void launch_quantize_pair(const edl_fp8_quant& x, const edl_fp8_quant& w,
+                          hipStream_t st) {
+  const int n = (int)tiles_of(x);
+  dim3 grid((unsigned)(n + tiles_of(w))), block(256);
+  if (w.type == EDL_T_F32)
+    quantize_pair_kernel<TX, float><<<grid, block, 0, st>>>(x, w, n);
+  else if (w.type == EDL_T_BF16)
+    quantize_pair_kernel<TX, __bf16><<<grid, block, 0, st>>>(x, w, n);
+  else
+    quantize_pair_kernel<TX, _Float16><<<grid, block, 0, st>>>(x, w, n);
+}
+
+int64_t tiles128(const edl_fp8_gemm& g) {
+  return ((g.M + 127) / 128) * ((g.N + 127) / 128);
+}
+int64_t tiles256(const edl_fp8_gemm& g) {
+  return ((g.M + 255) / 256) * ((g.N + 255) / 256);
+}
+
+// Which kernel. 256 x 256 reads each operand half as often but runs one
+// workgroup a CU, so it takes the products that give each of the 256 CUs
+// one. In 32 bits (wide) a wave's fragments take twice the registers: always
+// 128 x 128.
+bool takes_256(const edl_fp8_gemm& g) {
+  return !g.wide && tiles256(g) >= 256;
 }
 
 }  // namespace
@@ -814,52 +893,81 @@ extern "C" int edl_fp8_quantize(const edl_fp8_quant* a, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
-extern "C" int edl_fp8_column_sums(const float* sums, int64_t tiles, int64_t C,
-                                   void* out, int type, hipStream_t st) {
-  column_sums_kernel<<<dim3((unsigned)((C + 15) / 16)), dim3(256), 0, st>>>(
-      sums, tiles, C, out, type);
+extern "C" int edl_fp8_quantize_pair(const edl_fp8_quant* x,
+                                     const edl_fp8_quant* w, hipStream_t st) {
+  if (x->type == EDL_T_F32)
+    launch_quantize_pair<float>(*x, *w, st);
+  else if (x->type == EDL_T_BF16)
+    launch_quantize_pair<__bf16>(*x, *w, st);
+  else
+    launch_quantize_pair<_Float16>(*x, *w, st);
   return (int)hipGetLastError();
 }
 
-// Which tile, and how many splits. 256 x 256 reads each operand half as
-// often but runs one workgroup a CU, so it takes the products that give each
-// of the 256 CUs one; 128 x 128 takes the rest, split over the contraction
-// until there are 512 workgroups (two a CU) or four blocks are left to each.
-// In 32 bits a wave's fragments take twice the registers: always 128 x 128.
-static bool in_32_bits(const edl_fp8_gemm* g) {
-  return g->c_type == EDL_T_F32 || g->mask != nullptr;
-}
-static bool takes_256(const edl_fp8_gemm* g) {
-  return !in_32_bits(g) && ((g->M + 255) / 256) * ((g->N + 255) / 256) >= 256;
-}
-
-extern "C" int edl_fp8_gemm_splits(const edl_fp8_gemm* g) {
-  if (takes_256(g)) return 1;
-  const int64_t tiles = ((g->M + 127) / 128) * ((g->N + 127) / 128);
-  int64_t s = 512 / tiles, most = g->ld / kBlk / 4;
-  if (s > most) s = most;
-  if (s > 64) s = 64;
-  return s < 1 ? 1 : (int)s;
-}
-
-extern "C" int edl_fp8_gemm_run(const edl_fp8_gemm* g, hipStream_t st) {
-  if (takes_256(g)) {
-    const int64_t big = ((g->M + 255) / 256) * ((g->N + 255) / 256);
-    gemm_kernel<2, 4, 8, 4, false>
-        <<<dim3((unsigned)big, 1), dim3(512), 0, st>>>(*g);
-    return (int)hipGetLastError();
+// How many splits of the contraction each of n products (1 or 2, in one
+// launch) takes: as many as fill 512 workgroups (two a CU) together, with at
+// least four blocks to each.
+extern "C" void edl_fp8_gemm_splits(edl_fp8_gemm* g, int n) {
+  int64_t tiles = 0;
+  for (int i = 0; i < n; ++i)
+    if (!takes_256(g[i])) tiles += tiles128(g[i]);
+  for (int i = 0; i < n; ++i) {
+    g[i].splits = 1;
+    if (takes_256(g[i])) continue;
+    int64_t s = 512 / tiles, most = g[i].ld / kBlk / 4;
+    if (s > most) s = most;
+    if (s > 64) s = 64;
+    if (s > 1) g[i].splits = (int)s;
   }
-  const int64_t tiles = ((g->M + 127) / 128) * ((g->N + 127) / 128);
-  dim3 grid((unsigned)tiles, g->splits), block(256);
-  if (in_32_bits(g))
-    gemm_kernel<2, 2, 4, 4, true><<<grid, block, 0, st>>>(*g);
-  else
-    gemm_kernel<2, 2, 4, 4, false><<<grid, block, 0, st>>>(*g);
-  int rc = (int)hipGetLastError();
-  if (rc != 0 || g->splits == 1) return rc;
-  const int64_t n = g->M * (g->part_ld / 16);
-  gemm_join_kernel<<<dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st>>>(
-      *g);
+}
+
+static int launch_one(const edl_fp8_gemm& g, hipStream_t st) {
+  if (takes_256(g)) {
+    gemm_kernel<2, 4, 8, 4, false>
+        <<<dim3((unsigned)tiles256(g)), dim3(512), 0, st>>>(g);
+  } else {
+    dim3 grid((unsigned)(tiles128(g) * g.splits)), block(256);
+    if (g.wide)
+      gemm_kernel<2, 2, 4, 4, true><<<grid, block, 0, st>>>(g);
+    else
+      gemm_kernel<2, 2, 4, 4, false><<<grid, block, 0, st>>>(g);
+  }
+  return (int)hipGetLastError();
+}
+
+// n products (0 to 2), their joins, and where f's sums are not null a
+// bias's gradient
+extern "C" int edl_fp8_gemm_run(edl_fp8_finish* f, int n, hipStream_t st) {
+  edl_fp8_gemm* g = f->g;
+  int rc = 0;
+  if (n == 2 && !takes_256(g[0]) && !takes_256(g[1])) {
+    const int b0 = (int)tiles128(g[0]) * g[0].splits;
+    dim3 grid((unsigned)(b0 + tiles128(g[1]) * g[1].splits)), block(256);
+    const bool w0 = g[0].wide, w1 = g[1].wide;
+    if (w0 && w1)
+      gemm_pair_kernel<true, true><<<grid, block, 0, st>>>(g[0], g[1], b0);
+    else if (w0)
+      gemm_pair_kernel<true, false><<<grid, block, 0, st>>>(g[0], g[1], b0);
+    else if (w1)
+      gemm_pair_kernel<false, true><<<grid, block, 0, st>>>(g[0], g[1], b0);
+    else
+      gemm_pair_kernel<false, false><<<grid, block, 0, st>>>(g[0], g[1], b0);
+    rc = (int)hipGetLastError();
+  } else {
+    for (int i = 0; i < n && rc == 0; ++i) rc = launch_one(g[i], st);
+  }
+  if (rc != 0) return rc;
+  int64_t blocks = 0;
+  for (int i = 0; i < 2; ++i) {
+    f->join_blocks[i] =
+        i < n && g[i].splits > 1
+            ? (g[i].M * (g[i].part_ld / 16) + 255) / 256
+            : 0;
+    blocks += f->join_blocks[i];
+  }
+  if (f->sums) blocks += (f->C + 15) / 16;
+  if (blocks == 0) return 0;
+  finish_kernel<<<dim3((unsigned)blocks), dim3(256), 0, st>>>(*f);
   return (int)hipGetLastError();
 }
 

@@ -26,7 +26,7 @@ from typing import Optional, Union
 import torch
 from torch.autograd.function import once_differentiable
 
-from elasticdl_amd.ops import reference, use_native
+from elasticdl_amd.ops import reference, require_native, use_native
 from elasticdl_amd.ops.functional import _ACTS, ACT_RELU, ACT_SIGMOID
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
@@ -87,36 +87,21 @@ def quantize_fp8_weight(w: torch.Tensor) -> Fp8Blocks:
     return quantize_fp8(w, tile=True)
 
 
-def _weight_blocks(w, need_transposed):
-    """(bytes, scales) of w in tiles and, where asked for, of w^T."""
-    if use_native(w.device):
-        from elasticdl_amd.ops import _C
-
-        return _C.fp8_quantize(w, True, True, need_transposed)
-    q, s = reference.fp8_quantize(w, True)
-    if not need_transposed:
-        return q, s, None, None
-    return (q, s, *reference.fp8_quantize(w.t(), True))
-
-
 class _Fp8DenseFn(torch.autograd.Function):
+    """The CPU's; a GPU's is in csrc/fp8_bindings.cpp."""
+
     @staticmethod
     def forward(ctx, x, w, bias, act):
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        wq, ws, wtq, wts = _weight_blocks(w, need_x)
-        keep_mask = act == ACT_RELU and (need_x or need_w or need_b)
-        if use_native(x.device):
-            from elasticdl_amd.ops import _C
-
-            y, xtq, xts, mask = _C.fp8_dense_fwd(
-                x, wq, ws, w.shape[0], bias, act, need_w, keep_mask)
-        else:
-            y, xtq, xts, mask = reference.fp8_dense_fwd(
-                x, wq, ws, bias, act, need_w, keep_mask)
+        wtq = wts = None
+        if need_x:
+            wtq, wts = reference.fp8_quantize(w.t(), True)
+        y, xtq, xts, mask = reference.fp8_dense_fwd(
+            x, *reference.fp8_quantize(w, True), bias, act, need_w,
+            act == ACT_RELU and (need_x or need_w or need_b))
         ctx.act = act
         ctx.k = x.shape[1]
-        ctx.w_dtype = w.dtype
-        ctx.b_dtype = None if bias is None else bias.dtype
+        ctx.types = (w.dtype, None if bias is None else bias.dtype)
         ctx.save_for_backward(
             mask, y if act == ACT_SIGMOID else None, wtq, wts, xtq, xts)
         return y
@@ -124,17 +109,9 @@ class _Fp8DenseFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        mask, y, wtq, wts, xtq, xts = ctx.saved_tensors
-        need_x, need_w, need_b, _ = ctx.needs_input_grad
-        if use_native(dy.device):
-            from elasticdl_amd.ops import _C
-
-            bwd = _C.fp8_dense_bwd
-        else:
-            bwd = reference.fp8_dense_bwd
-        dx, dw, db = bwd(dy, ctx.act, mask, y, wtq, wts, xtq, xts, ctx.k,
-                         need_x, need_w, need_b, ctx.w_dtype, ctx.b_dtype)
-        return dx, dw, db, None
+        return (*reference.fp8_dense_bwd(
+            dy, ctx.act, *ctx.saved_tensors, ctx.k, *ctx.needs_input_grad[:3],
+            *ctx.types), None)
 
 
 def fp8_dense(x: torch.Tensor, w: Union[torch.Tensor, Fp8Blocks],
@@ -152,9 +129,16 @@ def fp8_dense(x: torch.Tensor, w: Union[torch.Tensor, Fp8Blocks],
     ``torch.autograd.grad`` (or drop eager graphs of the same leaves first):
     ``backward()`` accumulates on the stream of the eager graph's leaves,
     which ends the capture."""
-    if act not in _ACTS:
+    act_id = _ACTS.get(act)
+    if act_id is None:
         raise ValueError(f"unknown activation {act!r}, not in {list(_ACTS)}")
     frozen = isinstance(w, Fp8Blocks)
+    if x.is_cuda:
+        C = require_native()
+        if frozen:
+            return C.fp8_dense_frozen(x, w.data, w.scale, w.shape[1], bias,
+                                      act_id)
+        return C.fp8_dense(x, w, bias, act_id)
     if not frozen:
         _check_matrix(w, "w")
     if x.dtype not in _DTYPES:
@@ -165,6 +149,8 @@ def fp8_dense(x: torch.Tensor, w: Union[torch.Tensor, Fp8Blocks],
         raise ValueError(f"x is {tuple(x.shape)}, and the weight takes {k}")
     if w.device != x.device:
         raise ValueError(f"x is on {x.device}, and the weight on {w.device}")
+    if n == 0:
+        raise ValueError("the weight has no rows")
     if bias is not None:
         if bias.shape != (n,):
             raise ValueError(f"bias is {tuple(bias.shape)}, not ({n},)")
@@ -174,11 +160,7 @@ def fp8_dense(x: torch.Tensor, w: Union[torch.Tensor, Fp8Blocks],
         if bias.device != x.device:
             raise ValueError(
                 f"x is on {x.device}, and the bias on {bias.device}")
-        bias = bias.contiguous()
-    if n == 0:
-        raise ValueError("the weight has no rows")
     x2 = x.reshape(-1, k)
-    act_id = _ACTS[act]
     if not frozen:
         y = _Fp8DenseFn.apply(x2, w, bias, act_id)
     else:
@@ -187,12 +169,6 @@ def fp8_dense(x: torch.Tensor, w: Union[torch.Tensor, Fp8Blocks],
             raise RuntimeError(
                 "a weight from quantize_fp8_weight has no backward pass: call "
                 "under torch.no_grad(), or pass the weight as a tensor")
-        if use_native(x.device):
-            from elasticdl_amd.ops import _C
-
-            y = _C.fp8_dense_fwd(x2, w.data, w.scale, n, bias, act_id, False,
-                                 False)[0]
-        else:
-            y = reference.fp8_dense_fwd(x2, w.data, w.scale, bias, act_id,
-                                        False, False)[0]
+        y = reference.fp8_dense_fwd(x2, w.data, w.scale, bias, act_id, False,
+                                    False)[0]
     return y.reshape(*x.shape[:-1], n)
