@@ -1,11 +1,13 @@
 // Bindings of the embedding lookup and its gradient (embedding_kernels.hip):
-// argument checks, outputs and workspaces.
+// argument checks, outputs, workspaces, and the lookup's autograd function.
 
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <limits>
 
@@ -17,15 +19,17 @@ int edl_lookup_weight_grad(const edl_bag*, hipStream_t);
 int edl_segment_sums(const edl_segments*, hipStream_t);
 int edl_sort_rows(const void*, int, int64_t, int64_t, uint32_t* const*,
                   uint32_t* const*, uint32_t*, uint32_t*, hipStream_t);
-int edl_sort_ids_small(const int64_t*, int64_t, uint32_t*, uint32_t*, int64_t*,
-                       uint32_t*, hipStream_t);
+int edl_segment_chunk(int64_t, int, int);
+int64_t edl_sort_counts(int64_t);
+int edl_sort_unique_small(const int64_t*, int64_t, uint32_t*, uint32_t*,
+                          int64_t*, uint32_t*, hipStream_t);
 int edl_ids_range(const int64_t*, int64_t, int64_t*, hipStream_t);
 int edl_sort_ids32(const int64_t*, int64_t, int, int64_t, uint32_t* const*,
                    uint32_t* const*, uint32_t*, uint32_t*, hipStream_t);
 int edl_sort_ids64(const int64_t*, int64_t, uint64_t* const*,
                    uint32_t* const*, uint32_t*, uint32_t*, hipStream_t);
 int edl_unique32(const uint32_t*, int64_t, uint32_t*, uint32_t*, int64_t,
-                 const int64_t*, uint32_t*, int64_t*, hipStream_t);
+                 uint32_t*, int64_t*, hipStream_t);
 int edl_unique64(const uint64_t*, int64_t, uint32_t*, uint32_t*, uint32_t*,
                  int64_t*, hipStream_t);
 }
@@ -76,6 +80,27 @@ uint32_t* u32(const Tensor& t) {
   return reinterpret_cast<uint32_t*>(t.data_ptr<int32_t>());
 }
 
+// several pieces of a workspace in one allocation, on borders of 256 bytes
+class Pieces {
+ public:
+  template <typename T>
+  void add(T** p, int64_t n) {
+    *p = reinterpret_cast<T*>((intptr_t)size_);
+    size_ += (n * (int64_t)sizeof(T) + 255) / 256 * 256;
+    all_.push_back(reinterpret_cast<uint8_t**>(p));
+  }
+  Tensor place(const Tensor& like) {
+    Tensor t = words(like, {size_}, torch::kUInt8);
+    uint8_t* base = t.data_ptr<uint8_t>();
+    for (uint8_t** p : all_) *p = base + (intptr_t)*p;
+    return t;
+  }
+
+ private:
+  int64_t size_ = 0;
+  c10::SmallVector<uint8_t**, 12> all_;
+};
+
 edl_bag bag_of(const Tensor& ids, const OptTensor& weights, int64_t combiner,
                double scale) {
   TORCH_CHECK(ids.is_cuda(), "ids must be on a GPU");
@@ -124,127 +149,188 @@ void table_into(edl_bag& a, const Tensor& table, const Tensor& ids) {
   a.vec = vec_of(table, a.D, a.ld);
 }
 
-// (rows or pooled rows [.., D], each bag's factor where it is asked for)
-std::vector<OptTensor> embedding_fwd(Tensor table, Tensor ids,
-                                     OptTensor weights, int64_t combiner,
-                                     double scale, bool want_coef) {
-  c10::DeviceGuard guard(ids.device());
-  edl_bag a = bag_of(ids, weights, combiner, scale);
-  table_into(a, table, ids);
-  TORCH_CHECK(a.B * ((int64_t)a.D + 64) / 256 <
-                  std::numeric_limits<int32_t>::max(),
-              "the result is too large");
-  std::vector<OptTensor> out(2);
-  Tensor y = torch::empty({a.B, a.D}, table.options().requires_grad(false));
-  out[0] = y;
-  a.out = y.data_ptr();
-  if (want_coef) {
-    Tensor c = torch::empty({a.B}, y.options().dtype(torch::kFloat32));
-    a.coef = c.data_ptr<float>();
-    out[1] = c;
-  }
-  if (a.B > 0) launched(edl_lookup(&a, stream_of(ids)), "embedding lookup");
-  return out;
-}
-
-void segment_sums(edl_segments& s, const Tensor& like) {
-  const int64_t chunks = (s.N + EDL_SEG_CHUNK - 1) / EDL_SEG_CHUNK;
-  Tensor part = words(like, {chunks * 2, s.D}, torch::kFloat32);
-  Tensor marks = words(like, {chunks * 3 + 1});
-  s.part = part.data_ptr<float>();
-  s.head = u32(marks);
-  s.tail = s.head + chunks;
-  s.list = s.tail + chunks;
-  s.listed = s.list + chunks;
-  launched(edl_segment_sums(&s, stream_of(like)), "embedding gradient");
+void segments_into(edl_segments& s, Pieces& pieces) {
+  s.chunk = edl_segment_chunk(s.N, s.D, s.vec);
+  const int64_t chunks = (s.N + s.chunk - 1) / s.chunk;
+  pieces.add(&s.part, chunks * 2 * s.D);
+  pieces.add(&s.head, chunks);
+  pieces.add(&s.tail, chunks);
+  pieces.add(&s.list, chunks);
+  pieces.add(&s.listed, 1);
 }
 
 struct SortSpace {
-  Tensor keys, pos, counts;
-  uint32_t *k[2], *p[2], *count, *total;
-  SortSpace(const Tensor& like, int64_t n, bool with_keys = true) {
-    const int64_t tiles = (n + EDL_SORT_TILE - 1) / EDL_SORT_TILE;
-    if (with_keys) {
-      keys = words(like, {2, n});
-      k[0] = u32(keys);
-      k[1] = k[0] + n;
+  uint32_t *k[2] = {}, *p[2] = {}, *count = nullptr, *total = nullptr;
+  SortSpace(Pieces& pieces, int64_t n) {
+    for (int i = 0; i < 2; ++i) {
+      pieces.add(&k[i], n);
+      pieces.add(&p[i], n);
     }
-    pos = words(like, {2, n});
-    p[0] = u32(pos);
-    p[1] = p[0] + n;
-    counts = words(like, {(tiles + 1) * EDL_SORT_BINS});
-    count = u32(counts);
-    total = count + tiles * EDL_SORT_BINS;
+    pieces.add(&count, edl_sort_counts(n));
+    pieces.add(&total, EDL_SORT_BINS);
   }
 };
 
-// (the table's dense gradient [rows, D] of dy's type, the weights' [B, L] in
-// float32); each where it is asked for
-std::vector<OptTensor> embedding_bwd(Tensor dy, Tensor ids, OptTensor table,
-                                     OptTensor weights, OptTensor coef,
-                                     int64_t rows, int64_t combiner,
-                                     double scale, bool need_table,
-                                     bool need_weights) {
-  c10::DeviceGuard guard(ids.device());
-  edl_bag a = bag_of(ids, weights, combiner, scale);
-  TORCH_CHECK(dy.device() == ids.device() && dy.dim() == 2 &&
-                  dy.size(0) == a.B && dy.is_contiguous(),
-              "gradient does not match the ids");
-  TORCH_CHECK(rows >= 1 && rows < kMost, "too many rows: ", rows);
-  if (coef.has_value()) {
-    TORCH_CHECK(coef->device() == ids.device() &&
-                    coef->scalar_type() == torch::kFloat32 &&
-                    coef->numel() == a.B && coef->is_contiguous(),
-                "factors do not match the ids");
-    a.coef = coef->data_ptr<float>();
-  }
-  TORCH_CHECK(combiner < 0 || coef.has_value(), "no factors of the bags");
-  std::vector<OptTensor> out(2);
-  const int64_t n = ids.numel(), d = dy.size(1);
-  auto opts = dy.options().requires_grad(false);
-  if (need_weights) {
-    TORCH_CHECK(table.has_value() && weights.has_value(),
-                "no table or weights");
-    table_into(a, *table, ids);
-    TORCH_CHECK(a.D == d && table->scalar_type() == dy.scalar_type(),
-                "gradient does not match the table");
-    const int v = vec_of(dy, d, d);
-    if (v < a.vec) a.vec = v;
-    a.dy = dy.data_ptr();
-    Tensor dw = torch::empty(ids.sizes(), opts.dtype(torch::kFloat32));
-    a.dw = dw.data_ptr<float>();
-    if (n > 0)
-      launched(edl_lookup_weight_grad(&a, stream_of(ids)), "weights' gradient");
-    out[1] = dw;
-  }
-  if (need_table) {
-    Tensor dt = torch::zeros({rows, d}, opts);
-    if (n > 0) {
-      SortSpace sort(ids, n);
-      const int at =
-          edl_sort_rows(a.ids, a.ids64, rows, n, sort.k, sort.p, sort.count,
-                        sort.total, stream_of(ids));
-      launched(at < 0 ? -1 - at : 0, "sort of ids");
-      edl_segments s = {};
-      s.keys = sort.k[at];
-      s.pos = sort.p[at];
-      s.N = n;
-      s.limit = (uint32_t)rows;
-      s.src = dy.data_ptr();
-      s.D = (int)d;
-      s.type = type_code(dy.scalar_type(), "gradient");
-      s.vec = vec_of(dy, d, d);
-      s.L = a.L;
-      s.scale = a.scale;
-      s.coef = a.coef;
-      s.weights = a.weights;
-      s.w_type = a.w_type;
-      s.out = dt.data_ptr();
-      segment_sums(s, ids);
+class Lookup : public torch::autograd::Function<Lookup> {
+ public:
+  // grad: whether the caller's gradients are on
+  static Tensor forward(torch::autograd::AutogradContext* ctx, Tensor table,
+                        const OptTensor& weights_, Tensor ids,
+                        int64_t combiner, double scale, bool grad) {
+    const bool need_t = grad && table.requires_grad();
+    const bool need_w =
+        grad && weights_.has_value() && weights_->requires_grad();
+    c10::DeviceGuard guard(ids.device());
+    const OptTensor weights =
+        weights_.has_value() ? OptTensor(weights_->contiguous()) : OptTensor();
+    ids = ids.contiguous();
+    edl_bag a = bag_of(ids, weights, combiner, scale);
+    table_into(a, table, ids);
+    TORCH_CHECK(a.B * ((int64_t)a.D + 64) / 256 <
+                    std::numeric_limits<int32_t>::max(),
+                "the result is too large");
+    Tensor out =
+        torch::empty({a.B, a.D}, table.options().requires_grad(false));
+    a.out = out.data_ptr();
+    Tensor coef;  // each bag's factor, for the backward pass
+    if (combiner >= 0 && (need_t || need_w)) {
+      coef = words(ids, {a.B}, torch::kFloat32);
+      a.coef = coef.data_ptr<float>();
     }
-    out[0] = dt;
+    if (a.B > 0) launched(edl_lookup(&a, stream_of(ids)), "embedding lookup");
+    if (need_t || need_w) {
+      ctx->saved_data["rows"] = a.V;
+      ctx->saved_data["combiner"] = combiner;
+      ctx->saved_data["scale"] = scale;
+      ctx->saved_data["need"] = (int64_t)(need_t | need_w << 1);
+      ctx->save_for_backward({ids, need_w ? table : Tensor(),
+                              weights.has_value() ? *weights : Tensor(),
+                              coef});
+    }
+    return out;
   }
-  return out;
+
+  static torch::autograd::variable_list backward(
+      torch::autograd::AutogradContext* ctx,
+      torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t need = ctx->saved_data["need"].toInt();
+    torch::autograd::variable_list out(6);
+    if (!grads[0].defined()) return out;
+    {
+      at::NoGradGuard none;
+      run(grads[0].contiguous(), saved[0], saved[1], saved[2], saved[3],
+          ctx->saved_data["rows"].toInt(), ctx->saved_data["combiner"].toInt(),
+          ctx->saved_data["scale"].toDouble(),
+          (need & 1) && ctx->needs_input_grad(0),
+          (need & 2) && ctx->needs_input_grad(1), out);
+    }
+    if (at::GradMode::is_enabled()) {  // create_graph: fails where it is used
+      torch::autograd::variable_list held;
+      for (auto& t : out)
+        if (t.defined()) held.push_back(t.detach().requires_grad_(true));
+      auto fail = std::make_shared<torch::autograd::DelayedError>(
+          "embedding_lookup has no second derivative", (int64_t)held.size());
+      held = (*fail)(std::move(held));
+      size_t i = 0;
+      for (auto& t : out)
+        if (t.defined()) t = held[i++];
+    }
+    return out;
+  }
+
+ private:
+  // the table's dense gradient [rows, D] of dy's type, the weights' [B, L]
+  static void run(const Tensor& dy, const Tensor& ids, const Tensor& table,
+                  const Tensor& weights, const Tensor& coef, int64_t rows,
+                  int64_t combiner, double scale, bool need_t, bool need_w,
+                  torch::autograd::variable_list& out) {
+    c10::DeviceGuard guard(ids.device());
+    edl_bag a = bag_of(ids, weights.defined() ? OptTensor(weights) : OptTensor(),
+                       combiner, scale);
+    if (coef.defined()) a.coef = coef.data_ptr<float>();
+    const int64_t n = ids.numel(), d = dy.size(1);
+    const auto opts = dy.options().requires_grad(false);
+    if (need_w) {
+      table_into(a, table, ids);
+      const int v = vec_of(dy, d, d);
+      if (v < a.vec) a.vec = v;
+      a.dy = dy.data_ptr();
+      Tensor dw = torch::empty(ids.sizes(), opts.dtype(torch::kFloat32));
+      a.dw = dw.data_ptr<float>();
+      if (n > 0)
+        launched(edl_lookup_weight_grad(&a, stream_of(ids)),
+                 "weights' gradient");
+      out[1] = dw.to(weights.scalar_type());
+    }
+    if (!need_t) return;
+    Tensor dt = torch::zeros({rows, d}, opts);
+    out[0] = dt;
+    if (n == 0) return;
+    edl_segments s = {};
+    s.N = n;
+    s.limit = (uint32_t)rows;
+    s.src = dy.data_ptr();
+    s.D = (int)d;
+    s.type = type_code(dy.scalar_type(), "gradient");
+    s.vec = vec_of(dy, d, d);
+    s.L = a.L;
+    s.scale = a.scale;
+    s.coef = a.coef;
+    s.weights = a.weights;
+    s.w_type = a.w_type;
+    s.out = dt.data_ptr();
+    Pieces pieces;
+    SortSpace sort(pieces, n);
+    segments_into(s, pieces);
+    const Tensor space = pieces.place(ids);
+    const int at =
+        edl_sort_rows(a.ids, a.ids64, rows, n, sort.k, sort.p, sort.count,
+                      sort.total, stream_of(ids));
+    launched(at < 0 ? -1 - at : 0, "sort of ids");
+    s.keys = sort.k[at];
+    s.pos = sort.p[at];
+    launched(edl_segment_sums(&s, stream_of(ids)), "embedding gradient");
+  }
+};
+
+void check_type(const Tensor& t, const char* name) {
+  const auto d = t.scalar_type();
+  TORCH_CHECK_TYPE(d == torch::kFloat32 || d == torch::kBFloat16 ||
+                       d == torch::kFloat16,
+                   name, " must be float32, bfloat16 or float16, not ", d);
+}
+
+// the checks that a user meets are worded as on the CPU, in Python
+Tensor embedding_lookup(const Tensor& table_, const Tensor& ids,
+                        const OptTensor& weights, int64_t combiner,
+                        double scale) {
+  Tensor table = table_;
+  TORCH_CHECK_VALUE(
+      table.dim() == 2 && table.size(0) > 0 && table.size(1) > 0, "table is ",
+      table.sizes(), ", not [rows, dim]");
+  check_type(table, "table");
+  TORCH_CHECK_TYPE(ids.scalar_type() == torch::kInt64 ||
+                       ids.scalar_type() == torch::kInt32,
+                   "ids must be int64 or int32, not ", ids.scalar_type());
+  TORCH_CHECK_VALUE(ids.device() == table.device(), "ids are on ",
+                    ids.device(), ", and the table on ", table.device());
+  TORCH_CHECK_VALUE(combiner < 0 || ids.dim() == 2,
+                    "ids of bags must be [bags, length], not ", ids.sizes());
+  if (weights.has_value()) {
+    TORCH_CHECK_VALUE(combiner >= 0, "weights need a combiner");
+    TORCH_CHECK_VALUE(weights->sizes() == ids.sizes() &&
+                          weights->device() == ids.device(),
+                      "weights must have the ids' shape and device");
+    check_type(*weights, "weights");
+  }
+  if (table.size(1) > 1 && table.stride(1) != 1) table = table.contiguous();
+  Tensor out = Lookup::apply(table, weights, ids, combiner, scale,
+                             at::GradMode::is_enabled());
+  if (combiner >= 0 || ids.dim() == 1) return out;
+  auto shape = ids.sizes().vec();
+  shape.push_back(table.size(1));
+  return out.view(shape);
 }
 
 // (rows summed by id, the ids in order)
@@ -264,76 +350,88 @@ std::vector<Tensor> coalesce_rows(Tensor values, Tensor ids) {
   const int type = type_code(values.scalar_type(), "values");
   if (n == 0) return {torch::empty({0, d}, opts), torch::empty_like(ids)};
   const hipStream_t st = stream_of(ids);
-  Tensor place = words(ids, {n});
   Tensor unique = torch::empty_like(ids);
-  SortSpace sort(ids, n);
+  int64_t* ids_out = unique.data_ptr<int64_t>();
   const int64_t* id = ids.data_ptr<int64_t>();
-  uint32_t* pos = nullptr;
+  // what the host reads, in memory that the kernels write to directly: how
+  // many ids, whether they lie too far apart for the one-workgroup sort, and
+  // their smallest and largest by parts
+  const Tensor host =
+      torch::empty({1 + 2 * EDL_RANGE_PARTS},
+                   torch::TensorOptions().dtype(torch::kInt64).pinned_memory(
+                       true));
+  uint32_t* found_at = reinterpret_cast<uint32_t*>(host.data_ptr<int64_t>());
+  int64_t* range = host.data_ptr<int64_t>() + 1;
+  const auto wait = [&] {
+    c10::hip::getCurrentHIPStream(ids.device().index()).synchronize();
+  };
+  uint32_t* place = nullptr;
+  Pieces pieces;
+  pieces.add(&place, n);
+  SortSpace sort(pieces, n);
+  edl_segments s = {};
+  s.N = n;
+  s.D = (int)d;
+  s.vec = vec_of(values, d, d);
+  if (d > 0) segments_into(s, pieces);
+  const Tensor space = pieces.place(ids);
   int64_t found = -1;
   if (n <= EDL_SORT_SMALL) {
-    Tensor low = words(ids, {1}, torch::kInt64);
-    Tensor meta = words(ids, {2});  // how many; whether they lie too far apart
-    launched(edl_sort_ids_small(id, n, sort.k[0], sort.p[0],
-                                low.data_ptr<int64_t>(), u32(meta) + 1, st),
+    launched(edl_sort_unique_small(id, n, place, sort.p[0], ids_out, found_at,
+                                   st),
              "sort of ids");
-    launched(edl_unique32(sort.k[0], n, sort.count, u32(meta), 0,
-                          low.data_ptr<int64_t>(), u32(place),
-                          unique.data_ptr<int64_t>(), st),
-             "unique ids");
-    Tensor host = meta.cpu();
-    if (host.data_ptr<int32_t>()[1] == 0) {
-      found = host.data_ptr<int32_t>()[0];
-      pos = sort.p[0];
+    wait();
+    if (found_at[1] == 0) {
+      found = found_at[0];
+      s.pos = sort.p[0];
     }
   }
+  Tensor wide;  // 64-bit keys
   if (found < 0) {
-    Tensor range = words(ids, {2}, torch::kInt64);
-    launched(edl_ids_range(id, n, range.data_ptr<int64_t>(), st),
-             "range of ids");
-    Tensor host = range.cpu();
-    const int64_t low = host.data_ptr<int64_t>()[0];
-    const uint64_t span = (uint64_t)host.data_ptr<int64_t>()[1] - (uint64_t)low;
-    Tensor many = words(ids, {1});
+    launched(edl_ids_range(id, n, range, st), "range of ids");
+    wait();
+    int64_t low = range[0], high = range[1];
+    for (int i = 1; i < EDL_RANGE_PARTS; ++i) {
+      low = std::min(low, range[2 * i]);
+      high = std::max(high, range[2 * i + 1]);
+    }
+    const uint64_t span = (uint64_t)high - (uint64_t)low;
     if (span >> 32 == 0) {
       int bits = 1;
       while (bits < 32 && (span >> bits) != 0) ++bits;
       const int at = edl_sort_ids32(id, low, bits, n, sort.k, sort.p,
                                     sort.count, sort.total, st);
       launched(at < 0 ? -1 - at : 0, "sort of ids");
-      pos = sort.p[at];
-      launched(edl_unique32(sort.k[at], n, sort.count, u32(many), low, nullptr,
-                            u32(place), unique.data_ptr<int64_t>(), st),
+      s.pos = sort.p[at];
+      launched(edl_unique32(sort.k[at], n, sort.count, found_at, low, place,
+                            ids_out, st),
                "unique ids");
     } else {
-      Tensor wide = words(ids, {2, n}, torch::kInt64);
+      wide = words(ids, {2, n}, torch::kInt64);
       uint64_t* k[2];
       k[0] = reinterpret_cast<uint64_t*>(wide.data_ptr<int64_t>());
       k[1] = k[0] + n;
       const int at = edl_sort_ids64(id, n, k, sort.p, sort.count, sort.total,
                                     st);
       launched(at < 0 ? -1 - at : 0, "sort of ids");
-      pos = sort.p[at];
-      launched(edl_unique64(k[at], n, sort.count, u32(many), u32(place),
-                            unique.data_ptr<int64_t>(), st),
+      s.pos = sort.p[at];
+      launched(edl_unique64(k[at], n, sort.count, found_at, place, ids_out,
+                            st),
                "unique ids");
     }
-    found = many.item<int32_t>();
+    wait();
+    found = found_at[0];
   }
   Tensor rows = torch::empty({found, d}, opts);
   if (d > 0) {
-    edl_segments s = {};
-    s.keys = u32(place);
-    s.pos = pos;
-    s.N = n;
+    s.keys = place;
     s.limit = (uint32_t)found;
     s.src = values.data_ptr();
-    s.D = (int)d;
     s.type = type;
-    s.vec = vec_of(values, d, d);
     s.L = 1;
     s.scale = 1.f;
     s.out = rows.data_ptr();
-    segment_sums(s, ids);
+    launched(edl_segment_sums(&s, st), "sums of rows");
   }
   return {rows, unique.narrow(0, 0, found)};
 }
@@ -341,7 +439,8 @@ std::vector<Tensor> coalesce_rows(Tensor values, Tensor ids) {
 }  // namespace
 
 void edl_bind_embedding(py::module& m) {
-  m.def("embedding_fwd", &embedding_fwd);
-  m.def("embedding_bwd", &embedding_bwd);
-  m.def("coalesce_rows", &coalesce_rows);
+  m.def("embedding_lookup", &embedding_lookup,
+        py::call_guard<py::gil_scoped_release>());
+  m.def("coalesce_rows", &coalesce_rows,
+        py::call_guard<py::gil_scoped_release>());
 }

@@ -34,6 +34,7 @@ struct edl_bag {
 struct edl_segments {
   const uint32_t *keys, *pos;  // [N], sorted by key, then by pos
   int64_t N;
+  int chunk;       // tokens that a group of lanes takes
   uint32_t limit;  // keys from here on are no rows
   const void* src;  // [*, D] contiguous: row pos / L
   int D, type, vec, L;
@@ -48,7 +49,7 @@ struct edl_segments {
   uint32_t *list, *listed;    // long runs, and how many
 };
 
-#define EDL_SEG_CHUNK 32
+#define EDL_RANGE_PARTS 256
 #define EDL_SORT_TILE 4096
 #define EDL_SORT_BINS 512
 #define EDL_SORT_SMALL 8192

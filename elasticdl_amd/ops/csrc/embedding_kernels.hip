@@ -66,21 +66,20 @@ __host__ __device__ inline int pieces_of(int D, int vec) {
 
 // --------------------------------- lookup ---------------------------------
 // A row is read by the few lanes that its width takes, 8 ids at a time so
-// that 8 rows are in flight. SPLIT: a wave to a bag, its groups of lanes
-// taking every so-many-th eight, for calls with too few bags to fill the
-// chip otherwise.
-template <typename T, int VEC, bool SPLIT>
-__global__ __launch_bounds__(256) void lookup_kernel(edl_bag a) {
+// that 8 rows are in flight; `subs` such groups share a bag, each taking
+// every so-many-th eight, where bags alone are too few to fill the chip.
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void lookup_kernel(edl_bag a, int subs) {
   typedef Vec<T, VEC> V;
   constexpr int U = 8;
   const int lanes = lanes_of(a.D, VEC), pieces = pieces_of(a.D, VEC);
   const int lane = threadIdx.x & 63;
-  const int sub = SPLIT ? lane / lanes : 0, subs = SPLIT ? 64 / lanes : 1;
-  const int64_t id0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t unit = SPLIT ? id0 >> 6 : id0 / lanes;
+  const int sub = (lane / lanes) & (subs - 1);
+  const int64_t unit =
+      ((int64_t)blockIdx.x * 256 + threadIdx.x) / (lanes * subs);
   const int64_t bag = unit / pieces;
   const int col = ((int)(unit % pieces) * lanes + (lane & (lanes - 1))) * VEC;
-  if (bag >= a.B) return;  // whole groups, and whole waves where SPLIT
+  if (bag >= a.B) return;  // whole groups of lanes * subs
   const bool mine = col < a.D;
   const int at = mine ? col : 0;
   const T* table = static_cast<const T*>(a.table) + at;
@@ -115,14 +114,12 @@ __global__ __launch_bounds__(256) void lookup_kernel(edl_bag a) {
         acc[k] += bad == 0.f ? w * row[u].get(k) : bad;
     }
   }
-  if (SPLIT) {
-    for (int o = lanes; o < 64; o <<= 1) {
-      count += __shfl_xor(count, o);
+  for (int o = lanes; o < lanes * subs; o <<= 1) {
+    count += __shfl_xor(count, o);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) acc[k] += __shfl_xor(acc[k], o);
-    }
-    if (sub != 0) return;
+    for (int k = 0; k < VEC; ++k) acc[k] += __shfl_xor(acc[k], o);
   }
+  if (sub != 0) return;
   const float n = (float)(count > 1 ? count : 1);
   float c = a.scale;
   if (a.combiner == EDL_BAG_MEAN) c = a.scale / n;
@@ -221,10 +218,36 @@ struct KeysOf {  // what the pass before wrote
   __device__ K operator()(int64_t i) const { return keys[i]; }
 };
 
-constexpr int kTile = EDL_SORT_TILE, kBins = EDL_SORT_BINS;
-constexpr int kItems = kTile / 256;
+constexpr int kBins = EDL_SORT_BINS;
 
-template <typename S>
+// the lanes among `in` whose digit of `bits` bits is this lane's
+__device__ inline uint64_t same_digit(uint32_t d, int bits, bool in) {
+  const uint64_t all = __ballot(in);
+  uint32_t lo = (uint32_t)all, hi = (uint32_t)(all >> 32);
+  for (int b = 0; b < bits; ++b) {
+    const uint32_t mine = (uint32_t)((int32_t)(d << (31 - b)) >> 31);
+    const uint64_t set = __ballot((int32_t)mine < 0);
+    lo &= ~((uint32_t)set ^ mine);
+    hi &= ~((uint32_t)(set >> 32) ^ mine);
+  }
+  return (uint64_t)hi << 32 | lo;
+}
+// a lane's rank among the wave's items of its digit so far, which `count`
+// holds by digit: read by all, then moved on by the first of each digit
+template <typename C>
+__device__ inline uint32_t rank_digit(volatile C* count, uint32_t d, int bits,
+                                      bool in) {
+  const uint64_t same = same_digit(d, bits, in);
+  const uint32_t lower = __builtin_amdgcn_mbcnt_hi(
+      (uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
+  const uint32_t old = count[d];
+  __builtin_amdgcn_wave_barrier();
+  if (in && lower == 0) count[d] = (C)(old + __popcll(same));
+  __builtin_amdgcn_wave_barrier();
+  return old + lower;
+}
+
+template <typename S, int ITEMS>
 __global__ __launch_bounds__(256) void sort_count_kernel(S src, int64_t N,
                                                          int shift, int bits,
                                                          int tiles,
@@ -233,9 +256,9 @@ __global__ __launch_bounds__(256) void sort_count_kernel(S src, int64_t N,
   const int bins = 1 << bits;
   for (int d = threadIdx.x; d < bins; d += 256) h[d] = 0;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * kTile;
+  const int64_t base = (int64_t)blockIdx.x * (ITEMS * 256);
 #pragma unroll
-  for (int k = 0; k < kItems; ++k) {
+  for (int k = 0; k < ITEMS; ++k) {
     const int64_t i = base + k * 256 + threadIdx.x;
     if (i < N) atomicAdd(&h[(uint32_t)(src(i) >> shift) & (bins - 1)], 1u);
   }
@@ -284,13 +307,14 @@ __global__ __launch_bounds__(256) void sort_offsets_kernel(uint32_t* counts,
   if (threadIdx.x == 0) totals[blockIdx.x] = run;
 }
 
-template <typename S, bool FIRST>
+template <typename S, bool FIRST, int ITEMS>
 __global__ __launch_bounds__(256) void sort_move_kernel(
     S src, const uint32_t* __restrict__ pos_in, int64_t N, int shift, int bits,
     int tiles, const uint32_t* __restrict__ counts,
     const uint32_t* __restrict__ totals, typename S::K* __restrict__ keys_out,
     uint32_t* __restrict__ pos_out) {
   typedef typename S::K K;
+  constexpr int kTile = ITEMS * 256;
   __shared__ K s_key[kTile];
   __shared__ uint32_t s_pos[kTile];
   __shared__ uint32_t cnt[4][kBins];
@@ -300,40 +324,33 @@ __global__ __launch_bounds__(256) void sort_move_kernel(
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int bins = 1 << bits;
   const int64_t base = (int64_t)blockIdx.x * kTile;
-  for (int d = tid; d < 4 * kBins; d += 256) (&cnt[0][0])[d] = 0;
-  __syncthreads();
-
-  K key[kItems];
-  uint32_t pos[kItems], rank[kItems];
-  volatile uint32_t* mine = cnt[wave];
-  const uint64_t below = ((uint64_t)1 << lane) - 1;
+  const int64_t first = base + wave * (kTile / 4) + lane;
+  K key[ITEMS];
+  uint32_t pos[ITEMS], rank[ITEMS];
 #pragma unroll
-  for (int k = 0; k < kItems; ++k) {
-    const int64_t i = base + wave * (kTile / 4) + k * 64 + lane;
+  for (int k = 0; k < ITEMS; ++k) {
+    const int64_t i = first + k * 64;
     const bool in = i < N;
     key[k] = in ? src(i) : 0;
     pos[k] = in ? (FIRST ? (uint32_t)i : pos_in[i]) : 0;
   }
-#pragma unroll
-  for (int k = 0; k < kItems; ++k) {
-    const int64_t i = base + wave * (kTile / 4) + k * 64 + lane;
-    const bool in = i < N;
-    const uint32_t d = (uint32_t)(key[k] >> shift) & (bins - 1);
-    uint64_t same = __ballot(in);
-    for (int b = 0; b < bits; ++b) {
-      const uint64_t set = __ballot((d >> b) & 1);
-      same &= (d >> b) & 1 ? set : ~set;
-    }
-    const uint32_t lower = __popcll(same & below);
-    const uint32_t old = mine[d];  // read by all, then written by the first
-    rank[k] = old + lower;
-    __builtin_amdgcn_wave_barrier();
-    if (in && lower == 0) mine[d] = old + __popcll(same);
-    __builtin_amdgcn_wave_barrier();
-  }
-  __syncthreads();
   // two neighbouring digits to a thread
-  uint32_t sum[2], tot[2];
+  uint32_t tot[2], at_tile[2];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int d = tid * 2 + q;
+    tot[q] = d < bins ? totals[d] : 0;
+    at_tile[q] = d < bins ? counts[(int64_t)d * tiles + blockIdx.x] : 0;
+  }
+  for (int d = tid; d < 4 * kBins; d += 256) (&cnt[0][0])[d] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k)
+    rank[k] = rank_digit<uint32_t>(
+        cnt[wave], (uint32_t)(key[k] >> shift) & (bins - 1), bits,
+        first + k * 64 < N);
+  __syncthreads();
+  uint32_t sum[2];
 #pragma unroll
   for (int q = 0; q < 2; ++q) {
     const int d = tid * 2 + q;
@@ -345,7 +362,6 @@ __global__ __launch_bounds__(256) void sort_move_kernel(
       s += t;
     }
     sum[q] = s;
-    tot[q] = d < bins ? totals[d] : 0;
   }
   uint32_t all;
   const uint32_t l0 = block_scan(sum[0] + sum[1], s4, &all);
@@ -355,15 +371,12 @@ __global__ __launch_bounds__(256) void sort_move_kernel(
     const int d = tid * 2 + q;
     const uint32_t at = l0 + (q ? sum[0] : 0);
     local[d] = at;
-    if (d < bins)
-      goal[d] = g0 + (q ? tot[0] : 0) + counts[(int64_t)d * tiles + blockIdx.x] -
-                at;
+    goal[d] = g0 + (q ? tot[0] : 0) + at_tile[q] - at;
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < kItems; ++k) {
-    const int64_t i = base + wave * (kTile / 4) + k * 64 + lane;
-    if (i < N) {
+  for (int k = 0; k < ITEMS; ++k) {
+    if (first + k * 64 < N) {
       const uint32_t d = (uint32_t)(key[k] >> shift) & (bins - 1);
       const uint32_t at = local[d] + cnt[wave][d] + rank[k];
       s_key[at] = key[k];
@@ -382,35 +395,41 @@ __global__ __launch_bounds__(256) void sort_move_kernel(
 }
 
 // Up to EDL_SORT_SMALL items in one workgroup, all passes in LDS: one launch
-// in the place of three a pass. FROM: ids of any value, taken relative to
-// the smallest; *state is 1 where they do not fit 32 bits (and the output is
-// of no use), and the smallest goes to *low.
+// in the place of three a pass. A wave takes a run of 64 * items of them.
+//
+// UNIQUE: ids of any value, taken relative to the smallest. Also the unique
+// ids in order, each item's place among them, and for the host how many
+// there are (found[0]), or in found[1] that they lie too far apart for 32
+// bits, and nothing else.
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallItems = EDL_SORT_SMALL / kSmallThreads;
 constexpr int kSmallWaves = kSmallThreads / 64;
 
-template <typename S, bool FROM>
+template <typename S, bool UNIQUE>
 __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
     S src, int N, int bits_all, uint32_t* keys_out, uint32_t* pos_out,
-    int64_t* low, uint32_t* state) {
+    int64_t* unique, uint32_t* found) {
   __shared__ uint32_t s_key[EDL_SORT_SMALL];
   __shared__ uint16_t s_pos[EDL_SORT_SMALL];
-  __shared__ uint16_t cnt[kSmallWaves][256];
+  __shared__ __align__(16) uint16_t cnt[kSmallWaves][256];
   __shared__ uint32_t local[256];
   __shared__ int64_t s_min[kSmallWaves], s_max[kSmallWaves];
   __shared__ uint32_t s4[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int i0 = wave * (EDL_SORT_SMALL / kSmallWaves) + lane;
+  const int items = (N + kSmallThreads - 1) / kSmallThreads;
+  const int i0 = wave * items * 64 + lane;
   uint32_t key[kSmallItems], pos[kSmallItems];
   int bits = bits_all;
-  if constexpr (FROM) {
+  int64_t low = 0;
+  if constexpr (UNIQUE) {
     int64_t mn = INT64_MAX, mx = INT64_MIN;
     int64_t v[kSmallItems];
 #pragma unroll
     for (int k = 0; k < kSmallItems; ++k) {
       const int i = i0 + k * 64;
-      v[k] = i < N ? src.ids[i] : 0;
-      if (i < N) {
+      const bool in = k < items && i < N;
+      v[k] = in ? src.ids[i] : 0;
+      if (in) {
         mn = v[k] < mn ? v[k] : mn;
         mx = v[k] > mx ? v[k] : mx;
       }
@@ -432,11 +451,9 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
     }
     const uint64_t range = (uint64_t)mx - (uint64_t)mn;
     const bool far = range >> 32 != 0;
-    if (tid == 0) {
-      *low = mn;
-      *state = far;
-    }
+    if (tid == 0) found[1] = far;
     if (far) return;  // all threads alike
+    low = mn;
     bits = range ? 64 - __clzll((long long)range) : 1;
 #pragma unroll
     for (int k = 0; k < kSmallItems; ++k)
@@ -445,36 +462,26 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
 #pragma unroll
     for (int k = 0; k < kSmallItems; ++k) {
       const int i = i0 + k * 64;
-      key[k] = i < N ? (uint32_t)src(i) : 0;
+      key[k] = k < items && i < N ? (uint32_t)src(i) : 0;
     }
   }
 #pragma unroll
   for (int k = 0; k < kSmallItems; ++k) pos[k] = i0 + k * 64;
 
-  const uint64_t below = ((uint64_t)1 << lane) - 1;
-  volatile uint16_t* mine = cnt[wave];
-  for (int shift = 0; shift < bits; shift += 8) {
-    for (int d = tid; d < kSmallWaves * 256; d += kSmallThreads)
-      (&cnt[0][0])[d] = 0;
+  const int passes = (bits + 7) / 8;
+  int shift = 0;
+  for (int p = 0; p < passes; ++p) {
+    const int b = (bits - shift + passes - p - 1) / (passes - p);
+    const uint32_t digits = (1u << b) - 1;
+    for (int d = tid; d < kSmallWaves * 256 / 2; d += kSmallThreads)
+      reinterpret_cast<uint32_t*>(&cnt[0][0])[d] = 0;
     __syncthreads();
     uint32_t rank[kSmallItems];
 #pragma unroll
-    for (int k = 0; k < kSmallItems; ++k) {
-      const bool in = i0 + k * 64 < N;
-      const uint32_t d = (key[k] >> shift) & 255;
-      uint64_t same = __ballot(in);
-#pragma unroll
-      for (int b = 0; b < 8; ++b) {
-        const uint64_t set = __ballot((d >> b) & 1);
-        same &= (d >> b) & 1 ? set : ~set;
-      }
-      const uint32_t lower = __popcll(same & below);
-      const uint32_t old = mine[d];
-      rank[k] = old + lower;
-      __builtin_amdgcn_wave_barrier();
-      if (in && lower == 0) mine[d] = (uint16_t)(old + __popcll(same));
-      __builtin_amdgcn_wave_barrier();
-    }
+    for (int k = 0; k < kSmallItems; ++k)
+      if (k < items)  // whole waves
+        rank[k] = rank_digit<uint16_t>(cnt[wave], (key[k] >> shift) & digits,
+                                       b, i0 + k * 64 < N);
     __syncthreads();
     uint32_t total = 0;
     if (tid < 256) {
@@ -500,8 +507,8 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kSmallItems; ++k) {
-      if (i0 + k * 64 < N) {
-        const uint32_t d = (key[k] >> shift) & 255;
+      if (k < items && i0 + k * 64 < N) {
+        const uint32_t d = (key[k] >> shift) & digits;
         const uint32_t at = local[d] + cnt[wave][d] + rank[k];
         s_key[at] = key[k];
         s_pos[at] = (uint16_t)pos[k];
@@ -511,46 +518,95 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
 #pragma unroll
     for (int k = 0; k < kSmallItems; ++k) {
       const int i = i0 + k * 64;
-      if (i < N) {
+      if (k < items && i < N) {
         key[k] = s_key[i];
         pos[k] = s_pos[i];
       }
     }
     __syncthreads();
+    shift += b;
   }
+  if constexpr (UNIQUE) {
+    // each key's place: first occurrences before it, by wave, then overall
+    uint32_t here = 0, place[kSmallItems];
+    bool first[kSmallItems];
 #pragma unroll
-  for (int k = 0; k < kSmallItems; ++k) {
-    const int i = i0 + k * 64;
-    if (i < N) {
-      keys_out[i] = key[k];
-      pos_out[i] = pos[k];
+    for (int k = 0; k < kSmallItems; ++k) {
+      const int i = i0 + k * 64;
+      first[k] = k < items && i < N && (i == 0 || s_key[i - 1] != key[k]);
+      const uint64_t set = __ballot(first[k]);
+      place[k] = here + __builtin_amdgcn_mbcnt_hi(
+                            (uint32_t)(set >> 32),
+                            __builtin_amdgcn_mbcnt_lo((uint32_t)set, 0));
+      here += __popcll(set);
+    }
+    if (lane == 0) local[wave] = here;
+    __syncthreads();
+    uint32_t before = 0, all = 0;
+    for (int w = 0; w < kSmallWaves; ++w) {
+      if (w < wave) before += local[w];
+      all += local[w];
+    }
+    if (tid == 0) found[0] = all;
+#pragma unroll
+    for (int k = 0; k < kSmallItems; ++k) {
+      const int i = i0 + k * 64;
+      if (k < items && i < N) {
+        const uint32_t at = before + place[k] + first[k] - 1;
+        keys_out[i] = at;
+        pos_out[i] = pos[k];
+        if (first[k])
+          unique[at] = (int64_t)((uint64_t)low + (uint64_t)key[k]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kSmallItems; ++k) {
+      const int i = i0 + k * 64;
+      if (k < items && i < N) {
+        keys_out[i] = key[k];
+        pos_out[i] = pos[k];
+      }
     }
   }
 }
 
-// smallest and largest of ids: range[0], range[1], which hold the extremes
+// each workgroup's smallest and largest of ids, for the host: no atomics,
+// which thousands of waves would queue up for (100 us for 2.6 million ids,
+// against 9)
 __global__ __launch_bounds__(256) void range_kernel(
-    const int64_t* __restrict__ ids, int64_t N, long long* range) {
+    const int64_t* __restrict__ ids, int64_t N, int64_t* range) {
+  __shared__ long long s[2][4];
   long long mn = INT64_MAX, mx = INT64_MIN;
+  const int64_t step = (int64_t)gridDim.x * 256;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < N;
-       i += (int64_t)gridDim.x * 256) {
-    const long long v = ids[i];
-    mn = v < mn ? v : mn;
-    mx = v > mx ? v : mx;
+       i += 4 * step) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const long long v = ids[i + u * step < N ? i + u * step : i];
+      mn = v < mn ? v : mn;
+      mx = v > mx ? v : mx;
+    }
   }
   for (int o = 1; o < 64; o <<= 1) {
     const long long a = __shfl_xor(mn, o), b = __shfl_xor(mx, o);
     mn = a < mn ? a : mn;
     mx = b > mx ? b : mx;
   }
-  if ((threadIdx.x & 63) == 0 && mn <= mx) {
-    atomicMin(&range[0], mn);
-    atomicMax(&range[1], mx);
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) {
+    s[0][wave] = mn;
+    s[1][wave] = mx;
   }
-}
-__global__ void range_start_kernel(long long* range) {
-  range[0] = INT64_MAX;
-  range[1] = INT64_MIN;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 4; ++w) {
+      mn = s[0][w] < mn ? s[0][w] : mn;
+      mx = s[1][w] > mx ? s[1][w] : mx;
+    }
+    range[2 * blockIdx.x] = mn;
+    range[2 * blockIdx.x + 1] = mx;
+  }
 }
 
 // ------------------------------ unique ids --------------------------------
@@ -560,6 +616,8 @@ template <typename K>
 __device__ inline bool first_of(const K* keys, int64_t i) {
   return i == 0 || keys[i] != keys[i - 1];
 }
+
+constexpr int kItems = EDL_SORT_TILE / 256, kTile = EDL_SORT_TILE;
 
 template <typename K>
 __global__ __launch_bounds__(256) void unique_count_kernel(
@@ -579,37 +637,54 @@ __global__ __launch_bounds__(256) void unique_count_kernel(
 template <typename K>
 __global__ __launch_bounds__(256) void unique_place_kernel(
     const K* __restrict__ keys, int64_t N, const uint32_t* __restrict__ counts,
-    int64_t base, const int64_t* __restrict__ low, bool turned,
-    uint32_t* __restrict__ place, int64_t* __restrict__ unique) {
+    int64_t base, bool turned, uint32_t* __restrict__ place,
+    int64_t* __restrict__ unique) {
   __shared__ uint32_t s4[4];
-  uint32_t run = counts[blockIdx.x];
-  const int64_t add = low ? *low : base;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t i0 =
+      (int64_t)blockIdx.x * kTile + wave * (kTile / 4) + lane;
+  K key[kItems];
+  uint32_t at[kItems], here = 0;
+  bool first[kItems];
+#pragma unroll
   for (int k = 0; k < kItems; ++k) {
-    const int64_t i = (int64_t)blockIdx.x * kTile + k * 256 + threadIdx.x;
-    const bool f = i < N && first_of(keys, i);
-    uint32_t all;
-    const uint32_t x = block_scan(f, s4, &all);
-    if (i < N) {
-      const uint32_t at = run + x + (f ? 1 : 0) - 1;
-      place[i] = at;
-      if (f)
-        unique[at] = turned ? (int64_t)((uint64_t)keys[i] ^
-                                        0x8000000000000000ull)
-                            : (int64_t)((uint64_t)keys[i] + (uint64_t)add);
-    }
-    run += all;
+    const int64_t i = i0 + k * 64;
+    key[k] = i < N ? keys[i] : 0;
+    first[k] = i < N && (i == 0 || keys[i - 1] != key[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const uint64_t set = __ballot(first[k]);
+    at[k] = here + __builtin_amdgcn_mbcnt_hi(
+                       (uint32_t)(set >> 32),
+                       __builtin_amdgcn_mbcnt_lo((uint32_t)set, 0));
+    here += __popcll(set);
+  }
+  if (lane == 0) s4[wave] = here;
+  __syncthreads();
+  uint32_t before = counts[blockIdx.x];
+  for (int w = 0; w < wave; ++w) before += s4[w];
+#pragma unroll
+  for (int k = 0; k < kItems; ++k) {
+    const int64_t i = i0 + k * 64;
+    if (i >= N) break;
+    const uint32_t p = before + at[k] + first[k] - 1;
+    place[i] = p;
+    if (first[k])
+      unique[p] = turned
+                      ? (int64_t)((uint64_t)key[k] ^ 0x8000000000000000ull)
+                      : (int64_t)((uint64_t)key[k] + (uint64_t)base);
   }
 }
 
 // ------------------------------ summed rows -------------------------------
-// The sorted tokens are cut into chunks of EDL_SEG_CHUNK, whatever the runs
+// The sorted tokens are cut into chunks of a.chunk, whatever the runs
 // of equal keys are, so that a frequent id costs no more than rare ones. A
 // group of lanes adds its chunk's rows in order, 8 in flight; a run that
 // begins and ends in the chunk is written at once. One that goes on past an
 // end of the chunk leaves its sum in the workspace, and the chunk in which
 // it begins collects the sums of those behind: short runs by a group, long
 // ones (over kShort chunks) by a whole workgroup each.
-constexpr int kChunk = EDL_SEG_CHUNK;
 constexpr int kShort = 8;
 
 template <typename T, int VEC>
@@ -621,9 +696,9 @@ __global__ __launch_bounds__(256) void segment_kernel(edl_segments a) {
   const int64_t c = unit / pieces;
   const int col =
       ((int)(unit % pieces) * lanes + (threadIdx.x & (lanes - 1))) * VEC;
-  const int64_t t0 = c * kChunk;
+  const int64_t t0 = c * a.chunk;
   if (t0 >= a.N) return;
-  const int64_t t1 = t0 + kChunk < a.N ? t0 + kChunk : a.N;
+  const int64_t t1 = t0 + a.chunk < a.N ? t0 + a.chunk : a.N;
   const bool mine = col < a.D;
   const T* src = static_cast<const T*>(a.src) + (mine ? col : 0);
 
@@ -818,14 +893,14 @@ unsigned blocks_for(int64_t threads) {
 template <typename T, int VEC>
 void launch_lookup(const edl_bag& a, hipStream_t st) {
   const int64_t pieces = pieces_of(a.D, VEC), lanes = lanes_of(a.D, VEC);
-  // a wave to a bag where bags alone would leave most of the 256 CUs' 32
-  // waves empty
-  if (a.L > 8 && a.B * pieces * lanes < 256 * 8 * 64 && lanes < 64)
-    lookup_kernel<T, VEC, true>
-        <<<blocks_for(a.B * pieces * 64), 256, 0, st>>>(a);
-  else
-    lookup_kernel<T, VEC, false>
-        <<<blocks_for(a.B * pieces * lanes), 256, 0, st>>>(a);
+  // groups to a bag: until there are 32 waves for each of the 256 CUs, or
+  // one eight of ids is left to each
+  int subs = 1;
+  while (subs * lanes < 64 && subs * 8 < a.L &&
+         a.B * pieces * lanes * subs < 256 * 32 * 64)
+    subs *= 2;
+  lookup_kernel<T, VEC>
+      <<<blocks_for(a.B * pieces * lanes * subs), 256, 0, st>>>(a, subs);
 }
 template <typename T, int VEC>
 void launch_weight_grad(const edl_bag& a, hipStream_t st) {
@@ -835,7 +910,7 @@ void launch_weight_grad(const edl_bag& a, hipStream_t st) {
 }
 template <typename T, int VEC>
 void launch_segments(const edl_segments& a, hipStream_t st) {
-  const int64_t chunks = (a.N + kChunk - 1) / kChunk;
+  const int64_t chunks = (a.N + a.chunk - 1) / a.chunk;
   const int64_t threads =
       chunks * pieces_of(a.D, VEC) * lanes_of(a.D, VEC);
   segment_kernel<T, VEC><<<blocks_for(threads), 256, 0, st>>>(a);
@@ -863,35 +938,41 @@ void launch_segments(const edl_segments& a, hipStream_t st) {
     else FN<_Float16, 1>(A, ST);                     \
   }
 
-template <typename S, bool FIRST>
+// tiles of 1024 until there are enough of 4096 for the chip (160 thousand
+// ids: 14 us a move in 40 tiles of 4096)
+int sort_items(int64_t N) { return N < 1024 * 1024 ? 4 : 16; }
+
+template <typename S, bool FIRST, int ITEMS>
 int sort_pass(S src, const uint32_t* pos_in, int64_t N, int shift, int bits,
               uint32_t* counts, uint32_t* totals, typename S::K* keys_out,
               uint32_t* pos_out, hipStream_t st) {
-  const int tiles = (int)((N + kTile - 1) / kTile), bins = 1 << bits;
-  sort_count_kernel<S>
+  const int tiles = (int)((N + ITEMS * 256 - 1) / (ITEMS * 256));
+  const int bins = 1 << bits;
+  sort_count_kernel<S, ITEMS>
       <<<tiles, 256, 0, st>>>(src, N, shift, bits, tiles, counts);
   sort_offsets_kernel<<<bins, 256, 0, st>>>(counts, tiles, totals);
-  sort_move_kernel<S, FIRST><<<tiles, 256, 0, st>>>(
+  sort_move_kernel<S, FIRST, ITEMS><<<tiles, 256, 0, st>>>(
       src, pos_in, N, shift, bits, tiles, counts, totals, keys_out, pos_out);
   return (int)hipGetLastError();
 }
 
 // sorts into keys[0], pos[0], or keys[1], pos[1]: which, or -1 - error
-template <typename S>
-int sort_all(S src, int64_t N, int bits, typename S::K* const* keys,
-             uint32_t* const* pos, uint32_t* counts, uint32_t* totals,
-             hipStream_t st) {
+template <typename S, int ITEMS>
+int sort_by(S src, int64_t N, int bits, typename S::K* const* keys,
+            uint32_t* const* pos, uint32_t* counts, uint32_t* totals,
+            hipStream_t st) {
+  typedef typename S::K K;
   const int passes = (bits + 8) / 9;
   int done = 0, at = 0;
   for (int p = 0; p < passes; ++p) {
     const int left = passes - p, b = (bits - done + left - 1) / left;
     int rc;
     if (p == 0)
-      rc = sort_pass<S, true>(src, nullptr, N, done, b, counts, totals,
-                              keys[0], pos[0], st);
+      rc = sort_pass<S, true, ITEMS>(src, nullptr, N, done, b, counts, totals,
+                                     keys[0], pos[0], st);
     else
-      rc = sort_pass<KeysOf<typename S::K>, false>(
-          KeysOf<typename S::K>{keys[at]}, pos[at], N, done, b, counts, totals,
+      rc = sort_pass<KeysOf<K>, false, ITEMS>(
+          KeysOf<K>{keys[at]}, pos[at], N, done, b, counts, totals,
           keys[at ^ 1], pos[at ^ 1], st);
     if (rc) return -1 - rc;
     if (p) at ^= 1;
@@ -899,16 +980,24 @@ int sort_all(S src, int64_t N, int bits, typename S::K* const* keys,
   }
   return at;
 }
+template <typename S>
+int sort_all(S src, int64_t N, int bits, typename S::K* const* keys,
+             uint32_t* const* pos, uint32_t* counts, uint32_t* totals,
+             hipStream_t st) {
+  return sort_items(N) == 4
+             ? sort_by<S, 4>(src, N, bits, keys, pos, counts, totals, st)
+             : sort_by<S, 16>(src, N, bits, keys, pos, counts, totals, st);
+}
 
 template <typename K>
-int unique_all(const K* keys, int64_t N, uint32_t* counts, uint32_t* totals,
-               int64_t base, const int64_t* low, bool turned, uint32_t* place,
-               int64_t* unique, hipStream_t st) {
+int unique_all(const K* keys, int64_t N, uint32_t* counts, uint32_t* found,
+               int64_t base, bool turned, uint32_t* place, int64_t* unique,
+               hipStream_t st) {
   const int tiles = (int)((N + kTile - 1) / kTile);
   unique_count_kernel<K><<<tiles, 256, 0, st>>>(keys, N, counts);
-  sort_offsets_kernel<<<1, 256, 0, st>>>(counts, tiles, totals);
-  unique_place_kernel<K><<<tiles, 256, 0, st>>>(keys, N, counts, base, low,
-                                                turned, place, unique);
+  sort_offsets_kernel<<<1, 256, 0, st>>>(counts, tiles, found);
+  unique_place_kernel<K><<<tiles, 256, 0, st>>>(keys, N, counts, base, turned,
+                                                place, unique);
   return (int)hipGetLastError();
 }
 
@@ -947,21 +1036,35 @@ extern "C" int edl_sort_rows(const void* ids, int ids64, int64_t V, int64_t N,
   return sort_all(src, N, bits, keys, pos, counts, totals, st);
 }
 
-// the small sort of ids of any value; low and state as at the kernel
-extern "C" int edl_sort_ids_small(const int64_t* ids, int64_t N,
-                                  uint32_t* keys, uint32_t* pos, int64_t* low,
-                                  uint32_t* state, hipStream_t st) {
+// chunks for the segment kernels: as long as they leave 16 waves for each of
+// the 256 CUs, from 8 to 32 tokens
+extern "C" int edl_segment_chunk(int64_t N, int D, int vec) {
+  const int64_t per = (int64_t)pieces_of(D, vec) * lanes_of(D, vec);
+  int chunk = 32;
+  while (chunk > 8 && N / chunk * per < 256 * 16 * 64) chunk /= 2;
+  return chunk;
+}
+
+// how many counts a sort of N items needs
+extern "C" int64_t edl_sort_counts(int64_t N) {
+  const int64_t tile = sort_items(N) * 256;
+  return (N + tile - 1) / tile * EDL_SORT_BINS;
+}
+
+// the small sort of ids of any value: see the kernel
+extern "C" int edl_sort_unique_small(const int64_t* ids, int64_t N,
+                                     uint32_t* place, uint32_t* pos,
+                                     int64_t* unique, uint32_t* found,
+                                     hipStream_t st) {
   sort_small_kernel<Keys32From, true><<<1, kSmallThreads, 0, st>>>(
-      Keys32From{ids, 0}, (int)N, 0, keys, pos, low, state);
+      Keys32From{ids, 0}, (int)N, 0, place, pos, unique, found);
   return (int)hipGetLastError();
 }
 
+// pairs of smallest and largest, one for each of EDL_RANGE_PARTS parts
 extern "C" int edl_ids_range(const int64_t* ids, int64_t N, int64_t* range,
                              hipStream_t st) {
-  long long* r = reinterpret_cast<long long*>(range);
-  range_start_kernel<<<1, 1, 0, st>>>(r);
-  int64_t b = (N + 2047) / 2048;
-  range_kernel<<<(unsigned)(b > 1024 ? 1024 : b), 256, 0, st>>>(ids, N, r);
+  range_kernel<<<EDL_RANGE_PARTS, 256, 0, st>>>(ids, N, range);
   return (int)hipGetLastError();
 }
 
@@ -981,15 +1084,13 @@ extern "C" int edl_sort_ids64(const int64_t* ids, int64_t N,
 }
 
 extern "C" int edl_unique32(const uint32_t* keys, int64_t N, uint32_t* counts,
-                            uint32_t* totals, int64_t base, const int64_t* low,
-                            uint32_t* place, int64_t* unique, hipStream_t st) {
-  return unique_all(keys, N, counts, totals, base, low, false, place, unique,
-                    st);
+                            uint32_t* found, int64_t base, uint32_t* place,
+                            int64_t* unique, hipStream_t st) {
+  return unique_all(keys, N, counts, found, base, false, place, unique, st);
 }
 
 extern "C" int edl_unique64(const uint64_t* keys, int64_t N, uint32_t* counts,
-                            uint32_t* totals, uint32_t* place, int64_t* unique,
+                            uint32_t* found, uint32_t* place, int64_t* unique,
                             hipStream_t st) {
-  return unique_all(keys, N, counts, totals, 0, nullptr, true, place, unique,
-                    st);
+  return unique_all(keys, N, counts, found, 0, true, place, unique, st);
 }

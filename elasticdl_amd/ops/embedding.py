@@ -21,44 +21,11 @@ CPU the same formulas in torch (ops/reference.py).
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from elasticdl_amd.ops import reference, use_native
+from elasticdl_amd.ops import reference, require_native
 
 _COMBINERS = {None: -1, "sum": 0, "mean": 1, "sqrtn": 2}
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
-
-
-class _LookupFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, table, weights, ids, combiner, scale):
-        from elasticdl_amd.ops import _C
-
-        need_table, need_weights = ctx.needs_input_grad[:2]
-        pooled = combiner >= 0
-        out, coef = _C.embedding_fwd(
-            table, ids, weights, combiner, scale,
-            pooled and (need_table or need_weights))
-        ctx.args = (table.shape[0], combiner, scale,
-                    None if weights is None else weights.dtype)
-        ctx.save_for_backward(ids, table if need_weights else None, weights,
-                              coef)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        from elasticdl_amd.ops import _C
-
-        ids, table, weights, coef = ctx.saved_tensors
-        rows, combiner, scale, w_dtype = ctx.args
-        need_table, need_weights = ctx.needs_input_grad[:2]
-        dt, dw = _C.embedding_bwd(
-            dy.contiguous(), ids, table, weights, coef, rows, combiner, scale,
-            need_table, need_weights)
-        if dw is not None:
-            dw = dw.to(w_dtype)
-        return dt, dw, None, None, None
 
 
 def embedding_lookup(table: torch.Tensor, ids: torch.Tensor,
@@ -79,8 +46,12 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor,
     (float32, bfloat16 or float16), rounded once from a sum in 32 bits. The
     table's gradient is dense, in the table's type; weights have one too.
     Rows of the table may be strided."""
-    if combiner not in _COMBINERS:
+    code = _COMBINERS.get(combiner)
+    if code is None:
         raise ValueError(f"unknown combiner {combiner!r}")
+    if table.is_cuda:
+        return require_native().embedding_lookup(table, ids, weights, code,
+                                                 scale)
     if table.dim() != 2 or table.shape[0] == 0 or table.shape[1] == 0:
         raise ValueError(f"table is {tuple(table.shape)}, not [rows, dim]")
     if table.dtype not in _DTYPES:
@@ -102,16 +73,7 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor,
         if weights.dtype not in _DTYPES:
             raise TypeError("weights must be float32, bfloat16 or float16, "
                             f"not {weights.dtype}")
-    shape = ids.shape if combiner is None else ids.shape[:1]
-    if use_native(table.device):
-        if table.shape[1] > 1 and table.stride(1) != 1:
-            table = table.contiguous()
-        out = _LookupFn.apply(
-            table, None if weights is None else weights.contiguous(),
-            ids.contiguous(), _COMBINERS[combiner], float(scale))
-    else:
-        out = reference.embedding_lookup(table, ids, weights, combiner, scale)
-    return out.reshape(*shape, table.shape[1])
+    return reference.embedding_lookup(table, ids, weights, combiner, scale)
 
 
 def coalesce_rows(values: torch.Tensor, ids: torch.Tensor
@@ -119,15 +81,13 @@ def coalesce_rows(values: torch.Tensor, ids: torch.Tensor
     """(summed rows [u, dim], unique ids [u] in order) of values [n, dim] and
     ids [n], any int64. GPU only, without a gradient; it reads back how many
     ids there are, so it cannot be captured into a graph."""
-    if not use_native(values.device):
+    if not values.is_cuda:
         raise ValueError("coalesce_rows runs on a GPU; use "
                          "deduplicate_indexed_slices")
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(
             "coalesce_rows reads back how many ids there are and cannot be "
             "captured into a graph")
-    from elasticdl_amd.ops import _C
-
-    rows, unique = _C.coalesce_rows(values.detach().contiguous(),
-                                    ids.contiguous())
+    rows, unique = require_native().coalesce_rows(
+        values.detach().contiguous(), ids.contiguous())
     return rows, unique
