@@ -24,8 +24,10 @@ int64_t edl_sort_counts(int64_t);
 int edl_sort_unique_small(const int64_t*, int64_t, uint32_t*, uint32_t*,
                           int64_t*, uint32_t*, hipStream_t);
 int edl_ids_range(const int64_t*, int64_t, int64_t*, hipStream_t);
-int edl_sort_ids32(const int64_t*, int64_t, int, int64_t, uint32_t* const*,
-                   uint32_t* const*, uint32_t*, uint32_t*, hipStream_t);
+int edl_sort_ids32_first(const int64_t*, int, int64_t, uint32_t* const*,
+                         uint32_t* const*, uint32_t*, uint32_t*, hipStream_t);
+int edl_sort_ids32_rest(int, int, int64_t, uint32_t* const*, uint32_t* const*,
+                        uint32_t*, uint32_t*, hipStream_t);
 int edl_sort_ids64(const int64_t*, int64_t, uint64_t* const*,
                    uint32_t* const*, uint32_t*, uint32_t*, hipStream_t);
 int edl_unique32(const uint32_t*, int64_t, uint32_t*, uint32_t*, int64_t,
@@ -44,6 +46,19 @@ constexpr int64_t kMost = std::numeric_limits<int32_t>::max() - EDL_SORT_TILE;
 
 hipStream_t stream_of(const Tensor& t) {
   return c10::hip::getCurrentHIPStream(t.device().index()).stream();
+}
+
+// one event for each thread and device, kept: making one costs as much as it
+// saves
+hipEvent_t event_of(int device) {
+  constexpr int kDevices = 64;
+  static thread_local hipEvent_t events[kDevices] = {};
+  TORCH_CHECK(device >= 0 && device < kDevices, "device ", device);
+  if (!events[device])
+    TORCH_CHECK(hipEventCreateWithFlags(&events[device],
+                                        hipEventDisableTiming) == hipSuccess,
+                "event");
+  return events[device];
 }
 
 void launched(int rc, const char* what) {
@@ -362,8 +377,12 @@ std::vector<Tensor> coalesce_rows(Tensor values, Tensor ids) {
                        true));
   uint32_t* found_at = reinterpret_cast<uint32_t*>(host.data_ptr<int64_t>());
   int64_t* range = host.data_ptr<int64_t>() + 1;
-  const auto wait = [&] {
-    c10::hip::getCurrentHIPStream(ids.device().index()).synchronize();
+  const hipEvent_t known = event_of(ids.device().index());
+  const auto mark = [&] {
+    TORCH_CHECK(hipEventRecord(known, st) == hipSuccess, "event record");
+  };
+  const auto wait = [&] {  // for what was launched before the mark
+    TORCH_CHECK(hipEventSynchronize(known) == hipSuccess, "event wait");
   };
   uint32_t* place = nullptr;
   Pieces pieces;
@@ -375,36 +394,57 @@ std::vector<Tensor> coalesce_rows(Tensor values, Tensor ids) {
   s.vec = vec_of(values, d, d);
   if (d > 0) segments_into(s, pieces);
   const Tensor space = pieces.place(ids);
+  s.src = values.data_ptr();
+  s.type = type;
+  s.L = 1;
+  s.scale = 1.f;
+  s.keys = place;
+  s.limit = (uint32_t)n;
+  // small results are summed into room for n rows before the host knows how
+  // many there are, which takes it longer than the sums take
+  const bool early = n * d * values.element_size() <= (4 << 20);
+  Tensor rows;
+  const auto sum_into = [&](int64_t most) {
+    rows = torch::empty({most, d}, opts);
+    s.out = rows.data_ptr();
+    if (d > 0) launched(edl_segment_sums(&s, st), "sums of rows");
+  };
   int64_t found = -1;
   if (n <= EDL_SORT_SMALL) {
+    s.pos = sort.p[0];
     launched(edl_sort_unique_small(id, n, place, sort.p[0], ids_out, found_at,
                                    st),
              "sort of ids");
+    mark();
+    if (early) sum_into(n);
     wait();
-    if (found_at[1] == 0) {
-      found = found_at[0];
-      s.pos = sort.p[0];
-    }
+    if (found_at[1] == 0) found = found_at[0];
   }
   Tensor wide;  // 64-bit keys
   if (found < 0) {
+    rows = Tensor();
+    constexpr int kFirst = 9;
     launched(edl_ids_range(id, n, range, st), "range of ids");
+    mark();
+    launched(edl_sort_ids32_first(id, kFirst, n, sort.k, sort.p, sort.count,
+                                  sort.total, st),
+             "sort of ids");
     wait();
     int64_t low = range[0], high = range[1];
     for (int i = 1; i < EDL_RANGE_PARTS; ++i) {
       low = std::min(low, range[2 * i]);
       high = std::max(high, range[2 * i + 1]);
     }
-    const uint64_t span = (uint64_t)high - (uint64_t)low;
-    if (span >> 32 == 0) {
+    const uint64_t differ = (uint64_t)low ^ (uint64_t)high;
+    if (differ >> 32 == 0) {
       int bits = 1;
-      while (bits < 32 && (span >> bits) != 0) ++bits;
-      const int at = edl_sort_ids32(id, low, bits, n, sort.k, sort.p,
-                                    sort.count, sort.total, st);
+      while (bits < 32 && (differ >> bits) != 0) ++bits;
+      const int at = edl_sort_ids32_rest(kFirst, bits, n, sort.k, sort.p,
+                                         sort.count, sort.total, st);
       launched(at < 0 ? -1 - at : 0, "sort of ids");
       s.pos = sort.p[at];
-      launched(edl_unique32(sort.k[at], n, sort.count, found_at, low, place,
-                            ids_out, st),
+      launched(edl_unique32(sort.k[at], n, sort.count, found_at,
+                            low & ~(int64_t)0xffffffff, place, ids_out, st),
                "unique ids");
     } else {
       wide = words(ids, {2, n}, torch::kInt64);
@@ -419,21 +459,13 @@ std::vector<Tensor> coalesce_rows(Tensor values, Tensor ids) {
                             st),
                "unique ids");
     }
+    mark();
+    if (early) sum_into(n);
     wait();
     found = found_at[0];
   }
-  Tensor rows = torch::empty({found, d}, opts);
-  if (d > 0) {
-    s.keys = place;
-    s.limit = (uint32_t)found;
-    s.src = values.data_ptr();
-    s.type = type;
-    s.L = 1;
-    s.scale = 1.f;
-    s.out = rows.data_ptr();
-    launched(edl_segment_sums(&s, st), "sums of rows");
-  }
-  return {rows, unique.narrow(0, 0, found)};
+  if (!rows.defined()) sum_into(found);
+  return {rows.narrow(0, 0, found), unique.narrow(0, 0, found)};
 }
 
 }  // namespace

@@ -51,5 +51,5 @@ struct edl_segments {
 
 #define EDL_RANGE_PARTS 256
 #define EDL_SORT_TILE 4096
-#define EDL_SORT_BINS 512
+#define EDL_SORT_BINS 2048  // most of a pass
 #define EDL_SORT_SMALL 8192

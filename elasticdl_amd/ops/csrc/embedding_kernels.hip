@@ -182,7 +182,7 @@ __global__ __launch_bounds__(256) void weight_grad_kernel(edl_bag a) {
 }
 
 // ---------------------------------- sort ----------------------------------
-// Least significant digit first, stable, up to 9 bits a pass. A pass counts
+// Least significant digit first, stable, 9 or 11 bits a pass. A pass counts
 // each tile's digits, adds the counts up by digit, and moves each tile's
 // items: ranked by the wave (ballots find equal digits), brought in order in
 // LDS, and written in runs. The first pass makes the keys from the ids.
@@ -196,13 +196,10 @@ struct Keys32 {  // an id of a table of V rows; V where it has none
     return (uint64_t)v < (uint64_t)V ? (K)v : (K)V;
   }
 };
-struct Keys32From {  // an id less the smallest, within 32 bits
+struct Keys32Of {  // an id's low 32 bits
   typedef uint32_t K;
   const int64_t* ids;
-  int64_t base;
-  __device__ K operator()(int64_t i) const {
-    return (K)((uint64_t)ids[i] - (uint64_t)base);
-  }
+  __device__ K operator()(int64_t i) const { return (K)ids[i]; }
 };
 struct Keys64 {  // any id; the sign bit turned, so that the order is theirs
   typedef uint64_t K;
@@ -218,7 +215,15 @@ struct KeysOf {  // what the pass before wrote
   __device__ K operator()(int64_t i) const { return keys[i]; }
 };
 
-constexpr int kBins = EDL_SORT_BINS;
+struct Plan4x11 {  // tiles of 256 * ITEMS, digits of up to BITS
+  static constexpr int ITEMS = 4, BITS = 11;
+};
+struct Plan4x9 {
+  static constexpr int ITEMS = 4, BITS = 9;
+};
+struct Plan16x9 {
+  static constexpr int ITEMS = 16, BITS = 9;
+};
 
 // the lanes among `in` whose digit of `bits` bits is this lane's
 __device__ inline uint64_t same_digit(uint32_t d, int bits, bool in) {
@@ -247,12 +252,13 @@ __device__ inline uint32_t rank_digit(volatile C* count, uint32_t d, int bits,
   return old + lower;
 }
 
-template <typename S, int ITEMS>
+template <typename S, typename P>
 __global__ __launch_bounds__(256) void sort_count_kernel(S src, int64_t N,
                                                          int shift, int bits,
                                                          int tiles,
                                                          uint32_t* counts) {
-  __shared__ uint32_t h[kBins];
+  constexpr int ITEMS = P::ITEMS;
+  __shared__ uint32_t h[1 << P::BITS];
   const int bins = 1 << bits;
   for (int d = threadIdx.x; d < bins; d += 256) h[d] = 0;
   __syncthreads();
@@ -307,18 +313,19 @@ __global__ __launch_bounds__(256) void sort_offsets_kernel(uint32_t* counts,
   if (threadIdx.x == 0) totals[blockIdx.x] = run;
 }
 
-template <typename S, bool FIRST, int ITEMS>
+template <typename S, bool FIRST, typename P>
 __global__ __launch_bounds__(256) void sort_move_kernel(
     S src, const uint32_t* __restrict__ pos_in, int64_t N, int shift, int bits,
     int tiles, const uint32_t* __restrict__ counts,
     const uint32_t* __restrict__ totals, typename S::K* __restrict__ keys_out,
     uint32_t* __restrict__ pos_out) {
   typedef typename S::K K;
-  constexpr int kTile = ITEMS * 256;
+  constexpr int ITEMS = P::ITEMS, kTile = ITEMS * 256, kBins = 1 << P::BITS;
+  constexpr int kOwn = kBins / 256;  // neighbouring digits to a thread
   __shared__ K s_key[kTile];
   __shared__ uint32_t s_pos[kTile];
-  __shared__ uint32_t cnt[4][kBins];
-  __shared__ uint32_t local[kBins];  // a digit's first place in the tile
+  __shared__ __align__(16) uint16_t cnt[4][kBins];  // a wave's, up to 1024
+  __shared__ uint16_t local[kBins];  // a digit's first place in the tile
   __shared__ uint32_t goal[kBins];   // where it goes, less that place
   __shared__ uint32_t s4[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -334,44 +341,47 @@ __global__ __launch_bounds__(256) void sort_move_kernel(
     key[k] = in ? src(i) : 0;
     pos[k] = in ? (FIRST ? (uint32_t)i : pos_in[i]) : 0;
   }
-  // two neighbouring digits to a thread
-  uint32_t tot[2], at_tile[2];
+  uint32_t tot[kOwn], at_tile[kOwn];
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int d = tid * 2 + q;
+  for (int q = 0; q < kOwn; ++q) {
+    const int d = tid * kOwn + q;
     tot[q] = d < bins ? totals[d] : 0;
     at_tile[q] = d < bins ? counts[(int64_t)d * tiles + blockIdx.x] : 0;
   }
-  for (int d = tid; d < 4 * kBins; d += 256) (&cnt[0][0])[d] = 0;
+  for (int d = tid; d < 2 * kBins; d += 256)
+    reinterpret_cast<uint32_t*>(&cnt[0][0])[d] = 0;
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k)
-    rank[k] = rank_digit<uint32_t>(
+    rank[k] = rank_digit<uint16_t>(
         cnt[wave], (uint32_t)(key[k] >> shift) & (bins - 1), bits,
         first + k * 64 < N);
   __syncthreads();
-  uint32_t sum[2];
+  uint32_t sum[kOwn], sums = 0, tots = 0;
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int d = tid * 2 + q;
+  for (int q = 0; q < kOwn; ++q) {
+    const int d = tid * kOwn + q;
     uint32_t s = 0;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const uint32_t t = cnt[w][d];
-      cnt[w][d] = s;
+      cnt[w][d] = (uint16_t)s;
       s += t;
     }
     sum[q] = s;
+    sums += s;
+    tots += tot[q];
   }
   uint32_t all;
-  const uint32_t l0 = block_scan(sum[0] + sum[1], s4, &all);
-  const uint32_t g0 = block_scan(tot[0] + tot[1], s4, &all);
+  uint32_t l0 = block_scan(sums, s4, &all);
+  uint32_t g0 = block_scan(tots, s4, &all);
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int d = tid * 2 + q;
-    const uint32_t at = l0 + (q ? sum[0] : 0);
-    local[d] = at;
-    goal[d] = g0 + (q ? tot[0] : 0) + at_tile[q] - at;
+  for (int q = 0; q < kOwn; ++q) {
+    const int d = tid * kOwn + q;
+    local[d] = (uint16_t)l0;
+    goal[d] = g0 + at_tile[q] - l0;
+    l0 += sum[q];
+    g0 += tot[q];
   }
   __syncthreads();
 #pragma unroll
@@ -400,7 +410,7 @@ __global__ __launch_bounds__(256) void sort_move_kernel(
 // UNIQUE: ids of any value, taken relative to the smallest. Also the unique
 // ids in order, each item's place among them, and for the host how many
 // there are (found[0]), or in found[1] that they lie too far apart for 32
-// bits, and nothing else.
+// bits, and places of zero.
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallItems = EDL_SORT_SMALL / kSmallThreads;
 constexpr int kSmallWaves = kSmallThreads / 64;
@@ -452,7 +462,10 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
     const uint64_t range = (uint64_t)mx - (uint64_t)mn;
     const bool far = range >> 32 != 0;
     if (tid == 0) found[1] = far;
-    if (far) return;  // all threads alike
+    if (far) {  // all threads alike; what is launched behind stays in bounds
+      for (int i = tid; i < N; i += kSmallThreads) keys_out[i] = pos_out[i] = 0;
+      return;
+    }
     low = mn;
     bits = range ? 64 - __clzll((long long)range) : 1;
 #pragma unroll
@@ -938,55 +951,73 @@ void launch_segments(const edl_segments& a, hipStream_t st) {
     else FN<_Float16, 1>(A, ST);                     \
   }
 
-// tiles of 1024 until there are enough of 4096 for the chip (160 thousand
-// ids: 14 us a move in 40 tiles of 4096)
-int sort_items(int64_t N) { return N < 1024 * 1024 ? 4 : 16; }
+// Up to 256 thousand items, a pass less counts for more than the runs in
+// which it writes (160 thousand of 21 bits: 77 us for a whole gradient with 2
+// passes of 11 bits, 92 with 3 of 7), and tiles of 1024 fill the chip until
+// there are a million (820 thousand: 167 us with 9 bits, 177 with 11, 204
+// with tiles of 4096).
+int sort_plan(int64_t N) {
+  return N < 256 * 1024 ? 0 : N < 1024 * 1024 ? 1 : 2;
+}
+#define EDL_BY_PLAN(N, CALL)                              \
+  (sort_plan(N) == 0   ? CALL(Plan4x11)                   \
+   : sort_plan(N) == 1 ? CALL(Plan4x9)                    \
+                       : CALL(Plan16x9))
 
-template <typename S, bool FIRST, int ITEMS>
+template <typename S, bool FIRST, typename P>
 int sort_pass(S src, const uint32_t* pos_in, int64_t N, int shift, int bits,
               uint32_t* counts, uint32_t* totals, typename S::K* keys_out,
               uint32_t* pos_out, hipStream_t st) {
-  const int tiles = (int)((N + ITEMS * 256 - 1) / (ITEMS * 256));
+  constexpr int kTile = P::ITEMS * 256;
+  const int tiles = (int)((N + kTile - 1) / kTile);
   const int bins = 1 << bits;
-  sort_count_kernel<S, ITEMS>
+  sort_count_kernel<S, P>
       <<<tiles, 256, 0, st>>>(src, N, shift, bits, tiles, counts);
   sort_offsets_kernel<<<bins, 256, 0, st>>>(counts, tiles, totals);
-  sort_move_kernel<S, FIRST, ITEMS><<<tiles, 256, 0, st>>>(
+  sort_move_kernel<S, FIRST, P><<<tiles, 256, 0, st>>>(
       src, pos_in, N, shift, bits, tiles, counts, totals, keys_out, pos_out);
   return (int)hipGetLastError();
 }
 
-// sorts into keys[0], pos[0], or keys[1], pos[1]: which, or -1 - error
-template <typename S, int ITEMS>
-int sort_by(S src, int64_t N, int bits, typename S::K* const* keys,
-            uint32_t* const* pos, uint32_t* counts, uint32_t* totals,
-            hipStream_t st) {
-  typedef typename S::K K;
-  const int passes = (bits + 8) / 9;
-  int done = 0, at = 0;
-  for (int p = 0; p < passes; ++p) {
-    const int left = passes - p, b = (bits - done + left - 1) / left;
-    int rc;
-    if (p == 0)
-      rc = sort_pass<S, true, ITEMS>(src, nullptr, N, done, b, counts, totals,
-                                     keys[0], pos[0], st);
-    else
-      rc = sort_pass<KeysOf<K>, false, ITEMS>(
-          KeysOf<K>{keys[at]}, pos[at], N, done, b, counts, totals,
-          keys[at ^ 1], pos[at ^ 1], st);
+// Sorts bits `done` to `bits` of keys[at], pos[at] into whichever buffer the
+// last pass ends with: returns which, or -1 - error.
+template <typename K, typename P>
+int sort_rest(int at, int done, int bits, int64_t N, K* const* keys,
+              uint32_t* const* pos, uint32_t* counts, uint32_t* totals,
+              hipStream_t st) {
+  while (done < bits) {
+    const int left = (bits - done + P::BITS - 1) / P::BITS;
+    const int b = (bits - done + left - 1) / left;
+    const int rc = sort_pass<KeysOf<K>, false, P>(
+        KeysOf<K>{keys[at]}, pos[at], N, done, b, counts, totals,
+        keys[at ^ 1], pos[at ^ 1], st);
     if (rc) return -1 - rc;
-    if (p) at ^= 1;
+    at ^= 1;
     done += b;
   }
   return at;
+}
+// all of it; the first pass, into keys[0], makes the keys from src
+template <typename S, typename P>
+int sort_by(S src, int64_t N, int bits, typename S::K* const* keys,
+            uint32_t* const* pos, uint32_t* counts, uint32_t* totals,
+            hipStream_t st) {
+  const int passes = (bits + P::BITS - 1) / P::BITS;
+  const int b = (bits + passes - 1) / passes;
+  const int rc = sort_pass<S, true, P>(src, nullptr, N, 0, b, counts, totals,
+                                       keys[0], pos[0], st);
+  if (rc) return -1 - rc;
+  return sort_rest<typename S::K, P>(0, b, bits, N, keys, pos, counts, totals,
+                                     st);
 }
 template <typename S>
 int sort_all(S src, int64_t N, int bits, typename S::K* const* keys,
              uint32_t* const* pos, uint32_t* counts, uint32_t* totals,
              hipStream_t st) {
-  return sort_items(N) == 4
-             ? sort_by<S, 4>(src, N, bits, keys, pos, counts, totals, st)
-             : sort_by<S, 16>(src, N, bits, keys, pos, counts, totals, st);
+#define EDL_SORT_BY(P) \
+  sort_by<S, P>(src, N, bits, keys, pos, counts, totals, st)
+  return EDL_BY_PLAN(N, EDL_SORT_BY);
+#undef EDL_SORT_BY
 }
 
 template <typename K>
@@ -1047,8 +1078,10 @@ extern "C" int edl_segment_chunk(int64_t N, int D, int vec) {
 
 // how many counts a sort of N items needs
 extern "C" int64_t edl_sort_counts(int64_t N) {
-  const int64_t tile = sort_items(N) * 256;
-  return (N + tile - 1) / tile * EDL_SORT_BINS;
+#define EDL_COUNTS(P) \
+  ((N + P::ITEMS * 256 - 1) / (P::ITEMS * 256) << P::BITS)
+  return EDL_BY_PLAN(N, EDL_COUNTS);
+#undef EDL_COUNTS
 }
 
 // the small sort of ids of any value: see the kernel
@@ -1056,8 +1089,8 @@ extern "C" int edl_sort_unique_small(const int64_t* ids, int64_t N,
                                      uint32_t* place, uint32_t* pos,
                                      int64_t* unique, uint32_t* found,
                                      hipStream_t st) {
-  sort_small_kernel<Keys32From, true><<<1, kSmallThreads, 0, st>>>(
-      Keys32From{ids, 0}, (int)N, 0, place, pos, unique, found);
+  sort_small_kernel<Keys32Of, true><<<1, kSmallThreads, 0, st>>>(
+      Keys32Of{ids}, (int)N, 0, place, pos, unique, found);
   return (int)hipGetLastError();
 }
 
@@ -1068,12 +1101,28 @@ extern "C" int edl_ids_range(const int64_t* ids, int64_t N, int64_t* range,
   return (int)hipGetLastError();
 }
 
-extern "C" int edl_sort_ids32(const int64_t* ids, int64_t base, int bits,
-                              int64_t N, uint32_t* const* keys,
-                              uint32_t* const* pos, uint32_t* counts,
-                              uint32_t* totals, hipStream_t st) {
-  return sort_all(Keys32From{ids, base}, N, bits, keys, pos, counts, totals,
-                  st);
+// Ids whose bits from the 32nd up are all the same, by their low bits. The
+// first pass, over `first` bits into keys[0], needs not know how many: it is
+// launched while the host still waits for their range.
+extern "C" int edl_sort_ids32_first(const int64_t* ids, int first, int64_t N,
+                                    uint32_t* const* keys,
+                                    uint32_t* const* pos, uint32_t* counts,
+                                    uint32_t* totals, hipStream_t st) {
+  Keys32Of src{ids};
+#define EDL_FIRST(P)                                                        \
+  sort_pass<Keys32Of, true, P>(src, nullptr, N, 0, first, counts, totals,   \
+                               keys[0], pos[0], st)
+  return EDL_BY_PLAN(N, EDL_FIRST);
+#undef EDL_FIRST
+}
+extern "C" int edl_sort_ids32_rest(int first, int bits, int64_t N,
+                                   uint32_t* const* keys, uint32_t* const* pos,
+                                   uint32_t* counts, uint32_t* totals,
+                                   hipStream_t st) {
+#define EDL_REST(P)                                                         \
+  sort_rest<uint32_t, P>(0, first, bits, N, keys, pos, counts, totals, st)
+  return EDL_BY_PLAN(N, EDL_REST);
+#undef EDL_REST
 }
 
 extern "C" int edl_sort_ids64(const int64_t* ids, int64_t N,
