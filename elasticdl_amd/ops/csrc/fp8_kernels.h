@@ -48,7 +48,6 @@ struct edl_fp8_gemm {
   bool c_wide;    // 16-byte stores of 16 neighbours are aligned
   uint8_t* mask;  // relu: bits of c > 0, rows mask_ld bytes apart; may be null
   int64_t mask_ld;
-  bool wide;    // in bf16, with sums in 32 bits
   int splits;   // over the contraction
   float* part;  // [splits, M, part_ld] where splits > 1
   int64_t part_ld;  // N rounded up to 16

@@ -14,10 +14,11 @@
 // neighbouring products with about 16 bits below the largest of them (32
 // only between such groups): 1.6e-5 of a result's norm, measured over random
 // e4m3. That is far below e4m3's and a 16-bit result's own rounding, but not
-// 32 bits. So where a result is returned in 32 bits, and where the sign of
-// a sum decides a relu's gradient, the bytes are widened to bf16 in
-// registers on the way (exactly, scale included) and multiplied by the bf16
-// instruction, whose sums hold 24 bits (8e-9 measured), at half the rate.
+// 32 bits. So where a result is returned in 32 bits the bytes are widened to
+// bf16 in registers on the way (exactly, scale included) and multiplied by
+// the bf16 instruction, whose sums hold 24 bits (8e-9 measured), at half the
+// rate. And where the sign of a 16-bit result decides a relu's gradient, the
+// few sums that lie near zero are added up once more in 32 bits (settle).
 //
 // Layout. A matrix [R, C] that is contracted over C is stored as bytes
 // [R, Cp], Cp = C rounded up to 128 (zeros behind C), with scales
@@ -35,6 +36,7 @@ typedef __attribute__((ext_vector_type(8))) int i32x8;
 typedef __attribute__((ext_vector_type(4))) int i32x4;
 typedef __attribute__((ext_vector_type(2))) int i32x2;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
+typedef __attribute__((ext_vector_type(2))) float f32x2;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
@@ -462,54 +464,126 @@ __device__ inline f32x4 mfma_wide(const Wide& a, const Wide& b, f32x4 c) {
   return c;
 }
 
-// 16 neighbours of a row of C, from column n
-__device__ inline void epilogue16(const edl_fp8_gemm& g, int64_t m, int64_t n,
-                                  float* v) {
-  const int type = g.c_type;
-  if (g.bias) {
+// one element of A B^T by a whole wave, in 32 bits
+__device__ inline float dot_of(const edl_fp8_gemm& g, int64_t m, int64_t n,
+                               int lane) {
+  const uint8_t *pa = g.a + m * g.ld, *pb = g.b + n * g.ld;
+  const uint8_t *ps = g.sa + scale_slot(m), *pt = g.sb + scale_slot(n);
+  float t = 0.f;
+  for (int64_t k = lane * 16; k < g.ld; k += 1024) {
+    const i32x4 a = *reinterpret_cast<const i32x4*>(pa + k);
+    const i32x4 b = *reinterpret_cast<const i32x4*>(pb + k);
+    const int64_t kb = k / kBlk;
+    const float sa = scale_value(ps[kb * g.a_rp], 0);
+    const float sb = scale_value(pt[kb * g.b_rp], 0);
+    float u = 0.f;
 #pragma unroll
-    for (int k = 0; k < 16; ++k)
-      if (n + k < g.N) v[k] += load_any(g.bias, n + k, g.bias_type);
+    for (int q = 0; q < 4; ++q) {
+      const f32x2 a0 = __builtin_amdgcn_cvt_pk_f32_fp8(a[q], false);
+      const f32x2 a1 = __builtin_amdgcn_cvt_pk_f32_fp8(a[q], true);
+      const f32x2 b0 = __builtin_amdgcn_cvt_pk_f32_fp8(b[q], false);
+      const f32x2 b1 = __builtin_amdgcn_cvt_pk_f32_fp8(b[q], true);
+      u = __builtin_fmaf(a0[0], b0[0], u);
+      u = __builtin_fmaf(a0[1], b0[1], u);
+      u = __builtin_fmaf(a1[0], b1[0], u);
+      u = __builtin_fmaf(a1[1], b1[1], u);
+    }
+    t += u * sa * sb;
   }
+  for (int o = 1; o < 64; o <<= 1) t += __shfl_xor(t, o);
+  return t;
+}
+
+// Of a lane's 16 sums v (bias apart), those that with their bias lie within
+// 2^-12 of the neighbours' size from zero are replaced by dot_of. The size is
+// the squared mean of roots, which a single large neighbour hardly moves; 2^-12
+// is 11 times the usual error of a sum. One value in 8000 is met; each takes
+// the wave some 2 us, and a wave stops after 32 of its 1024.
+__device__ inline void settle(const edl_fp8_gemm& g, int64_t m, int64_t n,
+                              float* v, const float* bias, bool live) {
+  const int lane = threadIdx.x & 63;
+  float size = 0.f;
+#pragma unroll
+  for (int k = 0; k < 16; ++k)
+    if (n + k < g.N) size += __builtin_amdgcn_sqrtf(__builtin_fabsf(v[k]));
+  size *= 1.f / 16;
+  size *= size * (1.f / 4096);
+  uint32_t near = 0;
+#pragma unroll
+  for (int k = 0; k < 16; ++k)
+    near |= (n + k < g.N && __builtin_fabsf(v[k] + bias[k]) < size ? 1u : 0u)
+            << k;
+  if (!live || !(size < 3e38f)) near = 0;
+  for (int met = 0; met < 32; ++met) {
+    const uint64_t who = __ballot(near != 0);
+    if (who == 0) break;
+    const int at = __builtin_ctzll(who);
+    const int k = __builtin_ctz(__builtin_amdgcn_readlane((int)near, at));
+    const int64_t row = __builtin_amdgcn_readlane((int)m, at);
+    const int64_t col = __builtin_amdgcn_readlane((int)n, at) + k;
+    const float z = dot_of(g, row, col, lane);
+    if (lane == at) {
+      near &= near - 1;
+#pragma unroll
+      for (int q = 0; q < 16; ++q) v[q] = q == k ? z : v[q];
+    }
+  }
+}
+
+template <typename T>
+struct TypeOf;
+template <>
+struct TypeOf<float> {
+  static constexpr bool wide = true;  // sums in 32 bits
+};
+template <>
+struct TypeOf<__bf16> {
+  static constexpr bool wide = false;
+};
+template <>
+struct TypeOf<_Float16> {
+  static constexpr bool wide = false;
+};
+
+__device__ inline void load_bias16(const edl_fp8_gemm& g, int64_t n,
+                                   float* bias) {
+#pragma unroll
+  for (int k = 0; k < 16; ++k)
+    bias[k] = g.bias && n + k < g.N ? load_any(g.bias, n + k, g.bias_type)
+                                    : 0.f;
+}
+
+// 16 neighbours of a row of C, from column n; live: the row and column n are
+// C's. Whole waves call it.
+template <typename T>
+__device__ inline void epilogue16(const edl_fp8_gemm& g, int64_t m, int64_t n,
+                                  float* v, const float* bias, bool live) {
+  if (!TypeOf<T>::wide && g.mask) settle(g, m, n, v, bias, live);
+  if (!live) return;
   uint32_t bits = 0;
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
+    v[k] += bias[k];
     bits |= (v[k] > 0.f ? 1u : 0u) << k;
     v[k] = activate(v[k], g.act);
   }
   if (g.mask)
     *reinterpret_cast<uint16_t*>(g.mask + m * g.mask_ld + (n >> 3)) = bits;
-  const int64_t at = m * g.N + n;
+  T* p = static_cast<T*>(g.c) + m * g.N + n;
   if (n + 16 <= g.N && g.c_wide) {
-    if (type == EDL_T_F32) {
-      float* p = static_cast<float*>(g.c) + at;
+    constexpr int W = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(W)));
 #pragma unroll
-      for (int k = 0; k < 16; k += 4)
-        *reinterpret_cast<f32x4*>(p + k) =
-            (f32x4){v[k], v[k + 1], v[k + 2], v[k + 3]};
-    } else if (type == EDL_T_BF16) {
-      __bf16* p = static_cast<__bf16*>(g.c) + at;
+    for (int k = 0; k < 16; k += W) {
+      vec o;
 #pragma unroll
-      for (int k = 0; k < 16; k += 8) {
-        bf16x8 o;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) o[q] = (__bf16)v[k + q];
-        *reinterpret_cast<bf16x8*>(p + k) = o;
-      }
-    } else {
-      _Float16* p = static_cast<_Float16*>(g.c) + at;
-#pragma unroll
-      for (int k = 0; k < 16; k += 8) {
-        f16x8 o;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) o[q] = (_Float16)v[k + q];
-        *reinterpret_cast<f16x8*>(p + k) = o;
-      }
+      for (int q = 0; q < W; ++q) o[q] = (T)v[k + q];
+      *reinterpret_cast<vec*>(p + k) = o;
     }
   } else {
 #pragma unroll
     for (int k = 0; k < 16; ++k)
-      if (n + k < g.N) store_any(g.c, at + k, v[k], type);
+      if (n + k < g.N) p[k] = (T)v[k];
   }
 }
 
@@ -518,11 +592,12 @@ struct GemmLds {  // two buffers each: A's, B's, scales (256 of A's and B's)
   __align__(1024) uint8_t m[4 * BM * kBlk + 1024];
 };
 
-template <int WM, int WN, int FM, int FN, bool WIDE>
+template <int WM, int WN, int FM, int FN, typename T>
 __device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
                                  uint8_t* smem) {
+  constexpr bool WIDE = TypeOf<T>::wide;
   constexpr int BM = WM * FM * 16, BN = WN * FN * 16, NW = WM * WN;
-  static_assert(FN == 4 && FM % 4 == 0, "scale words hold four fragments");
+  static_assert(FN % 4 == 0 && FM % 4 == 0, "scale words: four fragments");
   static_assert(BM == BN && (BM == 128 || BM == 256), "buffers' toggle");
   constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW;  // 1 KB loads a wave
   constexpr uint32_t kTile = BM * kBlk, kB = 2 * kTile, kS = 4 * kTile;
@@ -543,7 +618,7 @@ __device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
   // this split's share of the steps
   const int kb_all = (int)(g.ld / kBlk);
   const int kb0 = (int)((int64_t)kb_all * split / g.splits);
-  const int T = (int)((int64_t)kb_all * (split + 1) / g.splits) - kb0;
+  const int steps = (int)((int64_t)kb_all * (split + 1) / g.splits) - kb0;
 
   // one load fills 8 rows: lane -> row lane>>3, slot lane&7
   const uint8_t* pa = g.a + m0 * g.ld + (int64_t)kb0 * kBlk;
@@ -611,17 +686,29 @@ __device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
     for (int k = 0; k < FN; ++k) acc[i][k] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
   i32x8 a[FM], b[FN];
-  int sa[FM / 4], sb, na[FM / 4], nb;
+  int sa[FM / 4], sb[FN / 4], na[FM / 4], nb[FN / 4];
   auto read_scales = [&]() {
 #pragma unroll
     for (int k = 0; k < FM / 4; ++k)
       na[k] = *reinterpret_cast<const int*>(smem + sAt + wA + k * 64);
-    nb = *reinterpret_cast<const int*>(smem + sAt + 256 + wB);
+#pragma unroll
+    for (int k = 0; k < FN / 4; ++k)
+      nb[k] = *reinterpret_cast<const int*>(smem + sAt + 256 + wB + k * 64);
+  };
+  auto next_scales = [&]() {
+#pragma unroll
+    for (int k = 0; k < FM / 4; ++k) sa[k] = na[k];
+#pragma unroll
+    for (int k = 0; k < FN / 4; ++k) sb[k] = nb[k];
+  };
+  auto product = [&](int i, int k) {
+    acc[i][k] = mfma_sel(k & 3, i & 3, b[k], a[i], acc[i][k], sb[k >> 2],
+                         sa[i >> 2]);
   };
   Wide bw[WIDE ? FN : 1];
   auto widen_b = [&]() {
 #pragma unroll
-    for (int k = 0; k < FN; ++k) bw[k] = widen(b[k], scale_value(sb, k));
+    for (int k = 0; k < FN; ++k) bw[k] = widen(b[k], scale_value(sb[k >> 2], k & 3));
   };
   auto rows_of = [&](int i) {  // fragment i of A against all of B
     if (WIDE) {
@@ -630,9 +717,7 @@ __device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
       for (int k = 0; k < FN; ++k) acc[i][k] = mfma_wide(bw[k], aw, acc[i][k]);
     } else {
 #pragma unroll
-      for (int k = 0; k < FN; ++k)
-        acc[i][k] =
-            mfma_sel(k, i & 3, b[k], a[i], acc[i][k], sb, sa[i >> 2]);
+      for (int k = 0; k < FN; ++k) product(i, k);
     }
   };
   auto step = [&](uint32_t buf, bool more) {
@@ -665,27 +750,21 @@ __device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
     } else {
 #pragma unroll
       for (int k = 0; k < FN; ++k) {
-#pragma unroll
-        for (int i = FM - 2; i < FM; ++i)
-          acc[i][k] =
-              mfma_sel(k, i & 3, b[k], a[i], acc[i][k], sb, sa[i >> 2]);
+        product(FM - 2, k);
+        product(FM - 1, k);
         __builtin_amdgcn_sched_barrier(0);
         b[k] = frag(bLo, bHi, k);
       }
     }
-#pragma unroll
-    for (int k = 0; k < FM / 4; ++k) sa[k] = na[k];
-    sb = nb;
+    next_scales();
   };
 
   stage(0);
-  if (T > 1) stage(1);
+  if (steps > 1) stage(1);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   read_scales();
-#pragma unroll
-  for (int k = 0; k < FM / 4; ++k) sa[k] = na[k];
-  sb = nb;
+  next_scales();
   a[0] = frag(aLo, aHi, 0);
   a[1] = frag(aLo, aHi, 1);
 #pragma unroll
@@ -693,58 +772,81 @@ __device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
   // the last two steps fetch no more; a branch in the loop's body would let
   // the compiler move matrix instructions behind the barrier
   int t = 0;
-  for (; t + 2 < T; ++t) step(t & 1, true);
-  for (; t < T; ++t) step(t & 1, false);
+  for (; t + 2 < steps; ++t) step(t & 1, true);
+  for (; t < steps; ++t) step(t & 1, false);
 
-  // lane: row rr + 4 i of C's 64, columns q4*16 + k*4 + 0..3
-  const int64_t n = n0 + wn * FN * 16 + q4 * 16;
-  if (n >= g.N) return;
+  // lane: row rr + 4 i of C's 64, columns q4*16 + k*4 + 0..3 of its 64. The
+  // sums pass through LDS, each lane's own, so that one copy of the code
+  // below takes all rows: unrolled, the large tile's 16 would not stay in
+  // registers.
+  __syncthreads();
+  f32x4* own = reinterpret_cast<f32x4*>(smem) + wave * (4 * 4 * 64) + lane;
+  static_assert(NW * 4 * 4 * 64 * 16 <= 4 * BM * kBlk, "");
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    int64_t m = m0 + wm * FM * 16 + (i >> 2) * 64 + rr + (i & 3) * 4;
-    if (m >= g.M) continue;
-    float v[16];
+  for (int h = 0; h < FM / 4 * (FN / 4); ++h) {  // 64 x 64 at a time
+    const int j = h % (FN / 4), i0 = h / (FN / 4) * 4;
+    const int64_t n = n0 + wB + j * 64 + q4 * 16;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) v[k] = acc[i][k >> 2][k & 3];
-    if (g.splits > 1) {
-      float* p = g.part + ((int64_t)split * g.M + m) * g.part_ld + n;
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int k = 0; k < 16; k += 4)
-        *reinterpret_cast<f32x4*>(p + k) =
-            (f32x4){v[k], v[k + 1], v[k + 2], v[k + 3]};
-    } else {
-      epilogue16(g, m, n, v);
+      for (int k = 0; k < 4; ++k)
+        own[(i * 4 + k) * 64] = acc[i0 + i][j * 4 + k];
+    float bias[16];
+    load_bias16(g, n, bias);
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+      const int64_t m = m0 + wA + i0 * 16 + rr + i * 4;
+      const bool live = m < g.M && n < g.N;
+      float v[16];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const f32x4 u = own[(i * 4 + k) * 64];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[k * 4 + q] = u[q];
+      }
+      if (BM == 128 && g.splits > 1) {
+        float* p = g.part + ((int64_t)split * g.M + m) * g.part_ld + n;
+        if (live) {
+#pragma unroll
+          for (int k = 0; k < 16; k += 4)
+            *reinterpret_cast<f32x4*>(p + k) =
+                (f32x4){v[k], v[k + 1], v[k + 2], v[k + 3]};
+        }
+      } else {
+        epilogue16<T>(g, m, n, v, bias, live);
+      }
     }
   }
 }
 
-template <int WM, int WN, int FM, int FN, bool WIDE>
-__global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(
+template <int WM, int WN, int FM, int FN, typename T>
+__global__ __launch_bounds__(WM* WN * 64, FN > 4 ? 1 : 2) void gemm_kernel(
     edl_fp8_gemm g) {
   __shared__ GemmLds<WM * FM * 16> lds;
-  gemm_tile<WM, WN, FM, FN, WIDE>(g, blockIdx.x, gridDim.x, lds.m);
+  gemm_tile<WM, WN, FM, FN, T>(g, blockIdx.x, gridDim.x, lds.m);
 }
 
 // the two products of a backward pass in one launch, each of 128 x 128
-template <bool WIDE0, bool WIDE1>
+template <typename T0, typename T1>
 __global__ __launch_bounds__(256, 2) void gemm_pair_kernel(edl_fp8_gemm g0,
                                                            edl_fp8_gemm g1,
                                                            int blocks0) {
   __shared__ GemmLds<128> lds;
   if ((int)blockIdx.x < blocks0)
-    gemm_tile<2, 2, 4, 4, WIDE0>(g0, blockIdx.x, blocks0, lds.m);
+    gemm_tile<2, 2, 4, 4, T0>(g0, blockIdx.x, blocks0, lds.m);
   else
-    gemm_tile<2, 2, 4, 4, WIDE1>(g1, blockIdx.x - blocks0,
-                                 gridDim.x - blocks0, lds.m);
+    gemm_tile<2, 2, 4, 4, T1>(g1, blockIdx.x - blocks0, gridDim.x - blocks0,
+                              lds.m);
 }
 
 // joins a product's splits in order; a thread takes 16 neighbours of a row
-__device__ inline void gemm_join(const edl_fp8_gemm& g, int64_t block) {
+template <typename T>
+__device__ inline void gemm_join_as(const edl_fp8_gemm& g, int64_t block) {
   const int64_t each = g.part_ld / 16;
   const int64_t id = block * 256 + threadIdx.x;
-  if (id >= g.M * each) return;
-  const int64_t m = id / each, n = (id % each) * 16;
-  float v[16];
+  const bool live = id < g.M * each;
+  const int64_t m = live ? id / each : 0, n = live ? (id % each) * 16 : 0;
+  float v[16], bias[16];
 #pragma unroll
   for (int k = 0; k < 16; ++k) v[k] = 0.f;
   for (int s = 0; s < g.splits; ++s) {
@@ -756,7 +858,16 @@ __device__ inline void gemm_join(const edl_fp8_gemm& g, int64_t block) {
       for (int q = 0; q < 4; ++q) v[k + q] += u[q];
     }
   }
-  epilogue16(g, m, n, v);
+  load_bias16(g, n, bias);
+  epilogue16<T>(g, m, n, v, bias, live);
+}
+__device__ inline void gemm_join(const edl_fp8_gemm& g, int64_t block) {
+  if (g.c_type == EDL_T_F32)
+    gemm_join_as<float>(g, block);
+  else if (g.c_type == EDL_T_BF16)
+    gemm_join_as<__bf16>(g, block);
+  else
+    gemm_join_as<_Float16>(g, block);
 }
 
 // what is left when a pass's products are done: the joins of up to two of
@@ -875,10 +986,10 @@ int64_t tiles256(const edl_fp8_gemm& g) {
 
 // Which kernel. 256 x 256 reads each operand half as often but runs one
 // workgroup a CU, so it takes the products that give each of the 256 CUs
-// one. In 32 bits (wide) a wave's fragments take twice the registers: always
+// one. In 32 bits a wave's fragments take twice the registers: always
 // 128 x 128.
 bool takes_256(const edl_fp8_gemm& g) {
-  return !g.wide && tiles256(g) >= 256;
+  return g.c_type != EDL_T_F32 && tiles256(g) >= 256;
 }
 
 }  // namespace
@@ -921,18 +1032,40 @@ extern "C" void edl_fp8_gemm_splits(edl_fp8_gemm* g, int n) {
   }
 }
 
-static int launch_one(const edl_fp8_gemm& g, hipStream_t st) {
-  if (takes_256(g)) {
-    gemm_kernel<2, 4, 8, 4, false>
+template <typename T>
+static void launch_as(const edl_fp8_gemm& g, hipStream_t st) {
+  if (takes_256(g))
+    gemm_kernel<2, 4, 8, 4, T>
         <<<dim3((unsigned)tiles256(g)), dim3(512), 0, st>>>(g);
-  } else {
-    dim3 grid((unsigned)(tiles128(g) * g.splits)), block(256);
-    if (g.wide)
-      gemm_kernel<2, 2, 4, 4, true><<<grid, block, 0, st>>>(g);
-    else
-      gemm_kernel<2, 2, 4, 4, false><<<grid, block, 0, st>>>(g);
-  }
+  else
+    gemm_kernel<2, 2, 4, 4, T>
+        <<<dim3((unsigned)(tiles128(g) * g.splits)), dim3(256), 0, st>>>(g);
+}
+static int launch_one(const edl_fp8_gemm& g, hipStream_t st) {
+  if (g.c_type == EDL_T_F32)
+    gemm_kernel<2, 2, 4, 4, float>
+        <<<dim3((unsigned)(tiles128(g) * g.splits)), dim3(256), 0, st>>>(g);
+  else if (g.c_type == EDL_T_BF16)
+    launch_as<__bf16>(g, st);
+  else
+    launch_as<_Float16>(g, st);
   return (int)hipGetLastError();
+}
+template <typename T0, typename T1>
+static void launch_pair(const edl_fp8_gemm* g, hipStream_t st) {
+  const int b0 = (int)tiles128(g[0]) * g[0].splits;
+  const int b1 = (int)tiles128(g[1]) * g[1].splits;
+  gemm_pair_kernel<T0, T1>
+      <<<dim3((unsigned)(b0 + b1)), dim3(256), 0, st>>>(g[0], g[1], b0);
+}
+template <typename T0>
+static void launch_pair_as(const edl_fp8_gemm* g, hipStream_t st) {
+  if (g[1].c_type == EDL_T_F32)
+    launch_pair<T0, float>(g, st);
+  else if (g[1].c_type == EDL_T_BF16)
+    launch_pair<T0, __bf16>(g, st);
+  else
+    launch_pair<T0, _Float16>(g, st);
 }
 
 // n products (0 to 2), their joins, and where f's sums are not null a
@@ -941,17 +1074,12 @@ extern "C" int edl_fp8_gemm_run(edl_fp8_finish* f, int n, hipStream_t st) {
   edl_fp8_gemm* g = f->g;
   int rc = 0;
   if (n == 2 && !takes_256(g[0]) && !takes_256(g[1])) {
-    const int b0 = (int)tiles128(g[0]) * g[0].splits;
-    dim3 grid((unsigned)(b0 + tiles128(g[1]) * g[1].splits)), block(256);
-    const bool w0 = g[0].wide, w1 = g[1].wide;
-    if (w0 && w1)
-      gemm_pair_kernel<true, true><<<grid, block, 0, st>>>(g[0], g[1], b0);
-    else if (w0)
-      gemm_pair_kernel<true, false><<<grid, block, 0, st>>>(g[0], g[1], b0);
-    else if (w1)
-      gemm_pair_kernel<false, true><<<grid, block, 0, st>>>(g[0], g[1], b0);
+    if (g[0].c_type == EDL_T_F32)
+      launch_pair_as<float>(g, st);
+    else if (g[0].c_type == EDL_T_BF16)
+      launch_pair_as<__bf16>(g, st);
     else
-      gemm_pair_kernel<false, false><<<grid, block, 0, st>>>(g[0], g[1], b0);
+      launch_pair_as<_Float16>(g, st);
     rc = (int)hipGetLastError();
   } else {
     for (int i = 0; i < n && rc == 0; ++i) rc = launch_one(g[i], st);
