@@ -469,45 +469,81 @@ __device__ inline float dot_of(const edl_fp8_gemm& g, int64_t m, int64_t n,
                                int lane) {
   const uint8_t *pa = g.a + m * g.ld, *pb = g.b + n * g.ld;
   const uint8_t *ps = g.sa + scale_slot(m), *pt = g.sb + scale_slot(n);
+  constexpr int U = 4;  // loads in flight: a wave waits here for nothing else
   float t = 0.f;
-  for (int64_t k = lane * 16; k < g.ld; k += 1024) {
-    const i32x4 a = *reinterpret_cast<const i32x4*>(pa + k);
-    const i32x4 b = *reinterpret_cast<const i32x4*>(pb + k);
-    const int64_t kb = k / kBlk;
-    const float sa = scale_value(ps[kb * g.a_rp], 0);
-    const float sb = scale_value(pt[kb * g.b_rp], 0);
-    float u = 0.f;
+  for (int64_t k0 = lane * 16; k0 < g.ld; k0 += 1024 * U) {
+    i32x4 a[U], b[U];
+    float s[U];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f32x2 a0 = __builtin_amdgcn_cvt_pk_f32_fp8(a[q], false);
-      const f32x2 a1 = __builtin_amdgcn_cvt_pk_f32_fp8(a[q], true);
-      const f32x2 b0 = __builtin_amdgcn_cvt_pk_f32_fp8(b[q], false);
-      const f32x2 b1 = __builtin_amdgcn_cvt_pk_f32_fp8(b[q], true);
-      u = __builtin_fmaf(a0[0], b0[0], u);
-      u = __builtin_fmaf(a0[1], b0[1], u);
-      u = __builtin_fmaf(a1[0], b1[0], u);
-      u = __builtin_fmaf(a1[1], b1[1], u);
+    for (int u = 0; u < U; ++u) {
+      const bool in = k0 + u * 1024 < g.ld;
+      const int64_t k = in ? k0 + u * 1024 : k0, kb = k / kBlk;
+      a[u] = *reinterpret_cast<const i32x4*>(pa + k);
+      b[u] = *reinterpret_cast<const i32x4*>(pb + k);
+      const float sa = scale_value(ps[kb * g.a_rp], 0);
+      s[u] = in ? sa * scale_value(pt[kb * g.b_rp], 0) : 0.f;
     }
-    t += u * sa * sb;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float d = 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x2 a0 = __builtin_amdgcn_cvt_pk_f32_fp8(a[u][q], false);
+        const f32x2 a1 = __builtin_amdgcn_cvt_pk_f32_fp8(a[u][q], true);
+        const f32x2 b0 = __builtin_amdgcn_cvt_pk_f32_fp8(b[u][q], false);
+        const f32x2 b1 = __builtin_amdgcn_cvt_pk_f32_fp8(b[u][q], true);
+        d = __builtin_fmaf(a0[0], b0[0], d);
+        d = __builtin_fmaf(a0[1], b0[1], d);
+        d = __builtin_fmaf(a1[0], b1[0], d);
+        d = __builtin_fmaf(a1[1], b1[1], d);
+      }
+      t = __builtin_fmaf(d, s[u], t);
+    }
   }
   for (int o = 1; o < 64; o <<= 1) t += __shfl_xor(t, o);
   return t;
 }
 
+// sum over the 16 lanes of a row of lanes; those that are off add nothing
+template <int CTRL>
+__device__ inline float add_ror(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(
+                 0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+__device__ inline float sum16(float v) {
+  return add_ror<0x121>(add_ror<0x122>(add_ror<0x124>(add_ror<0x128>(v))));
+}
+
 // Of a lane's 16 sums v (bias apart), those that with their bias lie within
-// 2^-12 of the neighbours' size from zero are replaced by dot_of. The size is
-// the squared mean of roots, which a single large neighbour hardly moves; 2^-12
-// is 11 times the usual error of a sum. One value in 8000 is met; each takes
-// the wave some 2 us, and a wave stops after 32 of its 1024.
+// 2^-13 of their neighbours' size from zero are replaced by dot_of. The size
+// is a mean, and of the means of every other neighbour the smaller, which one
+// large value does not move; at C's right edge, over 16 rows. 2^-13 of it is
+// 6 times the usual error of a sum. One value in 15000 is met; each takes the
+// wave some 3 us, and a wave stops after 32 of its 1024.
 __device__ inline void settle(const edl_fp8_gemm& g, int64_t m, int64_t n,
                               float* v, const float* bias, bool live) {
   const int lane = threadIdx.x & 63;
-  float size = 0.f;
+  float sum[2] = {0.f, 0.f}, count[2] = {8.f, 8.f};
 #pragma unroll
   for (int k = 0; k < 16; ++k)
-    if (n + k < g.N) size += __builtin_amdgcn_sqrtf(__builtin_fabsf(v[k]));
-  size *= 1.f / 16;
-  size *= size * (1.f / 4096);
+    sum[k & 1] += n + k < g.N ? __builtin_fabsf(v[k]) : 0.f;
+  if (g.N & 15) {  // all lanes alike
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int in = n >= g.N || !live ? 0
+                     : n + 16 <= g.N   ? 8
+                                       : (int)(g.N - n + 1 - h) / 2;
+      const float rows = sum16(live ? sum[h] : 0.f);
+      const float of = sum16((float)in);
+      if (n + 16 > g.N) {
+        sum[h] = rows;
+        count[h] = of;
+      }
+    }
+  }
+  const float a = count[0] > 0.f ? sum[0] / count[0] : 0.f;
+  const float b = count[1] > 0.f ? sum[1] / count[1] : a;
+  const float size = (a < b ? a : b) * (1.f / 8192);
   uint32_t near = 0;
 #pragma unroll
   for (int k = 0; k < 16; ++k)
@@ -648,17 +684,23 @@ __device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
   const uint32_t lds0 =
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
   uint32_t at = 0, atS = 0;
-  auto stage = [&](uint32_t buf) {  // the next block
-#pragma unroll
-    for (int q = 0; q < LA; ++q)
+  constexpr int kLoads = LA + LB + 1;
+  auto load = [&](uint32_t buf, int q) {  // the q-th of the next block's
+    if (q < LA) {
       dma16(bufA, offA[q], at, lds0 + buf * kTile + (wave * LA + q) * 1024);
+    } else if (q < LA + LB) {
+      const int o = q - LA;
+      dma16(bufB, offB[o], at,
+            lds0 + kB + buf * kTile + (wave * LB + o) * 1024);
+    } else if (q == LA + LB) {
+      dma4(bufS, lane * 4, atS, lds0 + kS + buf * 512 + odd * 256);
+      at += kBlk;
+      atS += (uint32_t)rp;
+    }
+  };
+  auto stage = [&](uint32_t buf) {
 #pragma unroll
-    for (int q = 0; q < LB; ++q)
-      dma16(bufB, offB[q], at,
-            lds0 + kB + buf * kTile + (wave * LB + q) * 1024);
-    dma4(bufS, lane * 4, atS, lds0 + kS + buf * 512 + odd * 256);
-    at += kBlk;
-    atS += (uint32_t)rp;
+    for (int q = 0; q < kLoads; ++q) load(buf, q);
   };
 
   // fragment f of a wave's rows: 32 bytes of row rr, in chunks q4 and 4 + q4.
@@ -720,17 +762,29 @@ __device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
       for (int k = 0; k < FN; ++k) product(i, k);
     }
   };
-  auto step = [&](uint32_t buf, bool more) {
+  // Block t + 1 goes into the other buffer in two parts: kEarly loads at the
+  // end of step t - 1, behind the barrier that frees it, and the rest (late)
+  // between the first products of step t. All at once they would queue up
+  // and hold back the reads and products behind them (8192^3: 403 us so, 394
+  // in parts).
+  constexpr int kEarly = 4;
+  constexpr int kLate = (kLoads - kEarly + FM - 3) / (FM - 2) > 2
+                            ? (kLoads - kEarly + FM - 3) / (FM - 2)
+                            : 2;
+  auto step = [&](uint32_t buf, bool late, bool more) {
     if (WIDE) widen_b();
 #pragma unroll
     for (int i = 0; i < FM - 2; ++i) {
       a[i + 2] = frag(aLo, aHi, i + 2);
       rows_of(i);
+      if (late) {
+#pragma unroll
+        for (int q = 0; q < kLate; ++q) load(buf ^ 1, kEarly + i * kLate + q);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
-    if (more) stage(buf);
     aLo ^= kTile;
     aHi ^= kTile;
     bLo ^= kTile;
@@ -744,6 +798,10 @@ __device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
     if (WIDE) {
 #pragma unroll
       for (int k = 0; k < FN; ++k) b[k] = frag(bLo, bHi, k);
+      if (more) {
+#pragma unroll
+        for (int q = 0; q < kEarly; ++q) load(buf, q);
+      }
       __builtin_amdgcn_sched_barrier(0);
       rows_of(FM - 2);
       rows_of(FM - 1);
@@ -754,6 +812,7 @@ __device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
         product(FM - 1, k);
         __builtin_amdgcn_sched_barrier(0);
         b[k] = frag(bLo, bHi, k);
+        if (more && k < kEarly) load(buf, k);
       }
     }
     next_scales();
@@ -769,11 +828,16 @@ __device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
   a[1] = frag(aLo, aHi, 1);
 #pragma unroll
   for (int k = 0; k < FN; ++k) b[k] = frag(bLo, bHi, k);
-  // the last two steps fetch no more; a branch in the loop's body would let
-  // the compiler move matrix instructions behind the barrier
+  // block 1 is there already, and the last steps fetch no more; branches in
+  // the loop's body would let the compiler move products behind the barrier
   int t = 0;
-  for (; t + 2 < steps; ++t) step(t & 1, true);
-  for (; t < steps; ++t) step(t & 1, false);
+  if (steps > 2) {
+    step(0, false, true);
+    for (t = 1; t + 2 < steps; ++t) step(t & 1, true, true);
+    step(t & 1, true, false);
+    ++t;
+  }
+  for (; t < steps; ++t) step(t & 1, false, false);
 
   // lane: row rr + 4 i of C's 64, columns q4*16 + k*4 + 0..3 of its 64. The
   // sums pass through LDS, each lane's own, so that one copy of the code
@@ -885,9 +949,9 @@ __global__ __launch_bounds__(256) void finish_kernel(edl_fp8_finish f) {
 // At most 16 rows of x, as served requests come: x is quantised in the
 // registers of the wave that multiplies it and the weights go from memory
 // straight to the matrix instruction, so that a layer is one launch. A
-// workgroup takes 16 columns; its 8 waves share the blocks of 128 between
+// workgroup takes 16 columns; its 16 waves share the blocks of 128 between
 // them and join through LDS in order. Bound by the read of the weights.
-constexpr int kFewWaves = 8;
+constexpr int kFewWaves = 16;
 
 template <typename T>
 __global__ __launch_bounds__(kFewWaves * 64) void few_rows_kernel(
