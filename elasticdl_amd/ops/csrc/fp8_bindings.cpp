@@ -19,7 +19,7 @@ extern "C" {
 int edl_fp8_quantize(const edl_fp8_quant*, hipStream_t);
 int edl_fp8_quantize_pair(const edl_fp8_quant*, const edl_fp8_quant*,
                           hipStream_t);
-void edl_fp8_gemm_splits(edl_fp8_gemm*, int);
+void edl_fp8_gemm_plan(edl_fp8_gemm*, int, int);
 int edl_fp8_gemm_run(edl_fp8_finish*, int, hipStream_t);
 int edl_fp8_few_rows(const edl_fp8_gemm*, const void*, int64_t, int, int, int,
                      hipStream_t);
@@ -212,9 +212,9 @@ void bias_into(edl_fp8_gemm& g, const Tensor& bias) {
   g.bias = bias.data_ptr();
   g.bias_type = type_code(bias.scalar_type(), "bias");
 }
-// decides the splits of f's n products and adds their workspace
-void splits_into(edl_fp8_finish& f, int n, Pieces& pieces) {
-  edl_fp8_gemm_splits(f.g, n);
+// decides the tiles and splits of f's n products and adds their workspace
+void plan_into(edl_fp8_finish& f, int n, Pieces& pieces) {
+  edl_fp8_gemm_plan(f.g, n, f.out != nullptr);
   for (int i = 0; i < n; ++i) {
     f.g[i].part_ld = round_up(f.g[i].N, 16);
     if (f.g[i].splits > 1)
@@ -321,7 +321,7 @@ class Fp8Dense : public torch::autograd::Function<Fp8Dense> {
     f.g[0].act = (int)act;
     bias_into(f.g[0], bias);
     f.g[0].mask_ld = mask_row(n);
-    if (!few && m > 0) splits_into(f, 1, passing);
+    if (!few && m > 0) plan_into(f, 1, passing);
     Tensor held;
     if (need_x || need_w || bits) held = kept.place(x);
     const Tensor space = passing.place(x);
@@ -457,7 +457,7 @@ class Fp8Dense : public torch::autograd::Function<Fp8Dense> {
       f.out = out[2].data_ptr();
       f.out_type = type_code(bt, "bias");
     }
-    splits_into(f, products, passing);
+    plan_into(f, products, passing);
     const Tensor space = passing.place(dy);
     f.sums = a.sums = sums;
     if (need_x) {
@@ -520,7 +520,7 @@ Tensor fp8_dense_frozen(const Tensor& x, const Tensor& wq, const Tensor& ws,
     } else {
       Pieces passing;
       passing.add(&r);
-      splits_into(f, 1, passing);
+      plan_into(f, 1, passing);
       const Tensor space = passing.place(x2);
       f.g[0].a = r.q;
       f.g[0].sa = r.s;

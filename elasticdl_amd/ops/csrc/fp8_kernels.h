@@ -14,6 +14,11 @@
 #define EDL_ACT_RELU 1
 #define EDL_ACT_SIGMOID 2
 
+// a workgroup's share of a product: 64 x 128, 128 x 128 or 256 x 256
+#define EDL_TILE_RING 0
+#define EDL_TILE_128 1
+#define EDL_TILE_256 2
+
 struct edl_fp8_quant {
   const void* x;  // [R, C], rows ld apart
   int64_t ld, R, C;
@@ -48,6 +53,7 @@ struct edl_fp8_gemm {
   bool c_wide;    // 16-byte stores of 16 neighbours are aligned
   uint8_t* mask;  // relu: bits of c > 0, rows mask_ld bytes apart; may be null
   int64_t mask_ld;
+  int tile;     // EDL_TILE_*
   int splits;   // over the contraction
   float* part;  // [splits, M, part_ld] where splits > 1
   int64_t part_ld;  // N rounded up to 16

@@ -124,9 +124,9 @@ __device__ inline uint32_t max16(uint32_t v) {
 }
 
 // --------------------------------- quantise -------------------------------
-// One workgroup takes a tile of 128 x 128 and each thread 8 x 8 of it, so
+// One workgroup takes a tile of 128 x 128 and each thread 4 x 8 of it, so
 // that a block's maximum lies in one 16-lane row of lanes (rows) or in the
-// four waves (columns), and both forms are written from one read of x.
+// eight waves (columns), and both forms are written from one read of x.
 // Bound by memory.
 //
 // DERIV: x is the gradient at an activation's output, which is turned into
@@ -173,9 +173,11 @@ __device__ inline void load_row8(const T* x, int64_t ld, int64_t R, int64_t C,
 
 constexpr int kLdsRow = 144;  // a transposed row: 128 bytes and 16 of padding
 
+constexpr int kQuantThreads = 512, kQuantWaves = 8, kQuantRows = 4;
+
 struct QuantLds {
-  uint32_t max[4][kBlk];
-  float sum[4][kBlk];
+  uint32_t max[kQuantWaves][kBlk];
+  float sum[kQuantWaves][kBlk];
   __align__(16) uint8_t t[kBlk * kLdsRow];
 };
 
@@ -189,21 +191,21 @@ __device__ inline void quantize_tile(const edl_fp8_quant& a, int64_t block,
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int j = tid & 15;  // columns j*8 .. j*8+7
-  const int i = tid >> 4;  // rows    i*8 .. i*8+7
+  const int i = tid >> 4;  // rows    i*4 .. i*4+3
   const int64_t ncb = (a.C + kBlk - 1) / kBlk;
   const int64_t rb = block / ncb, cb = block % ncb;
-  const int64_t r0 = rb * kBlk + i * 8, c0 = cb * kBlk + j * 8;
+  const int64_t r0 = rb * kBlk + i * kQuantRows, c0 = cb * kBlk + j * 8;
 
-  float v[8][8];
+  float v[kQuantRows][8];
 #pragma unroll
-  for (int r = 0; r < 8; ++r)
+  for (int r = 0; r < kQuantRows; ++r)
     load_row8<T>(static_cast<const T*>(a.x), a.ld, a.R, a.C, r0 + r, c0,
                  a.wide, v[r]);
 
   if (DERIV) {
     if (a.act == EDL_ACT_RELU) {
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
+      for (int r = 0; r < kQuantRows; ++r) {
         uint32_t bits = 0;
         if (r0 + r < a.R && c0 < a.C)
           bits = a.mask[(r0 + r) * a.mask_ld + (c0 >> 3)];
@@ -212,7 +214,7 @@ __device__ inline void quantize_tile(const edl_fp8_quant& a, int64_t block,
       }
     } else if (a.act == EDL_ACT_SIGMOID) {
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
+      for (int r = 0; r < kQuantRows; ++r) {
         float o[8];
         load_row8<T>(static_cast<const T*>(a.y), a.y_ld, a.R, a.C, r0 + r, c0,
                      a.y_wide, o);
@@ -225,7 +227,7 @@ __device__ inline void quantize_tile(const edl_fp8_quant& a, int64_t block,
       for (int c = 0; c < 8; ++c) {
         float s = 0.f;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) s += v[r][c];
+        for (int r = 0; r < kQuantRows; ++r) s += v[r][c];
         s += __shfl_xor(s, 16);
         s += __shfl_xor(s, 32);
         if (lane < 16) s_sum[wave][j * 8 + c] = s;
@@ -233,11 +235,13 @@ __device__ inline void quantize_tile(const edl_fp8_quant& a, int64_t block,
     }
   }
 
-  uint32_t rmax[8], cmax[8];
+  uint32_t rmax[kQuantRows], cmax[8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k) rmax[k] = cmax[k] = 0;
+  for (int r = 0; r < kQuantRows; ++r) rmax[r] = 0;
 #pragma unroll
-  for (int r = 0; r < 8; ++r)
+  for (int c = 0; c < 8; ++c) cmax[c] = 0;
+#pragma unroll
+  for (int r = 0; r < kQuantRows; ++r)
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
       uint32_t m = finite_abs(v[r][c]);
@@ -246,7 +250,7 @@ __device__ inline void quantize_tile(const edl_fp8_quant& a, int64_t block,
     }
   if (!TILE) {
 #pragma unroll
-    for (int r = 0; r < 8; ++r) rmax[r] = max16(rmax[r]);
+    for (int r = 0; r < kQuantRows; ++r) rmax[r] = max16(rmax[r]);
   }
   if (cols || TILE) {
 #pragma unroll
@@ -263,8 +267,9 @@ __device__ inline void quantize_tile(const edl_fp8_quant& a, int64_t block,
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
       int col = j * 8 + c;
-      cmax[c] = max(max(s_max[0][col], s_max[1][col]),
-                    max(s_max[2][col], s_max[3][col]));
+#pragma unroll
+      for (int w = 0; w < kQuantWaves; ++w)
+        cmax[c] = max(cmax[c], s_max[w][col]);
     }
   }
   if (TILE) {  // one scale for all of it
@@ -273,18 +278,21 @@ __device__ inline void quantize_tile(const edl_fp8_quant& a, int64_t block,
     for (int c = 1; c < 8; ++c) m = max(m, cmax[c]);
     m = max16(m);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) rmax[k] = cmax[k] = m;
+    for (int r = 0; r < kQuantRows; ++r) rmax[r] = m;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) cmax[c] = m;
   }
   if (DERIV && a.sums && tid < kBlk) {
     int64_t c = cb * kBlk + tid;
     if (c < a.C)
       a.sums[rb * a.C + c] =
-          (s_sum[0][tid] + s_sum[1][tid]) + (s_sum[2][tid] + s_sum[3][tid]);
+          ((s_sum[0][tid] + s_sum[1][tid]) + (s_sum[2][tid] + s_sum[3][tid])) +
+          ((s_sum[4][tid] + s_sum[5][tid]) + (s_sum[6][tid] + s_sum[7][tid]));
   }
 
   if (a.rows) {
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
+    for (int r = 0; r < kQuantRows; ++r) {
       int b = scale_byte(rmax[r]);
       float inv = inverse_of(b);
       if (j == 0) a.rows_scale[cb * a.rows_rp + scale_slot(r0 + r)] = b;
@@ -302,16 +310,14 @@ __device__ inline void quantize_tile(const edl_fp8_quant& a, int64_t block,
       int b = scale_byte(cmax[c]);
       float inv = inverse_of(b);
       if (i == 0) a.cols_scale[rb * a.cols_rp + scale_slot(c0 + c)] = b;
-      i32x2 q;
-      q[0] = pack4(v[0][c], v[1][c], v[2][c], v[3][c], inv);
-      q[1] = pack4(v[4][c], v[5][c], v[6][c], v[7][c], inv);
-      *reinterpret_cast<i32x2*>(s_t + (j * 8 + c) * kLdsRow + i * 8) = q;
+      *reinterpret_cast<uint32_t*>(s_t + (j * 8 + c) * kLdsRow + i * 4) =
+          pack4(v[0][c], v[1][c], v[2][c], v[3][c], inv);
     }
     __syncthreads();
     // 8 lanes write a transposed row's 128 bytes together
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      int col = s * 32 + (tid >> 3), part = (tid & 7) * 16;
+    for (int s = 0; s < 2; ++s) {
+      int col = s * 64 + (tid >> 3), part = (tid & 7) * 16;
       int64_t c = cb * kBlk + col;
       if (c < a.C)
         *reinterpret_cast<i32x4*>(a.cols + c * a.cols_ld + rb * kBlk + part) =
@@ -321,16 +327,15 @@ __device__ inline void quantize_tile(const edl_fp8_quant& a, int64_t block,
 }
 
 template <typename T, bool TILE, bool DERIV>
-__global__ __launch_bounds__(256) void quantize_kernel(edl_fp8_quant a) {
+__global__ __launch_bounds__(kQuantThreads) void quantize_kernel(edl_fp8_quant a) {
   __shared__ QuantLds lds;
   quantize_tile<T, TILE, DERIV>(a, blockIdx.x, lds);
 }
 
 // a layer's input and its weight in one launch
 template <typename TX, typename TW>
-__global__ __launch_bounds__(256) void quantize_pair_kernel(edl_fp8_quant x,
-                                                            edl_fp8_quant w,
-                                                            int x_tiles) {
+__global__ __launch_bounds__(kQuantThreads) void quantize_pair_kernel(
+    edl_fp8_quant x, edl_fp8_quant w, int x_tiles) {
   __shared__ QuantLds lds;
   if ((int)blockIdx.x < x_tiles)
     quantize_tile<TX, false, false>(x, blockIdx.x, lds);
@@ -623,136 +628,137 @@ __device__ inline void epilogue16(const edl_fp8_gemm& g, int64_t m, int64_t n,
   }
 }
 
-template <int BM>
-struct GemmLds {  // two buffers each: A's, B's, scales (256 of A's and B's)
-  __align__(1024) uint8_t m[4 * BM * kBlk + 1024];
+// where a workgroup's tile lies, and its share of the steps
+struct Spot {
+  int64_t m0, n0;
+  int split, kb_all, kb0, steps;
 };
-
-template <int WM, int WN, int FM, int FN, typename T>
-__device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
-                                 uint8_t* smem) {
-  constexpr bool WIDE = TypeOf<T>::wide;
-  constexpr int BM = WM * FM * 16, BN = WN * FN * 16, NW = WM * WN;
-  static_assert(FN % 4 == 0 && FM % 4 == 0, "scale words: four fragments");
-  static_assert(BM == BN && (BM == 128 || BM == 256), "buffers' toggle");
-  constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW;  // 1 KB loads a wave
-  constexpr uint32_t kTile = BM * kBlk, kB = 2 * kTile, kS = 4 * kTile;
-
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave / WN, wn = wave % WN;
-
+template <int BM, int BN>
+__device__ inline Spot spot_of(const edl_fp8_gemm& g, int block, int blocks) {
   // tiles in groups of 4 rows of tiles, column by column
   const int ntm = (g.M + BM - 1) / BM, ntn = (g.N + BN - 1) / BN;
   const int order = xcd_order(block, blocks);
-  const int bid = order % (ntm * ntn), split = order / (ntm * ntn);
+  const int bid = order % (ntm * ntn);
   const int per = 4 * ntn, grp = bid / per, in = bid % per;
   const int tall = min(4, ntm - grp * 4);
-  const int64_t m0 = (int64_t)(grp * 4 + in % tall) * BM;
-  const int64_t n0 = (int64_t)(in / tall) * BN;
+  Spot s;
+  s.m0 = (int64_t)(grp * 4 + in % tall) * BM;
+  s.n0 = (int64_t)(in / tall) * BN;
+  s.split = order / (ntm * ntn);
+  s.kb_all = (int)(g.ld / kBlk);
+  s.kb0 = (int)((int64_t)s.kb_all * s.split / g.splits);
+  s.steps = (int)((int64_t)s.kb_all * (s.split + 1) / g.splits) - s.kb0;
+  return s;
+}
 
-  // this split's share of the steps
-  const int kb_all = (int)(g.ld / kBlk);
-  const int kb0 = (int)((int64_t)kb_all * split / g.splits);
-  const int steps = (int)((int64_t)kb_all * (split + 1) / g.splits) - kb0;
+// A wave's loads of a block: its share of 1 KB pieces of A and of B, each 8
+// rows (lane -> row lane>>3, slot lane&7), and 256 bytes of scales, A's by
+// even waves and B's by odd ones (several fetch the same; a branch would
+// cost more). Rows behind the matrix's last are that one again.
+template <int BM, int BN, int NW>
+struct Loads {
+  static constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW;
+  static constexpr int kAll = LA + LB + 1;
+  i32x4 bufA, bufB, bufS;
+  uint32_t offA[LA], offB[LB], at = 0, atS = 0, rp;
+  int wave, lane;
+  bool odd;
 
-  // one load fills 8 rows: lane -> row lane>>3, slot lane&7
-  const uint8_t* pa = g.a + m0 * g.ld + (int64_t)kb0 * kBlk;
-  const uint8_t* pb = g.b + n0 * g.ld + (int64_t)kb0 * kBlk;
-  const i32x4 bufA = buffer_of(pa, g.a + g.M * g.ld - pa);
-  const i32x4 bufB = buffer_of(pb, g.b + g.N * g.ld - pb);
-  uint32_t offA[LA], offB[LB];
-  const uint32_t lastA = (uint32_t)min(g.M - 1 - m0, (int64_t)BM);
-  const uint32_t lastB = (uint32_t)min(g.N - 1 - n0, (int64_t)BN);
+  __device__ Loads(const edl_fp8_gemm& g, const Spot& s, int wave_, int lane_)
+      : wave(wave_), lane(lane_), odd(wave_ & 1) {
+    const uint8_t* pa = g.a + s.m0 * g.ld + (int64_t)s.kb0 * kBlk;
+    const uint8_t* pb = g.b + s.n0 * g.ld + (int64_t)s.kb0 * kBlk;
+    bufA = buffer_of(pa, g.a + g.M * g.ld - pa);
+    bufB = buffer_of(pb, g.b + g.N * g.ld - pb);
+    const uint32_t lastA = (uint32_t)min(g.M - 1 - s.m0, (int64_t)BM);
+    const uint32_t lastB = (uint32_t)min(g.N - 1 - s.n0, (int64_t)BN);
 #pragma unroll
-  for (int q = 0; q < LA; ++q) {
-    uint32_t r = (wave * LA + q) * 8 + (lane >> 3);
-    offA[q] = min(r, lastA) * (uint32_t)g.ld + (((lane & 7) ^ swz(r)) << 4);
-  }
+    for (int q = 0; q < LA; ++q) {
+      const uint32_t r = (wave * LA + q) * 8 + (lane >> 3);
+      offA[q] = min(r, lastA) * (uint32_t)g.ld + (((lane & 7) ^ swz(r)) << 4);
+    }
 #pragma unroll
-  for (int q = 0; q < LB; ++q) {
-    uint32_t r = (wave * LB + q) * 8 + (lane >> 3);
-    offB[q] = min(r, lastB) * (uint32_t)g.ld + (((lane & 7) ^ swz(r)) << 4);
+    for (int q = 0; q < LB; ++q) {
+      const uint32_t r = (wave * LB + q) * 8 + (lane >> 3);
+      offB[q] = min(r, lastB) * (uint32_t)g.ld + (((lane & 7) ^ swz(r)) << 4);
+    }
+    const int64_t rows = odd ? g.b_rp : g.a_rp;
+    const uint8_t* base = odd ? g.sb : g.sa;
+    const uint8_t* ps = base + (odd ? s.n0 : s.m0) + s.kb0 * rows;
+    bufS = buffer_of(ps, base + (int64_t)s.kb_all * rows - ps);
+    rp = (uint32_t)rows;
   }
-  // scales: 256 bytes a load, A's by even waves and B's by odd ones (several
-  // fetch the same; a branch would cost more)
-  const bool odd = wave & 1;
-  const int64_t rp = odd ? g.b_rp : g.a_rp;
-  const uint8_t* ps = (odd ? g.sb + n0 : g.sa + m0) + kb0 * rp;
-  const i32x4 bufS =
-      buffer_of(ps, (odd ? g.sb : g.sa) + (int64_t)kb_all * rp - ps);
-  const uint32_t lds0 =
-      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
-  uint32_t at = 0, atS = 0;
-  constexpr int kLoads = LA + LB + 1;
-  auto load = [&](uint32_t buf, int q) {  // the q-th of the next block's
+  // the q-th load of the next block, into LDS at these places
+  __device__ inline void one(uint32_t a, uint32_t b, uint32_t s, int q) {
     if (q < LA) {
-      dma16(bufA, offA[q], at, lds0 + buf * kTile + (wave * LA + q) * 1024);
+      dma16(bufA, offA[q], at, a + (wave * LA + q) * 1024);
     } else if (q < LA + LB) {
       const int o = q - LA;
-      dma16(bufB, offB[o], at,
-            lds0 + kB + buf * kTile + (wave * LB + o) * 1024);
+      dma16(bufB, offB[o], at, b + (wave * LB + o) * 1024);
     } else if (q == LA + LB) {
-      dma4(bufS, lane * 4, atS, lds0 + kS + buf * 512 + odd * 256);
+      dma4(bufS, lane * 4, atS, s + odd * 256);
       at += kBlk;
-      atS += (uint32_t)rp;
+      atS += rp;
     }
-  };
-  auto stage = [&](uint32_t buf) {
-#pragma unroll
-    for (int q = 0; q < kLoads; ++q) load(buf, q);
-  };
+  }
+};
 
-  // fragment f of a wave's rows: 32 bytes of row rr, in chunks q4 and 4 + q4.
-  // Which bytes of a block meet is the same for A and B, and a block has one
-  // scale, so the order within it does not matter. f*4 leaves swz as it is.
-  const int rr = ((lane & 15) >> 2) * 16 + (lane & 3), q4 = lane >> 4;
-  const uint32_t lo = rr * kBlk + ((q4 ^ swz(rr)) << 4);
-  const uint32_t hi = rr * kBlk + (((q4 + 4) ^ swz(rr)) << 4);
-  const int wA = wm * FM * 16, wB = wn * FN * 16;
-  // these move to the other buffer and back with a step
-  uint32_t aLo = wA * kBlk + lo, aHi = wA * kBlk + hi;
-  uint32_t bLo = kB + wB * kBlk + lo, bHi = kB + wB * kBlk + hi;
-  uint32_t sAt = kS + (lane & 15) * 4;
-  auto frag = [&](uint32_t x, uint32_t y, int f) -> i32x8 {
-    const int o = ((f >> 2) * 64 + (f & 3) * 4) * kBlk;
-    i32x4 u = *reinterpret_cast<const i32x4*>(smem + x + o);
-    i32x4 v = *reinterpret_cast<const i32x4*>(smem + y + o);
-    return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
-  };
-
+// What a wave multiplies: FM fragments of A from the fA0-th, FN of B, and in
+// 32 bits (WIDE) B's fragments widened.
+//
+// Fragment f of the tile's rows: 32 bytes of row rr, in chunks q4 and 4 + q4.
+// Which bytes of a block meet is the same for A and B, and a block has one
+// scale, so the order within it does not matter. f*4 leaves swz as it is.
+template <int FM, int FN, bool WIDE>
+struct Hand {
+  static constexpr int SA = (FM + 3) / 4;
+  static_assert(FN % 4 == 0 && (FM % 4 == 0 || FM == 2), "scale words");
   f32x4 acc[FM][FN];
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int k = 0; k < FN; ++k) acc[i][k] = (f32x4){0.f, 0.f, 0.f, 0.f};
-
   i32x8 a[FM], b[FN];
-  int sa[FM / 4], sb[FN / 4], na[FM / 4], nb[FN / 4];
-  auto read_scales = [&]() {
+  Wide bw[WIDE ? FN : 1];
+  int sa[SA], sb[FN / 4];
+
+  __device__ inline void clear() {
 #pragma unroll
-    for (int k = 0; k < FM / 4; ++k)
-      na[k] = *reinterpret_cast<const int*>(smem + sAt + wA + k * 64);
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int k = 0; k < FN; ++k) acc[i][k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  }
+  static __device__ inline uint32_t row_of(int f) {
+    return (f >> 2) * 64 + (f & 3) * 4;
+  }
+  static __device__ inline i32x8 read(const uint8_t* smem, uint32_t lo,
+                                      uint32_t hi, int f) {
+    const int o = row_of(f) * kBlk;
+    const i32x4 u = *reinterpret_cast<const i32x4*>(smem + lo + o);
+    const i32x4 v = *reinterpret_cast<const i32x4*>(smem + hi + o);
+    return __builtin_shufflevector(u, v, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  // the words of scales at s: A's from its 64 rows on, shifted to its first
+  // fragment; B's 256 bytes behind
+  static __device__ inline void read_scales(const uint8_t* s, int fA0, int wB,
+                                            int* to_a, int* to_b) {
+#pragma unroll
+    for (int k = 0; k < SA; ++k) {
+      to_a[k] = *reinterpret_cast<const int*>(s + ((fA0 >> 2) + k) * 64);
+      if (FM < 4) to_a[k] = (uint32_t)to_a[k] >> ((fA0 & 3) * 8);
+    }
 #pragma unroll
     for (int k = 0; k < FN / 4; ++k)
-      nb[k] = *reinterpret_cast<const int*>(smem + sAt + 256 + wB + k * 64);
-  };
-  auto next_scales = [&]() {
+      to_b[k] = *reinterpret_cast<const int*>(s + 256 + wB + k * 64);
+  }
+  __device__ inline void widen_b() {
+    if (WIDE) {
 #pragma unroll
-    for (int k = 0; k < FM / 4; ++k) sa[k] = na[k];
-#pragma unroll
-    for (int k = 0; k < FN / 4; ++k) sb[k] = nb[k];
-  };
-  auto product = [&](int i, int k) {
+      for (int k = 0; k < FN; ++k)
+        bw[k] = widen(b[k], scale_value(sb[k >> 2], k & 3));
+    }
+  }
+  __device__ inline void product(int i, int k) {
     acc[i][k] = mfma_sel(k & 3, i & 3, b[k], a[i], acc[i][k], sb[k >> 2],
                          sa[i >> 2]);
-  };
-  Wide bw[WIDE ? FN : 1];
-  auto widen_b = [&]() {
-#pragma unroll
-    for (int k = 0; k < FN; ++k) bw[k] = widen(b[k], scale_value(sb[k >> 2], k & 3));
-  };
-  auto rows_of = [&](int i) {  // fragment i of A against all of B
+  }
+  __device__ inline void products(int i) {  // fragment i of A, all of B
     if (WIDE) {
       const Wide aw = widen(a[i], scale_value(sa[i >> 2], i & 3));
 #pragma unroll
@@ -761,57 +767,158 @@ __device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
 #pragma unroll
       for (int k = 0; k < FN; ++k) product(i, k);
     }
+  }
+};
+
+// Lane: row rr of C's 64 and fragment i's 4 i on, columns q4*16 + k*4 + 0..3
+// of its 64. The sums pass through LDS, each lane's own, so that one copy of
+// the code takes all rows: unrolled, the large tile's 16 would not stay in
+// registers.
+template <typename T, int FM, int FN, typename H>
+__device__ inline void write_tile(const edl_fp8_gemm& g, const Spot& s,
+                                  const H& h, uint8_t* smem, int wave,
+                                  int lane, int fA0, int wB, bool may_split) {
+  constexpr int G = FM < 4 ? FM : 4;
+  const int rr = ((lane & 15) >> 2) * 16 + (lane & 3), q4 = lane >> 4;
+  f32x4* own = reinterpret_cast<f32x4*>(smem) + wave * (G * 4 * 64) + lane;
+  __syncthreads();  // the last blocks are read
+#pragma unroll
+  for (int p = 0; p < FM / G * (FN / 4); ++p) {  // up to 64 x 64 at a time
+    const int j = p % (FN / 4), i0 = p / (FN / 4) * G;
+    const int64_t n = s.n0 + wB + j * 64 + q4 * 16;
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        own[(i * 4 + k) * 64] = h.acc[i0 + i][j * 4 + k];
+    float bias[16];
+    load_bias16(g, n, bias);
+#pragma unroll 1
+    for (int i = 0; i < G; ++i) {
+      const int64_t m = s.m0 + H::row_of(fA0 + i0 + i) + rr;
+      const bool live = m < g.M && n < g.N;
+      float v[16];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const f32x4 u = own[(i * 4 + k) * 64];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[k * 4 + q] = u[q];
+      }
+      if (may_split && g.splits > 1) {
+        float* to = g.part + ((int64_t)s.split * g.M + m) * g.part_ld + n;
+        if (live) {
+#pragma unroll
+          for (int k = 0; k < 16; k += 4)
+            *reinterpret_cast<f32x4*>(to + k) =
+                (f32x4){v[k], v[k + 1], v[k + 2], v[k + 3]};
+        }
+      } else {
+        epilogue16<T>(g, m, n, v, bias, live);
+      }
+    }
+  }
+}
+
+template <int BM>
+struct GemmLds {  // two buffers each: A's, B's, scales (256 of A's and B's)
+  static constexpr uint32_t kTile = BM * kBlk, kB = 2 * kTile, kS = 4 * kTile;
+  __align__(1024) uint8_t m[4 * BM * kBlk + 1024];
+};
+
+template <int WM, int WN, int FM, int FN, typename T>
+__device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
+                                 uint8_t* smem) {
+  constexpr bool WIDE = TypeOf<T>::wide;
+  constexpr int BM = WM * FM * 16, BN = WN * FN * 16, NW = WM * WN;
+  static_assert(BM == BN && (BM == 128 || BM == 256), "buffers' toggle");
+  constexpr uint32_t kTile = GemmLds<BM>::kTile, kB = GemmLds<BM>::kB,
+                     kS = GemmLds<BM>::kS;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const Spot s = spot_of<BM, BN>(g, block, blocks);
+  const int steps = s.steps;
+  Loads<BM, BN, NW> loads(g, s, wave, lane);
+  constexpr int kLoads = Loads<BM, BN, NW>::kAll;
+  const uint32_t lds0 =
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+  auto load = [&](uint32_t buf, int q) {
+    loads.one(lds0 + buf * kTile, lds0 + kB + buf * kTile,
+              lds0 + kS + buf * 512, q);
   };
+  auto stage = [&](uint32_t buf) {
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q) load(buf, q);
+  };
+
+  const int rr = ((lane & 15) >> 2) * 16 + (lane & 3), q4 = lane >> 4;
+  const uint32_t lo = rr * kBlk + ((q4 ^ swz(rr)) << 4);
+  const uint32_t hi = rr * kBlk + (((q4 + 4) ^ swz(rr)) << 4);
+  const int wA = wm * FM * 16, wB = wn * FN * 16, fA0 = wm * FM;
+  // these move to the other buffer and back with a step
+  uint32_t aLo = wA * kBlk + lo, aHi = wA * kBlk + hi;
+  uint32_t bLo = kB + wB * kBlk + lo, bHi = kB + wB * kBlk + hi;
+  uint32_t sAt = kS + (lane & 15) * 4;
+  typedef Hand<FM, FN, WIDE> H;
+  H h;
+  h.clear();
+  int na[FM / 4], nb[FN / 4];
+  auto next_scales = [&]() {
+#pragma unroll
+    for (int k = 0; k < FM / 4; ++k) h.sa[k] = na[k];
+#pragma unroll
+    for (int k = 0; k < FN / 4; ++k) h.sb[k] = nb[k];
+  };
+
   // Block t + 1 goes into the other buffer in two parts: kEarly loads at the
   // end of step t - 1, behind the barrier that frees it, and the rest (late)
   // between the first products of step t. All at once they would queue up
-  // and hold back the reads and products behind them (8192^3: 403 us so, 394
+  // and hold back the reads and products behind them (8192^3: 403 us so, 388
   // in parts).
   constexpr int kEarly = 4;
   constexpr int kLate = (kLoads - kEarly + FM - 3) / (FM - 2) > 2
                             ? (kLoads - kEarly + FM - 3) / (FM - 2)
                             : 2;
   auto step = [&](uint32_t buf, bool late, bool more) {
-    if (WIDE) widen_b();
+    h.widen_b();
 #pragma unroll
     for (int i = 0; i < FM - 2; ++i) {
-      a[i + 2] = frag(aLo, aHi, i + 2);
-      rows_of(i);
+      h.a[i + 2] = H::read(smem, aLo, aHi, i + 2);
+      h.products(i);
       if (late) {
 #pragma unroll
         for (int q = 0; q < kLate; ++q) load(buf ^ 1, kEarly + i * kLate + q);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     aLo ^= kTile;
     aHi ^= kTile;
     bLo ^= kTile;
     bHi ^= kTile;
     sAt ^= 512;
     // after the last step these read a buffer that nobody writes any more
-    read_scales();
-    a[0] = frag(aLo, aHi, 0);
-    a[1] = frag(aLo, aHi, 1);
+    H::read_scales(smem + sAt, fA0, wB, na, nb);
+    h.a[0] = H::read(smem, aLo, aHi, 0);
+    h.a[1] = H::read(smem, aLo, aHi, 1);
     __builtin_amdgcn_sched_barrier(0);
     if (WIDE) {
 #pragma unroll
-      for (int k = 0; k < FN; ++k) b[k] = frag(bLo, bHi, k);
+      for (int k = 0; k < FN; ++k) h.b[k] = H::read(smem, bLo, bHi, k);
       if (more) {
 #pragma unroll
         for (int q = 0; q < kEarly; ++q) load(buf, q);
       }
       __builtin_amdgcn_sched_barrier(0);
-      rows_of(FM - 2);
-      rows_of(FM - 1);
+      h.products(FM - 2);
+      h.products(FM - 1);
     } else {
 #pragma unroll
       for (int k = 0; k < FN; ++k) {
-        product(FM - 2, k);
-        product(FM - 1, k);
+        h.product(FM - 2, k);
+        h.product(FM - 1, k);
         __builtin_amdgcn_sched_barrier(0);
-        b[k] = frag(bLo, bHi, k);
+        h.b[k] = H::read(smem, bLo, bHi, k);
         if (more && k < kEarly) load(buf, k);
       }
     }
@@ -820,14 +927,13 @@ __device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
 
   stage(0);
   if (steps > 1) stage(1);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  read_scales();
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+  H::read_scales(smem + sAt, fA0, wB, na, nb);
   next_scales();
-  a[0] = frag(aLo, aHi, 0);
-  a[1] = frag(aLo, aHi, 1);
+  h.a[0] = H::read(smem, aLo, aHi, 0);
+  h.a[1] = H::read(smem, aLo, aHi, 1);
 #pragma unroll
-  for (int k = 0; k < FN; ++k) b[k] = frag(bLo, bHi, k);
+  for (int k = 0; k < FN; ++k) h.b[k] = H::read(smem, bLo, bHi, k);
   // block 1 is there already, and the last steps fetch no more; branches in
   // the loop's body would let the compiler move products behind the barrier
   int t = 0;
@@ -838,56 +944,97 @@ __device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
     ++t;
   }
   for (; t < steps; ++t) step(t & 1, false, false);
-
-  // lane: row rr + 4 i of C's 64, columns q4*16 + k*4 + 0..3 of its 64. The
-  // sums pass through LDS, each lane's own, so that one copy of the code
-  // below takes all rows: unrolled, the large tile's 16 would not stay in
-  // registers.
-  __syncthreads();
-  f32x4* own = reinterpret_cast<f32x4*>(smem) + wave * (4 * 4 * 64) + lane;
-  static_assert(NW * 4 * 4 * 64 * 16 <= 4 * BM * kBlk, "");
-#pragma unroll
-  for (int h = 0; h < FM / 4 * (FN / 4); ++h) {  // 64 x 64 at a time
-    const int j = h % (FN / 4), i0 = h / (FN / 4) * 4;
-    const int64_t n = n0 + wB + j * 64 + q4 * 16;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        own[(i * 4 + k) * 64] = acc[i0 + i][j * 4 + k];
-    float bias[16];
-    load_bias16(g, n, bias);
-#pragma unroll 1
-    for (int i = 0; i < 4; ++i) {
-      const int64_t m = m0 + wA + i0 * 16 + rr + i * 4;
-      const bool live = m < g.M && n < g.N;
-      float v[16];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const f32x4 u = own[(i * 4 + k) * 64];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[k * 4 + q] = u[q];
-      }
-      if (BM == 128 && g.splits > 1) {
-        float* p = g.part + ((int64_t)split * g.M + m) * g.part_ld + n;
-        if (live) {
-#pragma unroll
-          for (int k = 0; k < 16; k += 4)
-            *reinterpret_cast<f32x4*>(p + k) =
-                (f32x4){v[k], v[k + 1], v[k + 2], v[k + 3]};
-        }
-      } else {
-        epilogue16<T>(g, m, n, v, bias, live);
-      }
-    }
-  }
+  write_tile<T, FM, FN>(g, s, h, smem, wave, lane, fA0, wB, BM == 128);
 }
 
 template <int WM, int WN, int FM, int FN, typename T>
-__global__ __launch_bounds__(WM* WN * 64, FN > 4 ? 1 : 2) void gemm_kernel(
+__global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(
     edl_fp8_gemm g) {
   __shared__ GemmLds<WM * FM * 16> lds;
   gemm_tile<WM, WN, FM, FN, T>(g, blockIdx.x, gridDim.x, lds.m);
+}
+
+// Products too small to fill the chip with the tiles above wait for memory,
+// not for the matrix cores: a workgroup takes 64 x 128, a wave 32 x 64, and
+// the blocks pass through three buffers, so that loads are two steps ahead.
+// A step waits for its own block's loads alone (vmcnt counts a wave's, in
+// order), then one barrier both shows the block to all waves and frees the
+// buffer of the step before, which all have read by then.
+struct RingLds {
+  static constexpr int BM = 64, BN = 128, kBuffers = 3;
+  static constexpr uint32_t kA = BM * kBlk, kB = BN * kBlk,
+                            kOne = kA + kB + 512;
+  __align__(1024) uint8_t m[kBuffers * kOne];
+};
+
+template <typename T>
+__device__ inline void gemm_ring(const edl_fp8_gemm& g, int block, int blocks,
+                                 uint8_t* smem) {
+  constexpr bool WIDE = TypeOf<T>::wide;
+  constexpr int FM = 2, FN = 4;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int fA0 = (wave >> 1) * FM, wB = (wave & 1) * 64;
+  const Spot s = spot_of<RingLds::BM, RingLds::BN>(g, block, blocks);
+  Loads<RingLds::BM, RingLds::BN, 4> loads(g, s, wave, lane);
+  constexpr int kLoads = Loads<RingLds::BM, RingLds::BN, 4>::kAll;
+  static_assert(kLoads == 7, "the waits below");
+  const uint32_t lds0 =
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+  auto stage = [&](uint32_t buf) {
+    const uint32_t at = lds0 + buf * RingLds::kOne;
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q)
+      loads.one(at, at + RingLds::kA, at + RingLds::kA + RingLds::kB, q);
+  };
+  const int rr = ((lane & 15) >> 2) * 16 + (lane & 3), q4 = lane >> 4;
+  const uint32_t lo = rr * kBlk + ((q4 ^ swz(rr)) << 4);
+  const uint32_t hi = rr * kBlk + (((q4 + 4) ^ swz(rr)) << 4);
+  typedef Hand<FM, FN, WIDE> H;
+  H h;
+  h.clear();
+  const uint32_t rows = H::row_of(fA0) * kBlk;
+
+  stage(0);
+  if (s.steps > 1) stage(1);
+  uint32_t buf = 0, ahead = 2;
+  for (int t = 0; t < s.steps; ++t) {
+    if (t + 1 < s.steps)
+      asm volatile("s_waitcnt vmcnt(7)\n\ts_barrier" ::: "memory");
+    else
+      asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    if (t + 2 < s.steps) stage(ahead);
+    const uint8_t* p = smem + buf * RingLds::kOne;
+    H::read_scales(p + RingLds::kA + RingLds::kB + (lane & 15) * 4, fA0, wB,
+                   h.sa, h.sb);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) h.a[i] = H::read(p, rows + lo, rows + hi, i);
+#pragma unroll
+    for (int k = 0; k < FN; ++k)
+      h.b[k] = H::read(p, RingLds::kA + wB * kBlk + lo,
+                       RingLds::kA + wB * kBlk + hi, k);
+    h.widen_b();
+#pragma unroll
+    for (int i = 0; i < FM; ++i) h.products(i);
+    buf = buf == 2 ? 0 : buf + 1;
+    ahead = ahead == 2 ? 0 : ahead + 1;
+  }
+  write_tile<T, FM, FN>(g, s, h, smem, wave, lane, fA0, wB, true);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256, 2) void gemm_ring_kernel(edl_fp8_gemm g) {
+  __shared__ RingLds lds;
+  gemm_ring<T>(g, blockIdx.x, gridDim.x, lds.m);
+}
+template <typename T0, typename T1>
+__global__ __launch_bounds__(256, 2) void gemm_ring_pair_kernel(
+    edl_fp8_gemm g0, edl_fp8_gemm g1, int blocks0) {
+  __shared__ RingLds lds;
+  if ((int)blockIdx.x < blocks0)
+    gemm_ring<T0>(g0, blockIdx.x, blocks0, lds.m);
+  else
+    gemm_ring<T1>(g1, blockIdx.x - blocks0, gridDim.x - blocks0, lds.m);
 }
 
 // the two products of a backward pass in one launch, each of 128 x 128
@@ -1019,7 +1166,7 @@ int64_t tiles_of(const edl_fp8_quant& a) {
 
 template <typename T>
 void launch_quantize(const edl_fp8_quant& a, hipStream_t st) {
-  dim3 grid((unsigned)tiles_of(a)), block(256);
+  dim3 grid((unsigned)tiles_of(a)), block(kQuantThreads);
   if (a.tile)
     quantize_kernel<T, true, false><<<grid, block, 0, st>>>(a);
   else if (a.deriv)
@@ -1032,7 +1179,7 @@ template <typename TX>
 void launch_quantize_pair(const edl_fp8_quant& x, const edl_fp8_quant& w,
                           hipStream_t st) {
   const int n = (int)tiles_of(x);
-  dim3 grid((unsigned)(n + tiles_of(w))), block(256);
+  dim3 grid((unsigned)(n + tiles_of(w))), block(kQuantThreads);
   if (w.type == EDL_T_F32)
     quantize_pair_kernel<TX, float><<<grid, block, 0, st>>>(x, w, n);
   else if (w.type == EDL_T_BF16)
@@ -1041,19 +1188,13 @@ void launch_quantize_pair(const edl_fp8_quant& x, const edl_fp8_quant& w,
     quantize_pair_kernel<TX, _Float16><<<grid, block, 0, st>>>(x, w, n);
 }
 
-int64_t tiles128(const edl_fp8_gemm& g) {
-  return ((g.M + 127) / 128) * ((g.N + 127) / 128);
+int64_t tiles_of(const edl_fp8_gemm& g, int64_t bm, int64_t bn) {
+  return ((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn);
 }
-int64_t tiles256(const edl_fp8_gemm& g) {
-  return ((g.M + 255) / 256) * ((g.N + 255) / 256);
-}
-
-// Which kernel. 256 x 256 reads each operand half as often but runs one
-// workgroup a CU, so it takes the products that give each of the 256 CUs
-// one. In 32 bits a wave's fragments take twice the registers: always
-// 128 x 128.
-bool takes_256(const edl_fp8_gemm& g) {
-  return g.c_type != EDL_T_F32 && tiles256(g) >= 256;
+int64_t tiles_of(const edl_fp8_gemm& g) {
+  return g.tile == EDL_TILE_RING  ? tiles_of(g, 64, 128)
+         : g.tile == EDL_TILE_128 ? tiles_of(g, 128, 128)
+                                  : tiles_of(g, 256, 256);
 }
 
 }  // namespace
@@ -1079,36 +1220,56 @@ extern "C" int edl_fp8_quantize_pair(const edl_fp8_quant* x,
   return (int)hipGetLastError();
 }
 
-// How many splits of the contraction each of n products (1 or 2, in one
-// launch) takes: as many as fill 512 workgroups (two a CU) together, with at
-// least four blocks to each.
-extern "C" void edl_fp8_gemm_splits(edl_fp8_gemm* g, int n) {
-  int64_t tiles = 0;
-  for (int i = 0; i < n; ++i)
-    if (!takes_256(g[i])) tiles += tiles128(g[i]);
+// Chooses each product's tile, and how many splits of the contraction it
+// takes, for n products (1 or 2, in one launch where their tiles agree).
+//
+// 256 x 256 reads each operand half as often but runs one workgroup a CU, so
+// it takes the products that give each of the 256 CUs one. (In 32 bits a
+// wave's fragments take twice the registers: no.) Where 128 x 128 leaves CUs
+// without work, the ring of 64 x 128 is in time what its loads take: 4096 x
+// 624 x 400 17.7 us in 128 tiles of 128, 10.1 in 256 of the ring.
+//
+// Splits, up to 512 workgroups in all (two a CU): a join is a launch more,
+// so a split has at least 8 blocks to do, or 4 where something else needs
+// the launch that joins (finish).
+extern "C" void edl_fp8_gemm_plan(edl_fp8_gemm* g, int n, int finish) {
+  bool ring = true;
   for (int i = 0; i < n; ++i) {
     g[i].splits = 1;
-    if (takes_256(g[i])) continue;
-    int64_t s = 512 / tiles, most = g[i].ld / kBlk / 4;
-    if (s > most) s = most;
-    if (s > 64) s = 64;
-    if (s > 1) g[i].splits = (int)s;
+    g[i].tile = g[i].c_type != EDL_T_F32 && tiles_of(g[i], 256, 256) >= 256
+                    ? EDL_TILE_256
+                    : EDL_TILE_128;
+    if (g[i].tile == EDL_TILE_256 || tiles_of(g[i], 128, 128) >= 256)
+      ring = false;
+  }
+  for (int i = 0; i < n; ++i)
+    if (ring) g[i].tile = EDL_TILE_RING;
+  for (int64_t least = finish ? 4 : 8; least < (1 << 20); least *= 2) {
+    int64_t all = 0;
+    for (int i = 0; i < n; ++i) {
+      if (g[i].tile == EDL_TILE_256) continue;
+      int64_t splits = g[i].ld / kBlk / least;
+      splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
+      g[i].splits = (int)splits;
+      all += tiles_of(g[i]) * splits;
+    }
+    if (all <= 512) break;
   }
 }
 
 template <typename T>
 static void launch_as(const edl_fp8_gemm& g, hipStream_t st) {
-  if (takes_256(g))
-    gemm_kernel<2, 4, 8, 4, T>
-        <<<dim3((unsigned)tiles256(g)), dim3(512), 0, st>>>(g);
-  else
-    gemm_kernel<2, 2, 4, 4, T>
-        <<<dim3((unsigned)(tiles128(g) * g.splits)), dim3(256), 0, st>>>(g);
+  dim3 grid((unsigned)(tiles_of(g) * g.splits));
+  if (g.tile == EDL_TILE_RING)
+    gemm_ring_kernel<T><<<grid, dim3(256), 0, st>>>(g);
+  else if (g.tile == EDL_TILE_128)
+    gemm_kernel<2, 2, 4, 4, T><<<grid, dim3(256), 0, st>>>(g);
+  else if constexpr (!TypeOf<T>::wide)
+    gemm_kernel<2, 4, 8, 4, T><<<grid, dim3(512), 0, st>>>(g);
 }
 static int launch_one(const edl_fp8_gemm& g, hipStream_t st) {
   if (g.c_type == EDL_T_F32)
-    gemm_kernel<2, 2, 4, 4, float>
-        <<<dim3((unsigned)(tiles128(g) * g.splits)), dim3(256), 0, st>>>(g);
+    launch_as<float>(g, st);
   else if (g.c_type == EDL_T_BF16)
     launch_as<__bf16>(g, st);
   else
@@ -1117,10 +1278,13 @@ static int launch_one(const edl_fp8_gemm& g, hipStream_t st) {
 }
 template <typename T0, typename T1>
 static void launch_pair(const edl_fp8_gemm* g, hipStream_t st) {
-  const int b0 = (int)tiles128(g[0]) * g[0].splits;
-  const int b1 = (int)tiles128(g[1]) * g[1].splits;
-  gemm_pair_kernel<T0, T1>
-      <<<dim3((unsigned)(b0 + b1)), dim3(256), 0, st>>>(g[0], g[1], b0);
+  const int b0 = (int)tiles_of(g[0]) * g[0].splits;
+  const int b1 = (int)tiles_of(g[1]) * g[1].splits;
+  dim3 grid((unsigned)(b0 + b1)), block(256);
+  if (g[0].tile == EDL_TILE_RING)
+    gemm_ring_pair_kernel<T0, T1><<<grid, block, 0, st>>>(g[0], g[1], b0);
+  else
+    gemm_pair_kernel<T0, T1><<<grid, block, 0, st>>>(g[0], g[1], b0);
 }
 template <typename T0>
 static void launch_pair_as(const edl_fp8_gemm* g, hipStream_t st) {
@@ -1137,7 +1301,7 @@ static void launch_pair_as(const edl_fp8_gemm* g, hipStream_t st) {
 extern "C" int edl_fp8_gemm_run(edl_fp8_finish* f, int n, hipStream_t st) {
   edl_fp8_gemm* g = f->g;
   int rc = 0;
-  if (n == 2 && !takes_256(g[0]) && !takes_256(g[1])) {
+  if (n == 2 && g[0].tile == g[1].tile && g[0].tile != EDL_TILE_256) {
     if (g[0].c_type == EDL_T_F32)
       launch_pair_as<float>(g, st);
     else if (g[0].c_type == EDL_T_BF16)
