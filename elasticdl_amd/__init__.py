@@ -21,6 +21,13 @@ def __getattr__(name):
     _exports = {
         "EdlEmbedding": ("elasticdl_amd.layers.embedding", "EdlEmbedding"),
         "FusedDense": ("elasticdl_amd.ops.functional", "FusedDense"),
+        "set_dense_precision": (
+            "elasticdl_amd.ops.functional", "set_dense_precision",
+        ),
+        "fp8_dense": ("elasticdl_amd.ops.fp8", "fp8_dense"),
+        "quantize_fp8": ("elasticdl_amd.ops.fp8", "quantize_fp8"),
+        "quantize_fp8_weight": ("elasticdl_amd.ops.fp8", "quantize_fp8_weight"),
+        "embedding_lookup": ("elasticdl_amd.ops.embedding", "embedding_lookup"),
         "DistributedOptimizer": (
             "elasticdl_amd.collective.distributed_optimizer",
             "DistributedOptimizer",

@@ -53,6 +53,7 @@ def deduplicate_indexed_slices(
     ids = ids.to(torch.int64)
     if (values.is_cuda and ids.device == values.device
             and values.dim() == 2 and ids.dim() == 1
+            and ids.numel() < 2 ** 31 - 8192 and values.shape[1] < 2 ** 20
             and values.dtype in (torch.float32, torch.bfloat16, torch.float16)
             and not (torch.is_grad_enabled() and values.requires_grad)):
         from elasticdl_amd.ops.embedding import coalesce_rows

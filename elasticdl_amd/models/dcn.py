@@ -32,6 +32,7 @@ class DCN(nn.Module):
         num_cross: int = 3,
         hidden: List[int] = (128, 64),
         max_rows: int = 1 << 22,
+        precision: str = "bf16",
     ):
         super().__init__()
         self.embedding = EdlEmbedding("dcn_embedding", embedding_dim,
@@ -40,7 +41,8 @@ class DCN(nn.Module):
         self.cross = nn.ModuleList(CrossLayer(dim) for _ in range(num_cross))
         dims = [dim, *hidden]
         self.deep = nn.Sequential(
-            *[FusedDense(dims[i], dims[i + 1], act="relu")
+            *[FusedDense(dims[i], dims[i + 1], act="relu",
+                         precision=precision)
               for i in range(len(hidden))]
         )
         self.head = nn.Linear(dim + dims[-1], 1)

@@ -24,6 +24,7 @@ class DeepFM(nn.Module):
         factor_dim: int = 16,
         hidden: List[int] = (400, 400, 400),
         max_rows: int = 1 << 24,
+        precision: str = "bf16",
     ):
         super().__init__()
         self.num_fields = num_fields
@@ -31,7 +32,8 @@ class DeepFM(nn.Module):
         self.factors = EdlEmbedding("fm_factors", factor_dim, max_rows=max_rows)
         dims = [num_fields * factor_dim, *hidden]
         self.tower = nn.Sequential(
-            *[FusedDense(dims[i], dims[i + 1], act="relu") for i in range(len(hidden))]
+            *[FusedDense(dims[i], dims[i + 1], act="relu",
+                         precision=precision) for i in range(len(hidden))]
         )
         self.head = FusedDense(dims[-1], 1, act="none")
 

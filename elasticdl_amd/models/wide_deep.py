@@ -23,6 +23,7 @@ class WideDeep(nn.Module):
         embedding_dim: int = 8,
         hidden: List[int] = (64, 32, 16),
         max_rows: int = 1 << 20,
+        precision: str = "bf16",
     ):
         super().__init__()
         self.num_features = num_features
@@ -30,7 +31,8 @@ class WideDeep(nn.Module):
         self.deep = EdlEmbedding("deep_embedding", embedding_dim, max_rows=max_rows)
         dims = [num_features * embedding_dim, *hidden]
         self.tower = nn.Sequential(
-            *[FusedDense(dims[i], dims[i + 1], act="relu") for i in range(len(hidden))]
+            *[FusedDense(dims[i], dims[i + 1], act="relu",
+                         precision=precision) for i in range(len(hidden))]
         )
         self.head = FusedDense(dims[-1], 1, act="none")
 

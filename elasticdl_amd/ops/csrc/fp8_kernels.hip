@@ -40,6 +40,10 @@ typedef __attribute__((ext_vector_type(2))) float f32x2;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+typedef __attribute__((ext_vector_type(2))) uint16_t u16x2;
+typedef __attribute__((ext_vector_type(2))) short s16x2;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 
 namespace {
 
@@ -124,10 +128,12 @@ __device__ inline uint32_t max16(uint32_t v) {
 }
 
 // --------------------------------- quantise -------------------------------
-// One workgroup takes a tile of 128 x 128 and each thread 4 x 8 of it, so
+// One workgroup takes a tile of 128 x 128 and each thread ROWS x 8 of it, so
 // that a block's maximum lies in one 16-lane row of lanes (rows) or in the
-// eight waves (columns), and both forms are written from one read of x.
-// Bound by memory.
+// waves (columns), and both forms are written from one read of x. Bound by
+// memory where there are many tiles (8 rows to a thread: 16384 x 4096 76 us,
+// against 85 with 4), by a thread's work where there are few (4096 x 624 10.2
+// us with 4, 12.8 with 8).
 //
 // DERIV: x is the gradient at an activation's output, which is turned into
 // the gradient at its input on the way (relu: one kept bit; sigmoid: the
@@ -173,17 +179,18 @@ __device__ inline void load_row8(const T* x, int64_t ld, int64_t R, int64_t C,
 
 constexpr int kLdsRow = 144;  // a transposed row: 128 bytes and 16 of padding
 
-constexpr int kQuantThreads = 512, kQuantWaves = 8, kQuantRows = 4;
-
+template <int ROWS>
 struct QuantLds {
+  static constexpr int kQuantWaves = 32 / ROWS;
   uint32_t max[kQuantWaves][kBlk];
   float sum[kQuantWaves][kBlk];
   __align__(16) uint8_t t[kBlk * kLdsRow];
 };
 
-template <typename T, bool TILE, bool DERIV>
+template <typename T, int kQuantRows, bool TILE, bool DERIV>
 __device__ inline void quantize_tile(const edl_fp8_quant& a, int64_t block,
-                                     QuantLds& lds) {
+                                     QuantLds<kQuantRows>& lds) {
+  constexpr int kQuantWaves = QuantLds<kQuantRows>::kQuantWaves;
   uint32_t(*s_max)[kBlk] = lds.max;
   float(*s_sum)[kBlk] = lds.sum;
   uint8_t* s_t = lds.t;
@@ -191,7 +198,7 @@ __device__ inline void quantize_tile(const edl_fp8_quant& a, int64_t block,
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int j = tid & 15;  // columns j*8 .. j*8+7
-  const int i = tid >> 4;  // rows    i*4 .. i*4+3
+  const int i = tid >> 4;  // rows    i*ROWS ..
   const int64_t ncb = (a.C + kBlk - 1) / kBlk;
   const int64_t rb = block / ncb, cb = block % ncb;
   const int64_t r0 = rb * kBlk + i * kQuantRows, c0 = cb * kBlk + j * 8;
@@ -285,9 +292,12 @@ __device__ inline void quantize_tile(const edl_fp8_quant& a, int64_t block,
   if (DERIV && a.sums && tid < kBlk) {
     int64_t c = cb * kBlk + tid;
     if (c < a.C)
-      a.sums[rb * a.C + c] =
-          ((s_sum[0][tid] + s_sum[1][tid]) + (s_sum[2][tid] + s_sum[3][tid])) +
-          ((s_sum[4][tid] + s_sum[5][tid]) + (s_sum[6][tid] + s_sum[7][tid]));
+    {
+      float t = 0.f;
+#pragma unroll
+      for (int w = 0; w < kQuantWaves; ++w) t += s_sum[w][tid];
+      a.sums[rb * a.C + c] = t;
+    }
   }
 
   if (a.rows) {
@@ -310,14 +320,17 @@ __device__ inline void quantize_tile(const edl_fp8_quant& a, int64_t block,
       int b = scale_byte(cmax[c]);
       float inv = inverse_of(b);
       if (i == 0) a.cols_scale[rb * a.cols_rp + scale_slot(c0 + c)] = b;
-      *reinterpret_cast<uint32_t*>(s_t + (j * 8 + c) * kLdsRow + i * 4) =
-          pack4(v[0][c], v[1][c], v[2][c], v[3][c], inv);
+      uint8_t* to = s_t + (j * 8 + c) * kLdsRow + i * kQuantRows;
+#pragma unroll
+      for (int r = 0; r < kQuantRows; r += 4)
+        *reinterpret_cast<uint32_t*>(to + r) =
+            pack4(v[r][c], v[r + 1][c], v[r + 2][c], v[r + 3][c], inv);
     }
     __syncthreads();
     // 8 lanes write a transposed row's 128 bytes together
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      int col = s * 64 + (tid >> 3), part = (tid & 7) * 16;
+    for (int s = 0; s < kQuantRows / 2; ++s) {
+      int col = s * kQuantWaves * 8 + (tid >> 3), part = (tid & 7) * 16;
       int64_t c = cb * kBlk + col;
       if (c < a.C)
         *reinterpret_cast<i32x4*>(a.cols + c * a.cols_ld + rb * kBlk + part) =
@@ -326,21 +339,22 @@ __device__ inline void quantize_tile(const edl_fp8_quant& a, int64_t block,
   }
 }
 
-template <typename T, bool TILE, bool DERIV>
-__global__ __launch_bounds__(kQuantThreads) void quantize_kernel(edl_fp8_quant a) {
-  __shared__ QuantLds lds;
-  quantize_tile<T, TILE, DERIV>(a, blockIdx.x, lds);
+template <typename T, int ROWS, bool TILE, bool DERIV>
+__global__ __launch_bounds__(2048 / ROWS) void quantize_kernel(
+    edl_fp8_quant a) {
+  __shared__ QuantLds<ROWS> lds;
+  quantize_tile<T, ROWS, TILE, DERIV>(a, blockIdx.x, lds);
 }
 
 // a layer's input and its weight in one launch
-template <typename TX, typename TW>
-__global__ __launch_bounds__(kQuantThreads) void quantize_pair_kernel(
+template <typename TX, typename TW, int ROWS>
+__global__ __launch_bounds__(2048 / ROWS) void quantize_pair_kernel(
     edl_fp8_quant x, edl_fp8_quant w, int x_tiles) {
-  __shared__ QuantLds lds;
+  __shared__ QuantLds<ROWS> lds;
   if ((int)blockIdx.x < x_tiles)
-    quantize_tile<TX, false, false>(x, blockIdx.x, lds);
+    quantize_tile<TX, ROWS, false, false>(x, blockIdx.x, lds);
   else
-    quantize_tile<TW, true, false>(w, blockIdx.x - x_tiles, lds);
+    quantize_tile<TW, ROWS, true, false>(w, blockIdx.x - x_tiles, lds);
 }
 
 // out[c] = sum over the tiles of sums[t][c], in order of t within each of 16
@@ -1100,6 +1114,92 @@ __global__ __launch_bounds__(256) void finish_kernel(edl_fp8_finish f) {
 // them and join through LDS in order. Bound by the read of the weights.
 constexpr int kFewWaves = 16;
 
+
+// 32 neighbours of a row as e4m3 bytes, and the scale's byte of the 128 that
+// the four lanes of a row hold together
+template <typename T>
+__device__ inline i32x8 round32(const T* x, int64_t ld, int64_t M, int K,
+                                int row, int64_t k0, bool wide, int* scale) {
+  float v[32];
+  uint32_t m = 0;
+#pragma unroll
+  for (int k = 0; k < 32; k += 8)
+    load_row8<T>(x, ld, M, K, row, k0 + k, wide, v + k);
+#pragma unroll
+  for (int k = 0; k < 32; ++k) m = max(m, finite_abs(v[k]));
+  m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+  m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+  *scale = scale_byte(m);
+  const float inv = inverse_of(*scale);
+  i32x8 a;
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    a[k] = pack4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3], inv);
+  return a;
+}
+
+// The same for 16-bit inputs of 32 whole neighbours: the largest by packed
+// 16-bit integers and two values a conversion, a fifth of the instructions.
+// Every workgroup rounds all of x, so they are what 16 rows cost: 16 x 4096 x
+// 4096 12.3 us without this.
+template <typename T>
+struct Halves;
+template <>
+struct Halves<__bf16> {
+  static constexpr uint16_t not_finite = 0x7f80;
+  static __device__ inline float value(uint32_t bits) {
+    return __uint_as_float(bits << 16);
+  }
+  static __device__ inline u16x2 pack(u16x2 old, uint32_t two, float s,
+                                      bool hi) {
+    const bf16x2 x = __builtin_bit_cast(bf16x2, two);
+    const s16x2 o = __builtin_bit_cast(s16x2, old);
+    return __builtin_bit_cast(
+        u16x2, hi ? __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(o, x, s, true)
+                  : __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(o, x, s, false));
+  }
+};
+template <>
+struct Halves<_Float16> {
+  static constexpr uint16_t not_finite = 0x7c00;
+  static __device__ inline float value(uint32_t bits) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
+  }
+  static __device__ inline u16x2 pack(u16x2 old, uint32_t two, float s,
+                                      bool hi) {
+    const f16x2 x = __builtin_bit_cast(f16x2, two);
+    const s16x2 o = __builtin_bit_cast(s16x2, old);
+    return __builtin_bit_cast(
+        u16x2, hi ? __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(o, x, s, true)
+                  : __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(o, x, s, false));
+  }
+};
+// false where a value of the wave's is not finite
+template <typename T>
+__device__ inline bool round32_fast(const u32x4* w, int* scale, i32x8* a) {
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const u16x2 t =
+        __builtin_bit_cast(u16x2, w[k >> 2][k & 3] & 0x7fff7fffu);
+    m = __builtin_elementwise_max(m, t);
+  }
+  uint32_t top = m[0] > m[1] ? m[0] : m[1];
+  top = max(top, (uint32_t)__shfl_xor((int)top, 16));
+  top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+  if (__any(top >= Halves<T>::not_finite)) return false;
+  *scale = scale_byte(__float_as_uint(Halves<T>::value(top)));
+  const float s = scale_value(*scale, 0);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    u16x2 o = {0, 0};
+    o = Halves<T>::pack(o, w[k >> 1][(k & 1) * 2], s, false);
+    o = Halves<T>::pack(o, w[k >> 1][(k & 1) * 2 + 1], s, true);
+    (*a)[k] = __builtin_bit_cast(int, o);
+  }
+  return true;
+}
+
 template <typename T>
 __global__ __launch_bounds__(kFewWaves * 64) void few_rows_kernel(
     edl_fp8_gemm g, const T* __restrict__ x, int64_t x_ld, int K, bool wide) {
@@ -1114,24 +1214,23 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_rows_kernel(
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 2
   for (int kb = wave; kb < kbs; kb += kFewWaves) {
-    i32x8 b = *reinterpret_cast<const i32x8*>(pb + (int64_t)kb * kBlk);
-    int sb = ps[(int64_t)kb * g.b_rp];
-    float v[32];
-    uint32_t m = 0;
-#pragma unroll
-    for (int k = 0; k < 32; k += 8)
-      load_row8<T>(x, x_ld, g.M, K, row, (int64_t)kb * kBlk + q4 * 32 + k,
-                   wide, v + k);
-#pragma unroll
-    for (int k = 0; k < 32; ++k) m = max(m, finite_abs(v[k]));
-    m = max(m, (uint32_t)__shfl_xor((int)m, 16));
-    m = max(m, (uint32_t)__shfl_xor((int)m, 32));
-    const int sa = scale_byte(m);
-    const float inv = inverse_of(sa);
+    const i32x8 b = *reinterpret_cast<const i32x8*>(pb + (int64_t)kb * kBlk);
+    const int sb = ps[(int64_t)kb * g.b_rp];
+    const int64_t k0 = (int64_t)kb * kBlk + q4 * 32;
     i32x8 a;
+    int sa;
+    bool done = false;
+    if constexpr (sizeof(T) == 2) {
+      if (wide && (kb + 1) * kBlk <= K) {  // the wave alike
+        u32x4 w[4];
+        const T* p = x + (row < g.M ? row : 0) * x_ld + k0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      a[k] = pack4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3], inv);
+        for (int k = 0; k < 4; ++k)
+          w[k] = *reinterpret_cast<const u32x4*>(p + k * 8);
+        done = round32_fast<T>(w, &sa, &a);
+      }
+    }
+    if (!done) a = round32<T>(x, x_ld, g.M, K, row, k0, wide, &sa);
     if (sizeof(T) == 4)  // the result is in 32 bits
       acc = mfma_wide(widen(b, scale_value(sb, 0)),
                       widen(a, scale_value(sa, 0)), acc);
@@ -1164,28 +1263,47 @@ int64_t tiles_of(const edl_fp8_quant& a) {
   return ((a.R + kBlk - 1) / kBlk) * ((a.C + kBlk - 1) / kBlk);
 }
 
+constexpr int64_t kManyTiles = 1024;  // four a CU
+
+template <typename T, int ROWS>
+void launch_quantize_by(const edl_fp8_quant& a, hipStream_t st) {
+  dim3 grid((unsigned)tiles_of(a)), block(2048 / ROWS);
+  if (a.tile)
+    quantize_kernel<T, ROWS, true, false><<<grid, block, 0, st>>>(a);
+  else if (a.deriv)
+    quantize_kernel<T, ROWS, false, true><<<grid, block, 0, st>>>(a);
+  else
+    quantize_kernel<T, ROWS, false, false><<<grid, block, 0, st>>>(a);
+}
 template <typename T>
 void launch_quantize(const edl_fp8_quant& a, hipStream_t st) {
-  dim3 grid((unsigned)tiles_of(a)), block(kQuantThreads);
-  if (a.tile)
-    quantize_kernel<T, true, false><<<grid, block, 0, st>>>(a);
-  else if (a.deriv)
-    quantize_kernel<T, false, true><<<grid, block, 0, st>>>(a);
+  if (tiles_of(a) >= kManyTiles)
+    launch_quantize_by<T, 8>(a, st);
   else
-    quantize_kernel<T, false, false><<<grid, block, 0, st>>>(a);
+    launch_quantize_by<T, 4>(a, st);
 }
 
-template <typename TX>
+template <typename TX, int ROWS>
 void launch_quantize_pair(const edl_fp8_quant& x, const edl_fp8_quant& w,
                           hipStream_t st) {
   const int n = (int)tiles_of(x);
-  dim3 grid((unsigned)(n + tiles_of(w))), block(kQuantThreads);
+  dim3 grid((unsigned)(n + tiles_of(w))), block(2048 / ROWS);
   if (w.type == EDL_T_F32)
-    quantize_pair_kernel<TX, float><<<grid, block, 0, st>>>(x, w, n);
+    quantize_pair_kernel<TX, float, ROWS><<<grid, block, 0, st>>>(x, w, n);
   else if (w.type == EDL_T_BF16)
-    quantize_pair_kernel<TX, __bf16><<<grid, block, 0, st>>>(x, w, n);
+    quantize_pair_kernel<TX, __bf16, ROWS><<<grid, block, 0, st>>>(x, w, n);
   else
-    quantize_pair_kernel<TX, _Float16><<<grid, block, 0, st>>>(x, w, n);
+    quantize_pair_kernel<TX, _Float16, ROWS><<<grid, block, 0, st>>>(x, w, n);
+}
+template <int ROWS>
+void launch_quantize_pair_by(const edl_fp8_quant& x, const edl_fp8_quant& w,
+                             hipStream_t st) {
+  if (x.type == EDL_T_F32)
+    launch_quantize_pair<float, ROWS>(x, w, st);
+  else if (x.type == EDL_T_BF16)
+    launch_quantize_pair<__bf16, ROWS>(x, w, st);
+  else
+    launch_quantize_pair<_Float16, ROWS>(x, w, st);
 }
 
 int64_t tiles_of(const edl_fp8_gemm& g, int64_t bm, int64_t bn) {
@@ -1211,12 +1329,10 @@ extern "C" int edl_fp8_quantize(const edl_fp8_quant* a, hipStream_t st) {
 
 extern "C" int edl_fp8_quantize_pair(const edl_fp8_quant* x,
                                      const edl_fp8_quant* w, hipStream_t st) {
-  if (x->type == EDL_T_F32)
-    launch_quantize_pair<float>(*x, *w, st);
-  else if (x->type == EDL_T_BF16)
-    launch_quantize_pair<__bf16>(*x, *w, st);
+  if (tiles_of(*x) + tiles_of(*w) >= kManyTiles)
+    launch_quantize_pair_by<8>(*x, *w, st);
   else
-    launch_quantize_pair<_Float16>(*x, *w, st);
+    launch_quantize_pair_by<4>(*x, *w, st);
   return (int)hipGetLastError();
 }
 

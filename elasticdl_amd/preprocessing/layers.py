@@ -298,15 +298,28 @@ def fit_normalizer(values: torch.Tensor) -> "Normalizer":
 class SparseEmbedding(nn.Module):
     """Local (non-PS) embedding over padded variable-length ids with a
     combiner (reference: sparse_embedding.py:20). For the PS-distributed
-    version use elasticdl_amd.layers.embedding.EdlEmbedding(combiner=...)."""
+    version use elasticdl_amd.layers.embedding.EdlEmbedding(combiner=...).
 
-    def __init__(self, input_dim: int, output_dim: int, combiner: str = "sum"):
+    On a GPU the lookup, its pooling and the table's gradient are the kernels
+    of ops/embedding.py, straight from the padded ids. ``scale`` multiplies
+    the result; ``weights`` [batch, max_len] each id's row."""
+
+    def __init__(self, input_dim: int, output_dim: int, combiner: str = "sum",
+                 scale: float = 1.0):
         super().__init__()
         mode = {"sum": "sum", "mean": "mean", "sqrtn": "sum"}[combiner]
         self.combiner = combiner
+        self.scale = scale
         self.bag = nn.EmbeddingBag(input_dim, output_dim, mode=mode)
 
-    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+    def forward(self, ids: torch.Tensor,
+                weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+        native = ids.is_cuda and self.bag.weight.dtype != torch.float64
+        if native or weights is not None or self.scale != 1.0:
+            from elasticdl_amd.ops.embedding import embedding_lookup
+
+            return embedding_lookup(self.bag.weight, ids, weights,
+                                    self.combiner, self.scale)
         mask = ids >= 0
         flat = ids[mask]
         offsets = torch.zeros(ids.shape[0] + 1, dtype=torch.int64,

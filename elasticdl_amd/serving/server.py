@@ -9,6 +9,9 @@ predictions over HTTP (FastAPI/uvicorn), bf16 on GPU.
     python -m elasticdl_amd.serving.server \
         --model_def mnist --model_path /ckpt/model.pt --port 8500
 
+With --precision fp8 the FusedDense towers are served in 8-bit floating
+point, their weights laid out once at start.
+
     POST /v1/models/default:predict   {"instances": [[...], ...]}
     GET  /health
 """
@@ -20,13 +23,15 @@ import torch
 
 from elasticdl_amd.common.args import parse_model_params
 from elasticdl_amd.common.log_utils import default_logger as logger
+from elasticdl_amd.ops.functional import PRECISIONS, set_dense_precision
 from elasticdl_amd.utils.model_utils import get_model_spec
 
 
 class ModelRunner:
     def __init__(self, model_def: str, model_path: str = "",
                  model_params: str = "", device: str = "auto",
-                 dtype: Optional[torch.dtype] = None):
+                 dtype: Optional[torch.dtype] = None,
+                 precision: str = "bf16"):
         if device == "auto":
             device = "cuda" if torch.cuda.is_available() else "cpu"
         self.device = torch.device(device)
@@ -41,6 +46,12 @@ class ModelRunner:
             dtype = torch.bfloat16 if self.device.type == "cuda" else torch.float32
         self.dtype = dtype
         self.model = self.model.to(self.device, dtype).eval()
+        self.precision = precision
+        if precision != "bf16":
+            found = set_dense_precision(self.model, precision, freeze=True)
+            if not found:
+                raise ValueError(
+                    f"{model_def} has no dense layers to serve in {precision}")
         self.input_dtype = self._infer_input_dtype()
         logger.info("Serving %s on %s (%s)", model_def, self.device, dtype)
 
@@ -113,6 +124,7 @@ def main(argv=None) -> int:
     ap.add_argument("--model_path", default="")
     ap.add_argument("--model_params", default="")
     ap.add_argument("--device", default="auto")
+    ap.add_argument("--precision", default="bf16", choices=PRECISIONS)
     ap.add_argument("--host", default="0.0.0.0")
     ap.add_argument("--port", type=int, default=8500)
     args = ap.parse_args(argv)
@@ -120,7 +132,7 @@ def main(argv=None) -> int:
     import uvicorn
 
     runner = ModelRunner(args.model_def, args.model_path, args.model_params,
-                         args.device)
+                         args.device, precision=args.precision)
     uvicorn.run(build_app(runner), host=args.host, port=args.port)
     return 0
 
