@@ -21,8 +21,10 @@ int edl_sort_rows(const void*, int, int64_t, int64_t, uint32_t* const*,
                   uint32_t* const*, uint32_t*, uint32_t*, hipStream_t);
 int edl_segment_chunk(int64_t, int, int);
 int64_t edl_sort_counts(int64_t);
-int edl_sort_unique_small(const int64_t*, int64_t, uint32_t*, uint32_t*,
-                          int64_t*, uint32_t*, hipStream_t);
+int edl_sort_rows_small(const void*, int, int64_t, int64_t, uint32_t*,
+                        uint32_t*, uint32_t*, uint32_t*, hipStream_t);
+int edl_sort_ids_small(const int64_t*, int64_t, uint32_t*, uint32_t*,
+                       uint32_t*, int64_t*, uint32_t*, hipStream_t);
 int edl_ids_range(const int64_t*, int64_t, int64_t*, hipStream_t);
 int edl_sort_ids32_first(const int64_t*, int, int64_t, uint32_t* const*,
                          uint32_t* const*, uint32_t*, uint32_t*, hipStream_t);
@@ -186,6 +188,23 @@ struct SortSpace {
   }
 };
 
+struct SmallSpace {  // of a one-workgroup sort
+  uint32_t *pos = nullptr, *starts = nullptr, *runs = nullptr,
+           *rows = nullptr;
+  SmallSpace(Pieces& pieces, int64_t n, bool with_rows) {
+    pieces.add(&pos, n);
+    pieces.add(&starts, n);
+    pieces.add(&runs, 1);
+    if (with_rows) pieces.add(&rows, n);
+  }
+  void into(edl_segments& s) const {
+    s.pos = pos;
+    s.starts = starts;
+    s.runs = runs;
+    s.rows = rows;
+  }
+};
+
 class Lookup : public torch::autograd::Function<Lookup> {
  public:
   // grad: whether the caller's gradients are on
@@ -296,6 +315,17 @@ class Lookup : public torch::autograd::Function<Lookup> {
     s.w_type = a.w_type;
     s.out = dt.data_ptr();
     Pieces pieces;
+    if (n <= EDL_SORT_SMALL) {
+      SmallSpace small(pieces, n, true);
+      const Tensor space = pieces.place(ids);
+      launched(edl_sort_rows_small(a.ids, a.ids64, rows, n, small.pos,
+                                   small.starts, small.runs, small.rows,
+                                   stream_of(ids)),
+               "sort of ids");
+      small.into(s);
+      launched(edl_segment_sums(&s, stream_of(ids)), "embedding gradient");
+      return;
+    }
     SortSpace sort(pieces, n);
     segments_into(s, pieces);
     const Tensor space = pieces.place(ids);
@@ -384,21 +414,14 @@ std::vector<Tensor> coalesce_rows(Tensor values, Tensor ids) {
   const auto wait = [&] {  // for what was launched before the mark
     TORCH_CHECK(hipEventSynchronize(known) == hipSuccess, "event wait");
   };
-  uint32_t* place = nullptr;
-  Pieces pieces;
-  pieces.add(&place, n);
-  SortSpace sort(pieces, n);
   edl_segments s = {};
   s.N = n;
   s.D = (int)d;
   s.vec = vec_of(values, d, d);
-  if (d > 0) segments_into(s, pieces);
-  const Tensor space = pieces.place(ids);
   s.src = values.data_ptr();
   s.type = type;
   s.L = 1;
   s.scale = 1.f;
-  s.keys = place;
   s.limit = (uint32_t)n;
   // small results are summed into room for n rows before the host knows how
   // many there are, which takes it longer than the sums take
@@ -411,18 +434,32 @@ std::vector<Tensor> coalesce_rows(Tensor values, Tensor ids) {
   };
   int64_t found = -1;
   if (n <= EDL_SORT_SMALL) {
-    s.pos = sort.p[0];
-    launched(edl_sort_unique_small(id, n, place, sort.p[0], ids_out, found_at,
-                                   st),
+    Pieces pieces;
+    SmallSpace small(pieces, n, false);
+    const Tensor space = pieces.place(ids);
+    launched(edl_sort_ids_small(id, n, small.pos, small.starts, small.runs,
+                                ids_out, found_at, st),
              "sort of ids");
     mark();
+    small.into(s);
     if (early) sum_into(n);
     wait();
-    if (found_at[1] == 0) found = found_at[0];
+    if (found_at[1] == 0) {
+      found = found_at[0];
+      if (!early) sum_into(found);
+      return {rows.narrow(0, 0, found), unique.narrow(0, 0, found)};
+    }
+    s.starts = s.runs = nullptr;  // too far apart
   }
+  uint32_t* place = nullptr;
+  Pieces pieces;
+  pieces.add(&place, n);
+  SortSpace sort(pieces, n);
+  if (d > 0) segments_into(s, pieces);
+  const Tensor space = pieces.place(ids);
+  s.keys = place;
   Tensor wide;  // 64-bit keys
-  if (found < 0) {
-    rows = Tensor();
+  {
     constexpr int kFirst = 9;
     launched(edl_ids_range(id, n, range, st), "range of ids");
     mark();
@@ -463,8 +500,8 @@ std::vector<Tensor> coalesce_rows(Tensor values, Tensor ids) {
     if (early) sum_into(n);
     wait();
     found = found_at[0];
+    if (!early) sum_into(found);
   }
-  if (!rows.defined()) sum_into(found);
   return {rows.narrow(0, 0, found), unique.narrow(0, 0, found)};
 }
 

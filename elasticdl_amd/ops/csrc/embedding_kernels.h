@@ -43,7 +43,10 @@ struct edl_segments {
   const void* weights;  // by pos, or null
   int w_type;
   void* out;  // [limit, D] of src's type: row keys[i]
-  // workspace: a row of sums for each chunk's open beginning and end
+  // where one workgroup sorted: each run's first token, how many runs there
+  // are, and their rows (null: the run's own number); keys is not used
+  const uint32_t *starts, *runs, *rows;
+  // else a workspace: a row of sums for each chunk's open beginning and end
   float* part;                // [chunks, 2, D]
   uint32_t *head, *tail;      // [chunks]: their keys
   uint32_t *list, *listed;    // long runs, and how many

@@ -405,20 +405,22 @@ __global__ __launch_bounds__(256) void sort_move_kernel(
 }
 
 // Up to EDL_SORT_SMALL items in one workgroup, all passes in LDS: one launch
-// in the place of three a pass. A wave takes a run of 64 * items of them.
+// in the place of three a pass. A wave takes a run of 64 * items of them. Out
+// come the items in order, where each run of equal keys starts, and how many
+// runs there are (runs[0]).
 //
-// UNIQUE: ids of any value, taken relative to the smallest. Also the unique
-// ids in order, each item's place among them, and for the host how many
-// there are (found[0]), or in found[1] that they lie too far apart for 32
-// bits, and places of zero.
+// IDS: ids of any value, taken relative to the smallest; the runs' ids go to
+// `unique`, and for the host how many there are (found[0]), or in found[1]
+// that they lie too far apart for 32 bits, and no runs. Else rows of a table:
+// the runs' go to `rows`.
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallItems = EDL_SORT_SMALL / kSmallThreads;
 constexpr int kSmallWaves = kSmallThreads / 64;
 
-template <typename S, bool UNIQUE>
+template <typename S, bool IDS>
 __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
-    S src, int N, int bits_all, uint32_t* keys_out, uint32_t* pos_out,
-    int64_t* unique, uint32_t* found) {
+    S src, int N, int bits_all, uint32_t* pos_out, uint32_t* starts,
+    uint32_t* runs, uint32_t* rows, int64_t* unique, uint32_t* found) {
   __shared__ uint32_t s_key[EDL_SORT_SMALL];
   __shared__ uint16_t s_pos[EDL_SORT_SMALL];
   __shared__ __align__(16) uint16_t cnt[kSmallWaves][256];
@@ -431,7 +433,7 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
   uint32_t key[kSmallItems], pos[kSmallItems];
   int bits = bits_all;
   int64_t low = 0;
-  if constexpr (UNIQUE) {
+  if constexpr (IDS) {
     int64_t mn = INT64_MAX, mx = INT64_MIN;
     int64_t v[kSmallItems];
 #pragma unroll
@@ -462,8 +464,8 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
     const uint64_t range = (uint64_t)mx - (uint64_t)mn;
     const bool far = range >> 32 != 0;
     if (tid == 0) found[1] = far;
-    if (far) {  // all threads alike; what is launched behind stays in bounds
-      for (int i = tid; i < N; i += kSmallThreads) keys_out[i] = pos_out[i] = 0;
+    if (far) {  // all threads alike
+      if (tid == 0) runs[0] = 0;
       return;
     }
     low = mn;
@@ -539,46 +541,42 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
     __syncthreads();
     shift += b;
   }
-  if constexpr (UNIQUE) {
-    // each key's place: first occurrences before it, by wave, then overall
-    uint32_t here = 0, place[kSmallItems];
-    bool first[kSmallItems];
+  // each run's number: first occurrences before it, by wave, then overall
+  uint32_t here = 0, place[kSmallItems];
+  bool first[kSmallItems];
 #pragma unroll
-    for (int k = 0; k < kSmallItems; ++k) {
-      const int i = i0 + k * 64;
-      first[k] = k < items && i < N && (i == 0 || s_key[i - 1] != key[k]);
-      const uint64_t set = __ballot(first[k]);
-      place[k] = here + __builtin_amdgcn_mbcnt_hi(
-                            (uint32_t)(set >> 32),
-                            __builtin_amdgcn_mbcnt_lo((uint32_t)set, 0));
-      here += __popcll(set);
-    }
-    if (lane == 0) local[wave] = here;
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-    for (int w = 0; w < kSmallWaves; ++w) {
-      if (w < wave) before += local[w];
-      all += local[w];
-    }
-    if (tid == 0) found[0] = all;
+  for (int k = 0; k < kSmallItems; ++k) {
+    const int i = i0 + k * 64;
+    first[k] = k < items && i < N && (i == 0 || s_key[i - 1] != key[k]);
+    const uint64_t set = __ballot(first[k]);
+    place[k] = here + __builtin_amdgcn_mbcnt_hi(
+                          (uint32_t)(set >> 32),
+                          __builtin_amdgcn_mbcnt_lo((uint32_t)set, 0));
+    here += __popcll(set);
+  }
+  if (lane == 0) local[wave] = here;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+  for (int w = 0; w < kSmallWaves; ++w) {
+    if (w < wave) before += local[w];
+    all += local[w];
+  }
+  if (tid == 0) {
+    runs[0] = all;
+    if constexpr (IDS) found[0] = all;
+  }
 #pragma unroll
-    for (int k = 0; k < kSmallItems; ++k) {
-      const int i = i0 + k * 64;
-      if (k < items && i < N) {
-        const uint32_t at = before + place[k] + first[k] - 1;
-        keys_out[i] = at;
-        pos_out[i] = pos[k];
-        if (first[k])
+  for (int k = 0; k < kSmallItems; ++k) {
+    const int i = i0 + k * 64;
+    if (k < items && i < N) {
+      pos_out[i] = pos[k];
+      if (first[k]) {
+        const uint32_t at = before + place[k];
+        starts[at] = i;
+        if constexpr (IDS)
           unique[at] = (int64_t)((uint64_t)low + (uint64_t)key[k]);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < kSmallItems; ++k) {
-      const int i = i0 + k * 64;
-      if (k < items && i < N) {
-        keys_out[i] = key[k];
-        pos_out[i] = pos[k];
+        else
+          rows[at] = key[k];
       }
     }
   }
@@ -795,6 +793,63 @@ __global__ __launch_bounds__(256) void segment_kernel(edl_segments a) {
   }
 }
 
+// where one workgroup has sorted and knows the runs: a wave to a run, its
+// groups of lanes taking every so-many-th token; one launch in place of three
+template <typename T, int VEC>
+__global__ __launch_bounds__(256) void segment_run_kernel(edl_segments a) {
+  typedef Vec<T, VEC> V;
+  constexpr int U = 4;
+  const int lanes = lanes_of(a.D, VEC), pieces = pieces_of(a.D, VEC);
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 6;
+  const uint32_t run = (uint32_t)(unit / pieces), runs = *a.runs;
+  if (run >= runs) return;
+  const int64_t to = a.rows ? a.rows[run] : run;
+  if (to >= a.limit) return;
+  const int col =
+      ((int)(unit % pieces) * lanes + (lane & (lanes - 1))) * VEC;
+  const bool mine = col < a.D;
+  const T* src = static_cast<const T*>(a.src) + (mine ? col : 0);
+  const int groups = 64 / lanes;
+  const uint32_t end = run + 1 < runs ? a.starts[run + 1] : (uint32_t)a.N;
+  float acc[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
+  for (uint32_t t = a.starts[run] + lane / lanes; t < end; t += groups * U) {
+    uint32_t row[U];
+    float w[U];
+    V v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = t + u * groups < end;
+      const uint32_t p = a.pos[in ? t + u * groups : t];
+      row[u] = a.L > 1 ? p / (uint32_t)a.L : p;
+      w[u] = a.weights ? load_any(a.weights, p, a.w_type) : 1.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      v[u].v = *reinterpret_cast<const decltype(v[u].v)*>(
+          src + (int64_t)row[u] * a.D);
+      w[u] *= a.coef ? a.coef[row[u]] : a.scale;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (t + u * groups < end) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] += w[u] * v[u].get(k);
+      }
+  }
+  for (int o = lanes; o < 64; o <<= 1)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) acc[k] += __shfl_xor(acc[k], o);
+  if (lane >= lanes || !mine) return;
+  V o;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) o.set(k, acc[k]);
+  *reinterpret_cast<decltype(o.v)*>(static_cast<T*>(a.out) + to * a.D + col) =
+      o.v;
+}
+
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void segment_short_kernel(edl_segments a,
                                                             int64_t chunks) {
@@ -923,6 +978,11 @@ void launch_weight_grad(const edl_bag& a, hipStream_t st) {
 }
 template <typename T, int VEC>
 void launch_segments(const edl_segments& a, hipStream_t st) {
+  if (a.starts) {
+    segment_run_kernel<T, VEC>
+        <<<blocks_for(a.N * pieces_of(a.D, VEC) * 64), 256, 0, st>>>(a);
+    return;
+  }
   const int64_t chunks = (a.N + a.chunk - 1) / a.chunk;
   const int64_t threads =
       chunks * pieces_of(a.D, VEC) * lanes_of(a.D, VEC);
@@ -1058,12 +1118,6 @@ extern "C" int edl_sort_rows(const void* ids, int ids64, int64_t V, int64_t N,
   int bits = 1;
   while (bits < 32 && (V >> bits) != 0) ++bits;
   Keys32 src{ids, ids64 != 0, V};
-  if (N <= EDL_SORT_SMALL) {
-    sort_small_kernel<Keys32, false><<<1, kSmallThreads, 0, st>>>(
-        src, (int)N, bits, keys[0], pos[0], nullptr, nullptr);
-    const int rc = (int)hipGetLastError();
-    return rc ? -1 - rc : 0;
-  }
   return sort_all(src, N, bits, keys, pos, counts, totals, st);
 }
 
@@ -1084,13 +1138,24 @@ extern "C" int64_t edl_sort_counts(int64_t N) {
 #undef EDL_COUNTS
 }
 
-// the small sort of ids of any value: see the kernel
-extern "C" int edl_sort_unique_small(const int64_t* ids, int64_t N,
-                                     uint32_t* place, uint32_t* pos,
-                                     int64_t* unique, uint32_t* found,
-                                     hipStream_t st) {
+// the one-workgroup sorts: see the kernel
+extern "C" int edl_sort_rows_small(const void* ids, int ids64, int64_t V,
+                                   int64_t N, uint32_t* pos, uint32_t* starts,
+                                   uint32_t* runs, uint32_t* rows,
+                                   hipStream_t st) {
+  int bits = 1;
+  while (bits < 32 && (V >> bits) != 0) ++bits;
+  sort_small_kernel<Keys32, false><<<1, kSmallThreads, 0, st>>>(
+      Keys32{ids, ids64 != 0, V}, (int)N, bits, pos, starts, runs, rows,
+      nullptr, nullptr);
+  return (int)hipGetLastError();
+}
+extern "C" int edl_sort_ids_small(const int64_t* ids, int64_t N, uint32_t* pos,
+                                  uint32_t* starts, uint32_t* runs,
+                                  int64_t* unique, uint32_t* found,
+                                  hipStream_t st) {
   sort_small_kernel<Keys32Of, true><<<1, kSmallThreads, 0, st>>>(
-      Keys32Of{ids}, (int)N, 0, place, pos, unique, found);
+      Keys32Of{ids}, (int)N, 0, pos, starts, runs, nullptr, unique, found);
   return (int)hipGetLastError();
 }
 

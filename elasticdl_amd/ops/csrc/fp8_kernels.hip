@@ -534,11 +534,12 @@ __device__ inline float sum16(float v) {
 }
 
 // Of a lane's 16 sums v (bias apart), those that with their bias lie within
-// 2^-13 of their neighbours' size from zero are replaced by dot_of. The size
+// 2^-12 of their neighbours' size from zero are replaced by dot_of. The size
 // is a mean, and of the means of every other neighbour the smaller, which one
-// large value does not move; at C's right edge, over 16 rows. 2^-13 of it is
-// 6 times the usual error of a sum. One value in 15000 is met; each takes the
-// wave some 3 us, and a wave stops after 32 of its 1024.
+// large value does not move; at C's right edge, over 16 rows. 2^-12 of it is
+// 11 times the usual error of a sum (with 2^-13 a few in 67 million signs were
+// still other than in 64 bits). One value in 8000 is met; each takes the wave
+// some 3 us, and a wave stops after 32 of its 1024.
 __device__ inline void settle(const edl_fp8_gemm& g, int64_t m, int64_t n,
                               float* v, const float* bias, bool live) {
   const int lane = threadIdx.x & 63;
@@ -562,7 +563,7 @@ __device__ inline void settle(const edl_fp8_gemm& g, int64_t m, int64_t n,
   }
   const float a = count[0] > 0.f ? sum[0] / count[0] : 0.f;
   const float b = count[1] > 0.f ? sum[1] / count[1] : a;
-  const float size = (a < b ? a : b) * (1.f / 8192);
+  const float size = (a < b ? a : b) * (1.f / 4096);
   uint32_t near = 0;
 #pragma unroll
   for (int k = 0; k < 16; ++k)
