@@ -225,11 +225,13 @@ struct Plan16x9 {
   static constexpr int ITEMS = 16, BITS = 9;
 };
 
-// the lanes among `in` whose digit of `bits` bits is this lane's
-__device__ inline uint64_t same_digit(uint32_t d, int bits, bool in) {
+// the lanes among `in` whose digit of BITS bits is this lane's
+template <int BITS>
+__device__ inline uint64_t same_digit(uint32_t d, bool in) {
   const uint64_t all = __ballot(in);
   uint32_t lo = (uint32_t)all, hi = (uint32_t)(all >> 32);
-  for (int b = 0; b < bits; ++b) {
+#pragma unroll
+  for (int b = 0; b < BITS; ++b) {
     const uint32_t mine = (uint32_t)((int32_t)(d << (31 - b)) >> 31);
     const uint64_t set = __ballot((int32_t)mine < 0);
     lo &= ~((uint32_t)set ^ mine);
@@ -239,10 +241,9 @@ __device__ inline uint64_t same_digit(uint32_t d, int bits, bool in) {
 }
 // a lane's rank among the wave's items of its digit so far, which `count`
 // holds by digit: read by all, then moved on by the first of each digit
-template <typename C>
-__device__ inline uint32_t rank_digit(volatile C* count, uint32_t d, int bits,
-                                      bool in) {
-  const uint64_t same = same_digit(d, bits, in);
+template <int BITS, typename C>
+__device__ inline uint32_t rank_digit(volatile C* count, uint32_t d, bool in) {
+  const uint64_t same = same_digit<BITS>(d, in);
   const uint32_t lower = __builtin_amdgcn_mbcnt_hi(
       (uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
   const uint32_t old = count[d];
@@ -353,8 +354,8 @@ __global__ __launch_bounds__(256) void sort_move_kernel(
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k)
-    rank[k] = rank_digit<uint16_t>(
-        cnt[wave], (uint32_t)(key[k] >> shift) & (bins - 1), bits,
+    rank[k] = rank_digit<P::BITS, uint16_t>(
+        cnt[wave], (uint32_t)(key[k] >> shift) & (bins - 1),
         first + k * 64 < N);
   __syncthreads();
   uint32_t sum[kOwn], sums = 0, tots = 0;
@@ -424,6 +425,7 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
   __shared__ uint32_t s_key[EDL_SORT_SMALL];
   __shared__ uint16_t s_pos[EDL_SORT_SMALL];
   __shared__ __align__(16) uint16_t cnt[kSmallWaves][256];
+  __shared__ uint16_t quarters[4][256];
   __shared__ uint32_t local[256];
   __shared__ int64_t s_min[kSmallWaves], s_max[kSmallWaves];
   __shared__ uint32_t s4[4];
@@ -495,17 +497,28 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
 #pragma unroll
     for (int k = 0; k < kSmallItems; ++k)
       if (k < items)  // whole waves
-        rank[k] = rank_digit<uint16_t>(cnt[wave], (key[k] >> shift) & digits,
-                                       b, i0 + k * 64 < N);
+        rank[k] = rank_digit<8, uint16_t>(
+            cnt[wave], (key[k] >> shift) & digits, i0 + k * 64 < N);
     __syncthreads();
-    uint32_t total = 0;
-    if (tid < 256) {
-      for (int w = 0; w < kSmallWaves; ++w) {
-        const uint32_t t = cnt[w][tid];
-        cnt[w][tid] = (uint16_t)total;
-        total += t;
-      }
+    // a digit's counts, wave by wave: four threads take four waves each
+    const int digit = tid & 255, quarter = tid >> 8;
+    uint32_t mine4[4], sum4 = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      mine4[w] = sum4;
+      sum4 += cnt[quarter * 4 + w][digit];
     }
+    quarters[quarter][digit] = (uint16_t)sum4;
+    __syncthreads();
+    uint32_t total = 0, lead = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (q < quarter) lead += quarters[q][digit];
+      total += quarters[q][digit];
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      cnt[quarter * 4 + w][digit] = (uint16_t)(lead + mine4[w]);
     // exclusive sum over the 256 digits, by the first four waves
     uint32_t x = total;
     for (int o = 1; o < 64; o <<= 1) {
