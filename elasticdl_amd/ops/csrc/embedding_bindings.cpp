@@ -5,10 +5,12 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
 #include <cstdint>
+#include <exception>
 #include <limits>
 
 #include "embedding_kernels.h"
@@ -220,9 +222,6 @@ class Lookup : public torch::autograd::Function<Lookup> {
     ids = ids.contiguous();
     edl_bag a = bag_of(ids, weights, combiner, scale);
     table_into(a, table, ids);
-    TORCH_CHECK(a.B * ((int64_t)a.D + 64) / 256 <
-                    std::numeric_limits<int32_t>::max(),
-                "the result is too large");
     Tensor out =
         torch::empty({a.B, a.D}, table.options().requires_grad(false));
     a.out = out.data_ptr();
@@ -391,6 +390,10 @@ std::vector<Tensor> coalesce_rows(Tensor values, Tensor ids) {
   const int64_t n = ids.size(0), d = values.size(1);
   TORCH_CHECK(n < kMost, "too many ids: ", n);
   c10::DeviceGuard guard(ids.device());
+  TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() ==
+                  c10::hip::CaptureStatus::None,
+              "coalesce_rows reads back how many ids there are and cannot be "
+              "captured into a graph");
   auto opts = values.options().requires_grad(false);
   const int type = type_code(values.scalar_type(), "values");
   if (n == 0) return {torch::empty({0, d}, opts), torch::empty_like(ids)};
@@ -407,6 +410,15 @@ std::vector<Tensor> coalesce_rows(Tensor values, Tensor ids) {
                        true));
   uint32_t* found_at = reinterpret_cast<uint32_t*>(host.data_ptr<int64_t>());
   int64_t* range = host.data_ptr<int64_t>() + 1;
+  // an error on the way does not give that memory back while kernels that
+  // were launched may write to it
+  struct Settled {
+    hipStream_t st;
+    int thrown = std::uncaught_exceptions();
+    ~Settled() {
+      if (std::uncaught_exceptions() > thrown) (void)hipStreamSynchronize(st);
+    }
+  } settled{st};
   const hipEvent_t known = event_of(ids.device().index());
   const auto mark = [&] {
     TORCH_CHECK(hipEventRecord(known, st) == hipSuccess, "event record");

@@ -69,14 +69,15 @@ __host__ __device__ inline int pieces_of(int D, int vec) {
 // that 8 rows are in flight; `subs` such groups share a bag, each taking
 // every so-many-th eight, where bags alone are too few to fill the chip.
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void lookup_kernel(edl_bag a, int subs) {
+__global__ __launch_bounds__(256) void lookup_kernel(edl_bag a, int subs,
+                                                     int64_t block0) {
   typedef Vec<T, VEC> V;
   constexpr int U = 8;
   const int lanes = lanes_of(a.D, VEC), pieces = pieces_of(a.D, VEC);
   const int lane = threadIdx.x & 63;
   const int sub = (lane / lanes) & (subs - 1);
   const int64_t unit =
-      ((int64_t)blockIdx.x * 256 + threadIdx.x) / (lanes * subs);
+      ((block0 + blockIdx.x) * 256 + threadIdx.x) / (lanes * subs);
   const int64_t bag = unit / pieces;
   const int col = ((int)(unit % pieces) * lanes + (lane & (lanes - 1))) * VEC;
   if (bag >= a.B) return;  // whole groups of lanes * subs
@@ -136,11 +137,12 @@ __global__ __launch_bounds__(256) void lookup_kernel(edl_bag a, int subs) {
 // the weights' gradient: a group of lanes keeps its bag's dy (its first
 // piece; wider rows read the rest again) and goes over the ids
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void weight_grad_kernel(edl_bag a) {
+__global__ __launch_bounds__(256) void weight_grad_kernel(edl_bag a,
+                                                          int64_t block0) {
   typedef Vec<T, VEC> V;
   constexpr int U = 4;
   const int lanes = lanes_of(a.D, VEC);
-  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
+  const int64_t unit = ((block0 + blockIdx.x) * 256 + threadIdx.x) / lanes;
   const int l_lane = threadIdx.x & (lanes - 1);
   // eight ids of a bag to a unit, so that long bags spread
   const int eights = (a.L + 7) / 8;
@@ -712,11 +714,12 @@ __global__ __launch_bounds__(256) void unique_place_kernel(
 constexpr int kShort = 8;
 
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void segment_kernel(edl_segments a) {
+__global__ __launch_bounds__(256) void segment_kernel(edl_segments a,
+                                                      int64_t block0) {
   typedef Vec<T, VEC> V;
   constexpr int U = 8;
   const int lanes = lanes_of(a.D, VEC), pieces = pieces_of(a.D, VEC);
-  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
+  const int64_t unit = ((block0 + blockIdx.x) * 256 + threadIdx.x) / lanes;
   const int64_t c = unit / pieces;
   const int col =
       ((int)(unit % pieces) * lanes + (threadIdx.x & (lanes - 1))) * VEC;
@@ -809,12 +812,13 @@ __global__ __launch_bounds__(256) void segment_kernel(edl_segments a) {
 // where one workgroup has sorted and knows the runs: a wave to a run, its
 // groups of lanes taking every so-many-th token; one launch in place of three
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void segment_run_kernel(edl_segments a) {
+__global__ __launch_bounds__(256) void segment_run_kernel(edl_segments a,
+                                                          int64_t block0) {
   typedef Vec<T, VEC> V;
   constexpr int U = 4;
   const int lanes = lanes_of(a.D, VEC), pieces = pieces_of(a.D, VEC);
   const int lane = threadIdx.x & 63;
-  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 6;
+  const int64_t unit = ((block0 + blockIdx.x) * 256 + threadIdx.x) >> 6;
   const uint32_t run = (uint32_t)(unit / pieces), runs = *a.runs;
   if (run >= runs) return;
   const int64_t to = a.rows ? a.rows[run] : run;
@@ -865,10 +869,11 @@ __global__ __launch_bounds__(256) void segment_run_kernel(edl_segments a) {
 
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void segment_short_kernel(edl_segments a,
-                                                            int64_t chunks) {
+                                                            int64_t chunks,
+                                                            int64_t block0) {
   typedef Vec<T, VEC> V;
   const int lanes = lanes_of(a.D, VEC), pieces = pieces_of(a.D, VEC);
-  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;
+  const int64_t unit = ((block0 + blockIdx.x) * 256 + threadIdx.x) / lanes;
   const int64_t c = unit / pieces;
   const int col =
       ((int)(unit % pieces) * lanes + (threadIdx.x & (lanes - 1))) * VEC;
@@ -967,8 +972,13 @@ __global__ __launch_bounds__(256) void segment_long_kernel(edl_segments a,
 }
 
 // -------------------------------- launches --------------------------------
-unsigned blocks_for(int64_t threads) {
-  return (unsigned)((threads + 255) / 256);
+// a launch holds fewer than 2^32 threads: more go in several
+template <typename F>
+void in_blocks(int64_t threads, F launch) {
+  constexpr int64_t kMost = 1 << 23;
+  const int64_t blocks = (threads + 255) / 256;
+  for (int64_t b0 = 0; b0 < blocks; b0 += kMost)
+    launch((unsigned)(blocks - b0 < kMost ? blocks - b0 : kMost), b0);
 }
 
 template <typename T, int VEC>
@@ -980,29 +990,35 @@ void launch_lookup(const edl_bag& a, hipStream_t st) {
   while (subs * lanes < 64 && subs * 8 < a.L &&
          a.B * pieces * lanes * subs < 256 * 32 * 64)
     subs *= 2;
-  lookup_kernel<T, VEC>
-      <<<blocks_for(a.B * pieces * lanes * subs), 256, 0, st>>>(a, subs);
+  in_blocks(a.B * pieces * lanes * subs, [&](unsigned n, int64_t b0) {
+    lookup_kernel<T, VEC><<<n, 256, 0, st>>>(a, subs, b0);
+  });
 }
 template <typename T, int VEC>
 void launch_weight_grad(const edl_bag& a, hipStream_t st) {
   const int64_t units = a.B * ((a.L + 7) / 8);
-  weight_grad_kernel<T, VEC>
-      <<<blocks_for(units * lanes_of(a.D, VEC)), 256, 0, st>>>(a);
+  in_blocks(units * lanes_of(a.D, VEC), [&](unsigned n, int64_t b0) {
+    weight_grad_kernel<T, VEC><<<n, 256, 0, st>>>(a, b0);
+  });
 }
 template <typename T, int VEC>
 void launch_segments(const edl_segments& a, hipStream_t st) {
   if (a.starts) {
-    segment_run_kernel<T, VEC>
-        <<<blocks_for(a.N * pieces_of(a.D, VEC) * 64), 256, 0, st>>>(a);
+    in_blocks(a.N * pieces_of(a.D, VEC) * 64, [&](unsigned n, int64_t b0) {
+      segment_run_kernel<T, VEC><<<n, 256, 0, st>>>(a, b0);
+    });
     return;
   }
   const int64_t chunks = (a.N + a.chunk - 1) / a.chunk;
   const int64_t threads =
       chunks * pieces_of(a.D, VEC) * lanes_of(a.D, VEC);
-  segment_kernel<T, VEC><<<blocks_for(threads), 256, 0, st>>>(a);
+  in_blocks(threads, [&](unsigned n, int64_t b0) {
+    segment_kernel<T, VEC><<<n, 256, 0, st>>>(a, b0);
+  });
   if (chunks == 1) return;
-  segment_short_kernel<T, VEC>
-      <<<blocks_for(threads), 256, 0, st>>>(a, chunks);
+  in_blocks(threads, [&](unsigned n, int64_t b0) {
+    segment_short_kernel<T, VEC><<<n, 256, 0, st>>>(a, chunks, b0);
+  });
   if (chunks <= kShort + 1) return;
   segment_long_kernel<T, VEC><<<256, 256, 0, st>>>(a, chunks);
 }

@@ -45,7 +45,12 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor,
     sqrtn's divisor counts ids, not weights. The result has the table's type
     (float32, bfloat16 or float16), rounded once from a sum in 32 bits. The
     table's gradient is dense, in the table's type; weights have one too.
-    Rows of the table may be strided."""
+    Rows of the table may be strided; ids are fewer than 2^31 - 4096.
+
+    In code that is captured into a graph, take gradients with
+    ``torch.autograd.grad`` (or drop eager graphs of the same leaves first):
+    ``backward()`` accumulates on the stream of the eager graph's leaves,
+    which ends the capture."""
     code = _COMBINERS.get(combiner)
     if code is None:
         raise ValueError(f"unknown combiner {combiner!r}")
@@ -84,10 +89,6 @@ def coalesce_rows(values: torch.Tensor, ids: torch.Tensor
     if not values.is_cuda:
         raise ValueError("coalesce_rows runs on a GPU; use "
                          "deduplicate_indexed_slices")
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError(
-            "coalesce_rows reads back how many ids there are and cannot be "
-            "captured into a graph")
     rows, unique = require_native().coalesce_rows(
         values.detach().contiguous(), ids.contiguous())
     return rows, unique

@@ -6,6 +6,8 @@ factor that go into each term); the result's own rounding is half a step of
 its type.
 """
 
+import threading
+
 import pytest
 import torch
 
@@ -289,6 +291,93 @@ def test_on_a_stream_of_its_own():
     assert torch.equal(got, want)
 
 
+@pytest.mark.gpu
+def test_more_tokens_than_a_launch_has_threads():
+    # 66 columns of 16 bits: 64 lanes a row, so 2^26 rows are 2^32 threads
+    n, v, d = (1 << 26) + 1000, 1000, 66
+    g = torch.Generator(device="cuda").manual_seed(0)
+    table = torch.randint(-4, 5, (v, d), generator=g, device="cuda").bfloat16()
+    ids = torch.randint(0, v, (n, 1), generator=g, device="cuda",
+                        dtype=torch.int32)
+    weights = torch.ones(n, 1, dtype=torch.bfloat16, device="cuda")
+    weights[ids == 7] = 2.0
+    leaves = table.requires_grad_(True), weights.requires_grad_(True)
+    out = embedding_lookup(*leaves[:1], ids, leaves[1], "sum")
+    dt, dw = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    sums = table.detach().float().sum(1)
+    for at in (0, (1 << 25) - 500, (1 << 26) - 500, n - 1000):  # whole numbers
+        part = ids[at:at + 1000, 0].long()
+        row = table.detach()[part] * weights.detach()[at:at + 1000]
+        assert torch.equal(out[at:at + 1000], row)
+        assert torch.equal(dw[at:at + 1000, 0], sums[part].bfloat16())
+    count = torch.bincount(ids[:, 0].long(), minlength=v).float()
+    count[7] *= 2
+    assert torch.equal(dt, count.bfloat16().unsqueeze(1).expand(-1, d))
+
+
+@pytest.mark.gpu
+def test_two_graphs_and_eager_calls_in_turn():
+    tables = [randn(500, 16, seed=i).cuda().requires_grad_(True)
+              for i in range(2)]
+    ids = [torch.randint(-1, 500, (300, 40), generator=gen(i)).cuda()
+           for i in range(2)]
+    dy = randn(300, 16, seed=2).cuda()
+
+    def step(i):
+        out = embedding_lookup(tables[i], ids[i], None, "mean")
+        return out.detach(), torch.autograd.grad(out, tables[i], dy)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(0)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs, held = [], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            held.append(step(i))
+    want = [step(0), step(1)]
+    for i in (0, 1, 1, 0, 1):
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        for k in range(2):
+            assert torch.equal(step(i)[k], want[i][k])
+            assert torch.equal(held[i][k], want[i][k])
+
+
+@pytest.mark.gpu
+def test_threads_at_once():
+    jobs = []
+    for i in range(4):
+        n = (500, 9000, 60000, 8000)[i]
+        ids = torch.randint(0, 300, (n,), generator=gen(i)).cuda()
+        values = randn(n, 12, seed=i).cuda()
+        jobs.append((values, ids, coalesce_rows(values, ids)))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(values, ids, want):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got = coalesce_rows(values, ids)
+                    stream.synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                        bad.append("differs")
+        except Exception as e:  # shown by the test
+            bad.append(e)
+
+    threads = [threading.Thread(target=work, args=job) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad
+
+
 # ----------------------------- sums by id ---------------------------------
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("n,d,low,high", [
@@ -367,3 +456,21 @@ def test_refusals_on_a_gpu():
         coalesce_rows(values, ids[0].int().cuda())
     with pytest.raises(RuntimeError, match="dim"):
         coalesce_rows(values[:2], ids[0].cuda())
+
+
+@pytest.mark.gpu
+def test_coalesce_refuses_to_be_captured():
+    values, ids = randn(30, 4).cuda(), torch.arange(30).cuda() // 2
+    want = coalesce_rows(values, ids)
+    torch.cuda.synchronize()
+    x = torch.zeros(4, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x.add_(1.0)
+        with pytest.raises(RuntimeError, match="captured"):
+            coalesce_rows(values, ids)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(x, torch.ones(4, device="cuda"))
+    for a, b in zip(coalesce_rows(values, ids), want):
+        assert torch.equal(a, b)
