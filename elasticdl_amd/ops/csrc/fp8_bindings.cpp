@@ -185,6 +185,9 @@ void check_blocks(const Tensor& q, const Tensor& s, int64_t rows,
           s.size(0) == q.size(1) / EDL_FP8_BLOCK &&
           s.size(1) == round_up(rows, 256),
       name, " does not match: expected ", rows, " x ", contracted);
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(s.data_ptr()) % 16 == 0,
+              name, " must lie on a border of 16 bytes");
 }
 
 // c = a b^T; returns c, of `type`

@@ -675,7 +675,7 @@ struct Loads {
   static constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW;
   static constexpr int kAll = LA + LB + 1;
   i32x4 bufA, bufB, bufS;
-  uint32_t offA[LA], offB[LB], at = 0, atS = 0, rp;
+  uint32_t offA[LA], offB[LB], offS, at = 0, atS = 0, rp;
   int wave, lane;
   bool odd;
 
@@ -702,6 +702,10 @@ struct Loads {
     const uint8_t* ps = base + (odd ? s.n0 : s.m0) + s.kb0 * rows;
     bufS = buffer_of(ps, base + (int64_t)s.kb_all * rows - ps);
     rp = (uint32_t)rows;
+    // 256 bytes from a tile of fewer rows may be more than there are
+    offS = lane * 4;
+    if (BM < 256)
+      offS = (uint32_t)min((int64_t)offS, rows - 4 - (odd ? s.n0 : s.m0));
   }
   // the q-th load of the next block, into LDS at these places
   __device__ inline void one(uint32_t a, uint32_t b, uint32_t s, int q) {
@@ -711,7 +715,7 @@ struct Loads {
       const int o = q - LA;
       dma16(bufB, offB[o], at, b + (wave * LB + o) * 1024);
     } else if (q == LA + LB) {
-      dma4(bufS, lane * 4, atS, s + odd * 256);
+      dma4(bufS, offS, atS, s + odd * 256);
       at += kBlk;
       atS += rp;
     }
@@ -1015,9 +1019,9 @@ __device__ inline void gemm_ring(const edl_fp8_gemm& g, int block, int blocks,
   uint32_t buf = 0, ahead = 2;
   for (int t = 0; t < s.steps; ++t) {
     if (t + 1 < s.steps)
-      asm volatile("s_waitcnt vmcnt(7)\n\ts_barrier" ::: "memory");
+      asm volatile("s_waitcnt vmcnt(7) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     else
-      asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (t + 2 < s.steps) stage(ahead);
     const uint8_t* p = smem + buf * RingLds::kOne;
     H::read_scales(p + RingLds::kA + RingLds::kB + (lane & 15) * 4, fA0, wB,

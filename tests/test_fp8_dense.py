@@ -9,6 +9,8 @@ half a step of its type. A sigmoid is at most 1/4 as steep, and its own
 exp and division are off by less than 2^-20 of it.
 """
 
+import threading
+
 import pytest
 import torch
 
@@ -417,6 +419,101 @@ def test_same_call_twice_gives_the_same_bits():
         assert torch.equal(a, c)
 
 
+@pytest.mark.gpu
+def test_outputs_and_checkpoints_past_32_bit_offsets():
+    # whole numbers: e4m3 holds them, and every sum is below 2^24, so exact
+    m, k, n = (1 << 24) - 200, 130, 200
+    g = torch.Generator(device="cuda").manual_seed(0)
+
+    def whole(*shape, most):
+        return torch.randint(-most, most + 1, shape, generator=g,
+                             device="cuda", dtype=torch.int8).bfloat16()
+
+    x, w, b = whole(m, k, most=2), whole(n, k, most=2), whole(n, most=3)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = fp8_dense(*leaves, "relu")
+    dy = whole(m, n, most=1)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    x, w, b = (t.detach().float() for t in leaves)
+    want_w = torch.zeros(n, k, dtype=torch.float64, device="cuda")
+    want_b = torch.zeros(n, dtype=torch.float64, device="cuda")
+    step = 1 << 20
+    for at in range(0, m, step):
+        z = x[at:at + step] @ w.t() + b
+        assert torch.equal(y.detach()[at:at + step],
+                           z.clamp(min=0).bfloat16())
+        dz = dy[at:at + step].float() * (z > 0)
+        assert torch.equal(dx[at:at + step], (dz @ w).bfloat16())
+        want_w += (dz.t() @ x[at:at + step]).double()
+        want_b += dz.double().sum(0)
+    assert torch.equal(dw, want_w.bfloat16())
+    assert torch.equal(db, want_b.bfloat16())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [4, 300])
+def test_two_graphs_of_a_laid_out_weight(m):
+    layers = []
+    for i in range(2):
+        w = randn(200, 300, seed=i, dtype=torch.bfloat16).cuda()
+        b = randn(200, seed=5 + i).cuda()
+        layers.append((quantize_fp8_weight(w), b))
+    x = randn(m, 300, seed=9, dtype=torch.bfloat16).cuda()
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            fp8_dense(x, *layers[0], "relu")
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graphs, held = [], []
+        for w, b in layers:
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1]):
+                held.append(fp8_dense(x, w, b, "relu"))
+        for r, i in enumerate((0, 1, 1, 0, 1)):
+            x.copy_(randn(m, 300, seed=20 + r, dtype=torch.bfloat16).cuda())
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(held[i], fp8_dense(x, *layers[i], "relu"))
+
+
+@pytest.mark.gpu
+def test_threads_at_once():
+    jobs = []
+    for i in range(4):
+        x = randn(700, 256 + 64 * i, seed=i, dtype=torch.bfloat16).cuda()
+        w = randn(384, 256 + 64 * i, seed=9 + i, dtype=torch.bfloat16).cuda()
+
+        def step(x=x.requires_grad_(True), w=w.requires_grad_(True)):
+            y = fp8_dense(x, w, None, "relu")
+            return (y.detach(),
+                    *torch.autograd.grad(y, (x, w), torch.ones_like(y)))
+
+        jobs.append((step, step()))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(step, want):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got = step()
+                    stream.synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                        bad.append("differs")
+        except Exception as e:  # shown by the test
+            bad.append(e)
+
+    threads = [threading.Thread(target=work, args=job) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad
+
+
 # ------------------------------- refusals ---------------------------------
 def test_refusals():
     x, w = torch.randn(4, 32), torch.randn(8, 32)
@@ -456,3 +553,20 @@ def test_refuses_mixed_devices():
         fp8_dense(x.cuda(), w)
     with pytest.raises(ValueError, match="bias on"):
         fp8_dense(x.cuda(), w.cuda(), torch.zeros(8))
+
+
+@pytest.mark.gpu
+def test_refusals_on_a_gpu():
+    x, w = randn(20, 256).cuda(), randn(64, 256).cuda()
+    frozen = quantize_fp8_weight(w)
+    room = torch.zeros(64 * 256 + 1, dtype=torch.uint8, device="cuda")
+    odd = room[1:].view(64, 256)
+    with pytest.raises(RuntimeError, match="16 bytes"):
+        fp8_dense(x, fp8.Fp8Blocks(odd, frozen.scale, 256))
+    with pytest.raises(RuntimeError, match="does not match"):
+        fp8_dense(x, fp8.Fp8Blocks(frozen.data, frozen.scale[:1], 256))
+    with pytest.raises(RuntimeError, match="bytes and scales"):
+        fp8_dense(x, fp8.Fp8Blocks(frozen.data.float(), frozen.scale, 256))
+    many = torch.zeros(1, 256, device="cuda").expand(1 << 24, -1)
+    with pytest.raises(RuntimeError, match="too many rows"):
+        fp8_dense(many, w.requires_grad_(True))
