@@ -125,15 +125,29 @@ class FusedDense(nn.Module):
 
     def freeze(self) -> "FusedDense":
         """Lay the 8-bit weight out once, for serving. The layer then has no
-        gradients, and refuses to run once its weight has changed; train(),
-        a move to another device or type and set_precision() undo it."""
+        gradients, and refuses to run once its weight has been replaced or
+        changed in place (writes through ``.data``, which torch does not
+        count, are not seen: freeze again). train(), a move to another device
+        or type and set_precision() undo it, and copies of the layer are not
+        frozen."""
         if self.precision != "fp8":
             raise RuntimeError("only fp8 layers can be frozen")
         from elasticdl_amd.ops.fp8 import quantize_fp8_weight
 
         self._frozen = (quantize_fp8_weight(self.weight[:, :self.in_features]),
-                        self.weight._version)
+                        self.weight, self._weight_version())
         return self
+
+    def _weight_version(self):
+        # inference tensors have none, and cannot be changed in place
+        # outside of inference_mode
+        w = self.weight
+        return None if w.is_inference() else w._version
+
+    def __getstate__(self):
+        state = self.__dict__.copy()
+        state["_frozen"] = None
+        return state
 
     def train(self, mode: bool = True):
         if mode:
@@ -149,8 +163,9 @@ class FusedDense(nn.Module):
             from elasticdl_amd.ops.fp8 import fp8_dense
 
             if self._frozen is not None:
-                weight, version = self._frozen
-                if version != self.weight._version:
+                weight, source, version = self._frozen
+                if (source is not self.weight
+                        or version != self._weight_version()):
                     raise RuntimeError(
                         "the weight has changed since freeze()")
             else:

@@ -304,6 +304,8 @@ class SparseEmbedding(nn.Module):
     of ops/embedding.py, straight from the padded ids. ``scale`` multiplies
     the result; ``weights`` [batch, max_len] each id's row."""
 
+    scale = 1.0
+
     def __init__(self, input_dim: int, output_dim: int, combiner: str = "sum",
                  scale: float = 1.0):
         super().__init__()

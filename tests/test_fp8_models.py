@@ -6,6 +6,9 @@ Tolerances are those of test_fp8_dense.py and test_embedding_ops.py, applied
 to each operator on what it was given.
 """
 
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -69,6 +72,30 @@ def test_freeze(device):
         fd.set_precision("bf16").freeze()
     with pytest.raises(ValueError, match="unknown precision"):
         FusedDense(4, 4, precision="fp4")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_frozen_layers_that_are_copied_or_given_another_weight(device):
+    fd = layer(64, 32, device).eval().freeze()
+    x = torch.randn(5, 64, device=device)
+    with torch.no_grad():
+        want = fd(x)
+        for other in (copy.deepcopy(fd), pickle.loads(pickle.dumps(fd))):
+            other.weight.mul_(2.0)
+            assert torch.equal(other(x),
+                               fp8_dense(x, other.weight, fd.bias, "relu"))
+        assert torch.equal(fd(x), want)
+        new = {k: v.clone() for k, v in fd.state_dict().items()}
+        fd.load_state_dict(new, assign=True)
+        with pytest.raises(RuntimeError, match="changed"):
+            fd(x)
+        assert torch.equal(fd.freeze()(x), want)
+        fd.load_state_dict(new)
+        with pytest.raises(RuntimeError, match="changed"):
+            fd(x)
+    with torch.inference_mode():
+        made = layer(64, 32, device).eval().freeze()
+        assert torch.equal(made(x), want)
 
 
 def test_set_dense_precision_leaves_the_head():
