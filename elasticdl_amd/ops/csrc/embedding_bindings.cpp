@@ -20,11 +20,13 @@ int edl_lookup(const edl_bag*, hipStream_t);
 int edl_lookup_weight_grad(const edl_bag*, hipStream_t);
 int edl_segment_sums(const edl_segments*, hipStream_t);
 int edl_sort_rows(const void*, int, int64_t, int64_t, uint32_t* const*,
-                  uint32_t* const*, uint32_t*, uint32_t*, hipStream_t);
+                  uint32_t* const*, uint32_t*, uint32_t*, void*, int64_t,
+                  hipStream_t);
 int edl_segment_chunk(int64_t, int, int);
 int64_t edl_sort_counts(int64_t);
 int edl_sort_rows_small(const void*, int, int64_t, int64_t, uint32_t*,
-                        uint32_t*, uint32_t*, uint32_t*, hipStream_t);
+                        uint32_t*, uint32_t*, uint32_t*, void*, int64_t,
+                        hipStream_t);
 int edl_sort_ids_small(const int64_t*, int64_t, uint32_t*, uint32_t*,
                        uint32_t*, int64_t*, uint32_t*, hipStream_t);
 int edl_ids_range(const int64_t*, int64_t, int64_t*, hipStream_t);
@@ -174,8 +176,6 @@ void segments_into(edl_segments& s, Pieces& pieces) {
   pieces.add(&s.part, chunks * 2 * s.D);
   pieces.add(&s.head, chunks);
   pieces.add(&s.tail, chunks);
-  pieces.add(&s.list, chunks);
-  pieces.add(&s.listed, 1);
 }
 
 struct SortSpace {
@@ -297,9 +297,13 @@ class Lookup : public torch::autograd::Function<Lookup> {
       out[1] = dw.to(weights.scalar_type());
     }
     if (!need_t) return;
-    Tensor dt = torch::zeros({rows, d}, opts);
+    if (n == 0) {
+      out[0] = torch::zeros({rows, d}, opts);
+      return;
+    }
+    Tensor dt = torch::empty({rows, d}, opts);  // the sort fills it with zeros
+    const int64_t bytes = dt.numel() * dt.element_size();
     out[0] = dt;
-    if (n == 0) return;
     edl_segments s = {};
     s.N = n;
     s.limit = (uint32_t)rows;
@@ -319,7 +323,7 @@ class Lookup : public torch::autograd::Function<Lookup> {
       const Tensor space = pieces.place(ids);
       launched(edl_sort_rows_small(a.ids, a.ids64, rows, n, small.pos,
                                    small.starts, small.runs, small.rows,
-                                   stream_of(ids)),
+                                   dt.data_ptr(), bytes, stream_of(ids)),
                "sort of ids");
       small.into(s);
       launched(edl_segment_sums(&s, stream_of(ids)), "embedding gradient");
@@ -330,7 +334,7 @@ class Lookup : public torch::autograd::Function<Lookup> {
     const Tensor space = pieces.place(ids);
     const int at =
         edl_sort_rows(a.ids, a.ids64, rows, n, sort.k, sort.p, sort.count,
-                      sort.total, stream_of(ids));
+                      sort.total, dt.data_ptr(), bytes, stream_of(ids));
     launched(at < 0 ? -1 - at : 0, "sort of ids");
     s.keys = sort.k[at];
     s.pos = sort.p[at];

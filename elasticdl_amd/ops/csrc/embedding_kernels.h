@@ -49,7 +49,6 @@ struct edl_segments {
   // else a workspace: a row of sums for each chunk's open beginning and end
   float* part;                // [chunks, 2, D]
   uint32_t *head, *tail;      // [chunks]: their keys
-  uint32_t *list, *listed;    // long runs, and how many
 };
 
 #define EDL_RANGE_PARTS 256

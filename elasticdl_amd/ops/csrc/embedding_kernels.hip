@@ -15,6 +15,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "embedding_kernels.h"
@@ -255,12 +256,35 @@ __device__ inline uint32_t rank_digit(volatile C* count, uint32_t d, bool in) {
   return old + lower;
 }
 
+// Zeros, by workgroups beside those of a sort, whose waits they fill, and past
+// L2, which the sort uses: a whole gradient of 128 MB 157 us, 163 with a launch
+// of its own for them.
+struct Zeros {
+  uint8_t* to;  // on a border of 16 bytes
+  int64_t bytes;
+};
+constexpr int kZeroBlocks = 1024;
+template <int THREADS>
+__device__ inline void fill_zeros(const Zeros& z, int64_t block,
+                                  int64_t blocks) {
+  typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+  const int64_t n = z.bytes / 16, step = blocks * THREADS;
+  const u32x4 none = {0, 0, 0, 0};
+  for (int64_t i = block * THREADS + threadIdx.x; i < n; i += step)
+    __builtin_nontemporal_store(none, reinterpret_cast<u32x4*>(z.to) + i);
+  if (block == 0 && threadIdx.x < z.bytes % 16)
+    z.to[n * 16 + threadIdx.x] = 0;
+}
+
 template <typename S, typename P>
 __global__ __launch_bounds__(256) void sort_count_kernel(S src, int64_t N,
                                                          int shift, int bits,
                                                          int tiles,
-                                                         uint32_t* counts) {
+                                                         uint32_t* counts,
+                                                         Zeros zeros) {
   constexpr int ITEMS = P::ITEMS;
+  if ((int)blockIdx.x >= tiles)
+    return fill_zeros<256>(zeros, blockIdx.x - tiles, gridDim.x - tiles);
   __shared__ uint32_t h[1 << P::BITS];
   const int bins = 1 << bits;
   for (int d = threadIdx.x; d < bins; d += 256) h[d] = 0;
@@ -423,7 +447,8 @@ constexpr int kSmallWaves = kSmallThreads / 64;
 template <typename S, bool IDS>
 __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
     S src, int N, int bits_all, uint32_t* pos_out, uint32_t* starts,
-    uint32_t* runs, uint32_t* rows, int64_t* unique, uint32_t* found) {
+    uint32_t* runs, uint32_t* rows, int64_t* unique, uint32_t* found,
+    Zeros zeros) {
   __shared__ uint32_t s_key[EDL_SORT_SMALL];
   __shared__ uint16_t s_pos[EDL_SORT_SMALL];
   __shared__ __align__(16) uint16_t cnt[kSmallWaves][256];
@@ -432,6 +457,8 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
   __shared__ int64_t s_min[kSmallWaves], s_max[kSmallWaves];
   __shared__ uint32_t s4[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (blockIdx.x > 0)
+    return fill_zeros<kSmallThreads>(zeros, blockIdx.x - 1, gridDim.x - 1);
   const int items = (N + kSmallThreads - 1) / kSmallThreads;
   const int i0 = wave * items * 64 + lane;
   uint32_t key[kSmallItems], pos[kSmallItems];
@@ -708,9 +735,9 @@ __global__ __launch_bounds__(256) void unique_place_kernel(
 // of equal keys are, so that a frequent id costs no more than rare ones. A
 // group of lanes adds its chunk's rows in order, 8 in flight; a run that
 // begins and ends in the chunk is written at once. One that goes on past an
-// end of the chunk leaves its sum in the workspace, and the chunk in which
-// it begins collects the sums of those behind: short runs by a group, long
-// ones (over kShort chunks) by a whole workgroup each.
+// end of the chunk leaves its sum in the workspace, and where it begins the
+// join collects the sums of those behind: short runs by a group of lanes of
+// a workgroup's first wave, long ones (over kShort chunks) by all of it.
 constexpr int kShort = 8;
 
 template <typename T, int VEC>
@@ -805,7 +832,6 @@ __global__ __launch_bounds__(256) void segment_kernel(edl_segments a,
   if (col == 0) {
     a.head[c] = head;
     a.tail[c] = tail;
-    if (c == 0) *a.listed = 0;
   }
 }
 
@@ -867,70 +893,77 @@ __global__ __launch_bounds__(256) void segment_run_kernel(edl_segments a,
       o.v;
 }
 
-template <typename T, int VEC>
-__global__ __launch_bounds__(256) void segment_short_kernel(edl_segments a,
-                                                            int64_t chunks,
-                                                            int64_t block0) {
-  typedef Vec<T, VEC> V;
-  const int lanes = lanes_of(a.D, VEC), pieces = pieces_of(a.D, VEC);
-  const int64_t unit = ((block0 + blockIdx.x) * 256 + threadIdx.x) / lanes;
-  const int64_t c = unit / pieces;
-  const int col =
-      ((int)(unit % pieces) * lanes + (threadIdx.x & (lanes - 1))) * VEC;
-  if (c >= chunks) return;
-  const uint32_t key = a.tail[c];
-  if (key == kNone) return;
-  int n = 0;  // chunks behind that the run goes on into
-  while (n <= kShort && c + 1 + n < chunks && a.head[c + 1 + n] == key) ++n;
-  if (n > kShort) {
-    if (col == 0) a.list[atomicAdd(a.listed, 1u)] = (uint32_t)c;
-    return;
+// how many of the chunks from `in` on begin with this key: they lie together.
+// The workgroup looks at 256 places at a time, 80 thousand chunks in 3 rounds
+__device__ inline int64_t end_of(const uint32_t* head, uint32_t key,
+                                 int64_t in, int64_t out) {
+  while (in < out) {
+    const int64_t step = (out - in + 255) / 256;
+    const int64_t at = in + threadIdx.x * step;
+    const int k = __syncthreads_count(at < out && head[at] == key);
+    if (k == 0) return in;
+    out = in + k * step < out ? in + k * step : out;
+    in += (k - 1) * step + 1;
   }
-  if (col >= a.D) return;
-  const float* p = a.part + (c * 2 + 1) * a.D + col;
-  float acc[VEC];
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) acc[k] = p[k];
-  for (int q = 0; q < n; ++q) {
-    const float* h = a.part + (c + 1 + q) * 2 * a.D + col;
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) acc[k] += h[k];
-  }
-  V o;
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) o.set(k, acc[k]);
-  *reinterpret_cast<decltype(o.v)*>(static_cast<T*>(a.out) +
-                                    (int64_t)key * a.D + col) = o.v;
+  return in;
 }
 
 template <typename T, int VEC>
-__global__ __launch_bounds__(256) void segment_long_kernel(edl_segments a,
-                                                           int64_t chunks) {
+__global__ __launch_bounds__(256) void segment_join_kernel(edl_segments a,
+                                                           int64_t chunks,
+                                                           int64_t block0) {
   typedef Vec<T, VEC> V;
   constexpr int U = 4;
   __shared__ float s[256 * VEC];
+  __shared__ int64_t s_long[64 / kShort + 1];
+  __shared__ uint32_t s_longs;
+  const int tid = threadIdx.x;
   const int lanes = lanes_of(a.D, VEC), pieces = pieces_of(a.D, VEC);
-  const int groups = 256 / lanes, g = threadIdx.x / lanes;
-  const uint32_t n = *a.listed;
-  for (uint32_t at = blockIdx.x; at < n * pieces; at += gridDim.x) {
-    const int64_t c = a.list[at / pieces];
-    const uint32_t key = a.tail[c];
-    const int col =
-        ((int)(at % pieces) * lanes + (threadIdx.x & (lanes - 1))) * VEC;
-    // the chunks behind that begin with this key: up to the first that does
-    // not, and they lie together
-    int64_t in = c + 1, out = chunks;
-    while (in < out) {
-      const int64_t mid = (in + out) / 2;
-      if (a.head[mid] == key)
-        in = mid + 1;
-      else
-        out = mid;
+  const int l_lane = tid & (lanes - 1);
+  const int64_t unit = ((block0 + blockIdx.x) * 64 + tid) / lanes;
+  if (tid == 0) s_longs = 0;
+  __syncthreads();
+  const int64_t c0 = unit / pieces;
+  const uint32_t key0 = tid < 64 && c0 < chunks ? a.tail[c0] : kNone;
+  if (key0 != kNone) {
+    const int col = ((int)(unit % pieces) * lanes + l_lane) * VEC;
+    int n = 0;  // chunks behind that the run goes on into, up to kShort + 1
+    bool on = true;
+#pragma unroll
+    for (int q = 0; q <= kShort; ++q) {
+      const int64_t at = c0 + 1 + q < chunks ? c0 + 1 + q : c0;
+      on &= a.head[at] == key0 && c0 + 1 + q < chunks;
+      n += on;
     }
+    if (n > kShort) {
+      if (l_lane == 0) s_long[atomicAdd(&s_longs, 1u)] = unit;
+    } else if (col < a.D) {
+      const float* p = a.part + (c0 * 2 + 1) * a.D + col;
+      float acc[VEC];
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] = p[k];
+      for (int q = 0; q < n; ++q) {
+        const float* h = a.part + (c0 + 1 + q) * 2 * a.D + col;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] += h[k];
+      }
+      V o;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) o.set(k, acc[k]);
+      *reinterpret_cast<decltype(o.v)*>(static_cast<T*>(a.out) +
+                                        (int64_t)key0 * a.D + col) = o.v;
+    }
+  }
+  __syncthreads();
+  const int groups = 256 / lanes, g = tid / lanes;
+  for (uint32_t at = 0; at < s_longs; ++at) {  // the workgroup together
+    const int64_t c = s_long[at] / pieces;
+    const int col = ((int)(s_long[at] % pieces) * lanes + l_lane) * VEC;
+    const uint32_t key = a.tail[c];
+    const int64_t end = end_of(a.head, key, c + 1, chunks);
     float acc[VEC];
 #pragma unroll
     for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
-    const int64_t end = in;
     if (col < a.D) {
       for (int64_t q = c + 1 + g; q < end; q += (int64_t)groups * U) {
         float v[U][VEC];
@@ -948,13 +981,13 @@ __global__ __launch_bounds__(256) void segment_long_kernel(edl_segments a,
       }
     }
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) s[threadIdx.x * VEC + k] = acc[k];
+    for (int k = 0; k < VEC; ++k) s[tid * VEC + k] = acc[k];
     __syncthreads();
     for (int h = groups / 2; h > 0; h >>= 1) {
       if (g < h) {
 #pragma unroll
         for (int k = 0; k < VEC; ++k)
-          s[threadIdx.x * VEC + k] += s[(threadIdx.x + h * lanes) * VEC + k];
+          s[tid * VEC + k] += s[(tid + h * lanes) * VEC + k];
       }
       __syncthreads();
     }
@@ -962,8 +995,7 @@ __global__ __launch_bounds__(256) void segment_long_kernel(edl_segments a,
       const float* p = a.part + (c * 2 + 1) * a.D + col;
       V o;
 #pragma unroll
-      for (int k = 0; k < VEC; ++k)
-        o.set(k, s[threadIdx.x * VEC + k] + p[k]);
+      for (int k = 0; k < VEC; ++k) o.set(k, s[tid * VEC + k] + p[k]);
       *reinterpret_cast<decltype(o.v)*>(static_cast<T*>(a.out) +
                                         (int64_t)key * a.D + col) = o.v;
     }
@@ -1016,11 +1048,9 @@ void launch_segments(const edl_segments& a, hipStream_t st) {
     segment_kernel<T, VEC><<<n, 256, 0, st>>>(a, b0);
   });
   if (chunks == 1) return;
-  in_blocks(threads, [&](unsigned n, int64_t b0) {
-    segment_short_kernel<T, VEC><<<n, 256, 0, st>>>(a, chunks, b0);
+  in_blocks(threads * 4, [&](unsigned n, int64_t b0) {
+    segment_join_kernel<T, VEC><<<n, 256, 0, st>>>(a, chunks, b0);
   });
-  if (chunks <= kShort + 1) return;
-  segment_long_kernel<T, VEC><<<256, 256, 0, st>>>(a, chunks);
 }
 
 #define EDL_BY_TYPE(FN, A, ST)                       \
@@ -1056,12 +1086,12 @@ int sort_plan(int64_t N) {
 template <typename S, bool FIRST, typename P>
 int sort_pass(S src, const uint32_t* pos_in, int64_t N, int shift, int bits,
               uint32_t* counts, uint32_t* totals, typename S::K* keys_out,
-              uint32_t* pos_out, hipStream_t st) {
+              uint32_t* pos_out, hipStream_t st, Zeros zeros = {}) {
   constexpr int kTile = P::ITEMS * 256;
   const int tiles = (int)((N + kTile - 1) / kTile);
-  const int bins = 1 << bits;
-  sort_count_kernel<S, P>
-      <<<tiles, 256, 0, st>>>(src, N, shift, bits, tiles, counts);
+  const int bins = 1 << bits, fill = zeros.bytes ? kZeroBlocks : 0;
+  sort_count_kernel<S, P><<<tiles + fill, 256, 0, st>>>(src, N, shift, bits,
+                                                        tiles, counts, zeros);
   sort_offsets_kernel<<<bins, 256, 0, st>>>(counts, tiles, totals);
   sort_move_kernel<S, FIRST, P><<<tiles, 256, 0, st>>>(
       src, pos_in, N, shift, bits, tiles, counts, totals, keys_out, pos_out);
@@ -1090,11 +1120,11 @@ int sort_rest(int at, int done, int bits, int64_t N, K* const* keys,
 template <typename S, typename P>
 int sort_by(S src, int64_t N, int bits, typename S::K* const* keys,
             uint32_t* const* pos, uint32_t* counts, uint32_t* totals,
-            hipStream_t st) {
+            hipStream_t st, Zeros zeros) {
   const int passes = (bits + P::BITS - 1) / P::BITS;
   const int b = (bits + passes - 1) / passes;
   const int rc = sort_pass<S, true, P>(src, nullptr, N, 0, b, counts, totals,
-                                       keys[0], pos[0], st);
+                                       keys[0], pos[0], st, zeros);
   if (rc) return -1 - rc;
   return sort_rest<typename S::K, P>(0, b, bits, N, keys, pos, counts, totals,
                                      st);
@@ -1102,9 +1132,9 @@ int sort_by(S src, int64_t N, int bits, typename S::K* const* keys,
 template <typename S>
 int sort_all(S src, int64_t N, int bits, typename S::K* const* keys,
              uint32_t* const* pos, uint32_t* counts, uint32_t* totals,
-             hipStream_t st) {
+             hipStream_t st, Zeros zeros = {}) {
 #define EDL_SORT_BY(P) \
-  sort_by<S, P>(src, N, bits, keys, pos, counts, totals, st)
+  sort_by<S, P>(src, N, bits, keys, pos, counts, totals, st, zeros)
   return EDL_BY_PLAN(N, EDL_SORT_BY);
 #undef EDL_SORT_BY
 }
@@ -1138,16 +1168,18 @@ extern "C" int edl_segment_sums(const edl_segments* a, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
-// Sorts the ids of a table of V rows, those without a row behind the rest.
-// Returns which of the two buffers holds the result, or -1 - error.
+// Sorts the ids of a table of V rows, those without a row behind the rest,
+// and fills `zeros` with them. Returns which of the two buffers holds the
+// result, or -1 - error.
 extern "C" int edl_sort_rows(const void* ids, int ids64, int64_t V, int64_t N,
                              uint32_t* const* keys, uint32_t* const* pos,
-                             uint32_t* counts, uint32_t* totals,
-                             hipStream_t st) {
+                             uint32_t* counts, uint32_t* totals, void* zeros,
+                             int64_t zero_bytes, hipStream_t st) {
   int bits = 1;
   while (bits < 32 && (V >> bits) != 0) ++bits;
   Keys32 src{ids, ids64 != 0, V};
-  return sort_all(src, N, bits, keys, pos, counts, totals, st);
+  return sort_all(src, N, bits, keys, pos, counts, totals, st,
+                  Zeros{static_cast<uint8_t*>(zeros), zero_bytes});
 }
 
 // chunks for the segment kernels: as long as they leave 16 waves for each of
@@ -1171,12 +1203,16 @@ extern "C" int64_t edl_sort_counts(int64_t N) {
 extern "C" int edl_sort_rows_small(const void* ids, int ids64, int64_t V,
                                    int64_t N, uint32_t* pos, uint32_t* starts,
                                    uint32_t* runs, uint32_t* rows,
+                                   void* zeros, int64_t zero_bytes,
                                    hipStream_t st) {
   int bits = 1;
   while (bits < 32 && (V >> bits) != 0) ++bits;
-  sort_small_kernel<Keys32, false><<<1, kSmallThreads, 0, st>>>(
+  const int64_t fill = std::min<int64_t>(
+      (zero_bytes + kSmallThreads * 16 - 1) / (kSmallThreads * 16),
+      kZeroBlocks * 256 / kSmallThreads);
+  sort_small_kernel<Keys32, false><<<1 + (int)fill, kSmallThreads, 0, st>>>(
       Keys32{ids, ids64 != 0, V}, (int)N, bits, pos, starts, runs, rows,
-      nullptr, nullptr);
+      nullptr, nullptr, Zeros{static_cast<uint8_t*>(zeros), zero_bytes});
   return (int)hipGetLastError();
 }
 extern "C" int edl_sort_ids_small(const int64_t* ids, int64_t N, uint32_t* pos,
@@ -1184,7 +1220,8 @@ extern "C" int edl_sort_ids_small(const int64_t* ids, int64_t N, uint32_t* pos,
                                   int64_t* unique, uint32_t* found,
                                   hipStream_t st) {
   sort_small_kernel<Keys32Of, true><<<1, kSmallThreads, 0, st>>>(
-      Keys32Of{ids}, (int)N, 0, pos, starts, runs, nullptr, unique, found);
+      Keys32Of{ids}, (int)N, 0, pos, starts, runs, nullptr, unique, found,
+      Zeros{});
   return (int)hipGetLastError();
 }
 
