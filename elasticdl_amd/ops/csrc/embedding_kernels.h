@@ -32,9 +32,11 @@ struct edl_bag {
 };
 
 struct edl_segments {
-  const uint32_t *keys, *pos;  // [N], sorted by key, then by pos
+  // [N], sorted by key, then by pos; on borders of 16 bytes, with room to
+  // read up to a multiple of 8
+  const uint32_t *keys, *pos;
   int64_t N;
-  int chunk;       // tokens that a group of lanes takes
+  int chunk;       // tokens that a group of lanes takes: a multiple of 8
   uint32_t limit;  // keys from here on are no rows
   const void* src;  // [*, D] contiguous: row pos / L
   int D, type, vec, L;

@@ -20,6 +20,8 @@
 
 #include "embedding_kernels.h"
 
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+
 namespace {
 
 constexpr uint32_t kNone = 0xffffffffu;
@@ -267,13 +269,22 @@ constexpr int kZeroBlocks = 1024;
 template <int THREADS>
 __device__ inline void fill_zeros(const Zeros& z, int64_t block,
                                   int64_t blocks) {
-  typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
   const int64_t n = z.bytes / 16, step = blocks * THREADS;
   const u32x4 none = {0, 0, 0, 0};
   for (int64_t i = block * THREADS + threadIdx.x; i < n; i += step)
     __builtin_nontemporal_store(none, reinterpret_cast<u32x4*>(z.to) + i);
   if (block == 0 && threadIdx.x < z.bytes % 16)
     z.to[n * 16 + threadIdx.x] = 0;
+}
+
+// Workgroups go to the 8 XCDs in turn; this gives each XCD a run of
+// neighbouring tiles. A digit's items from them, and their counts, lie
+// together where they go, so that its L2 writes whole lines (a pass over 2.6
+// million items 35 us otherwise, 28 so).
+__device__ inline int xcd_order(int bid, int n) {
+  if (n < 8) return bid;
+  const int xcd = bid & 7, idx = bid >> 3, q = n >> 3, r = n & 7;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
 }
 
 template <typename S, typename P>
@@ -289,7 +300,8 @@ __global__ __launch_bounds__(256) void sort_count_kernel(S src, int64_t N,
   const int bins = 1 << bits;
   for (int d = threadIdx.x; d < bins; d += 256) h[d] = 0;
   __syncthreads();
-  const int64_t base = (int64_t)blockIdx.x * (ITEMS * 256);
+  const int tile = xcd_order(blockIdx.x, tiles);
+  const int64_t base = (int64_t)tile * (ITEMS * 256);
 #pragma unroll
   for (int k = 0; k < ITEMS; ++k) {
     const int64_t i = base + k * 256 + threadIdx.x;
@@ -297,7 +309,7 @@ __global__ __launch_bounds__(256) void sort_count_kernel(S src, int64_t N,
   }
   __syncthreads();
   for (int d = threadIdx.x; d < bins; d += 256)
-    counts[(int64_t)d * tiles + blockIdx.x] = h[d];
+    counts[(int64_t)d * tiles + tile] = h[d];
 }
 
 // exclusive sum over the 256 threads, and the total
@@ -357,7 +369,8 @@ __global__ __launch_bounds__(256) void sort_move_kernel(
   __shared__ uint32_t s4[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int bins = 1 << bits;
-  const int64_t base = (int64_t)blockIdx.x * kTile;
+  const int tile = xcd_order(blockIdx.x, tiles);
+  const int64_t base = (int64_t)tile * kTile;
   const int64_t first = base + wave * (kTile / 4) + lane;
   K key[ITEMS];
   uint32_t pos[ITEMS], rank[ITEMS];
@@ -373,7 +386,7 @@ __global__ __launch_bounds__(256) void sort_move_kernel(
   for (int q = 0; q < kOwn; ++q) {
     const int d = tid * kOwn + q;
     tot[q] = d < bins ? totals[d] : 0;
-    at_tile[q] = d < bins ? counts[(int64_t)d * tiles + blockIdx.x] : 0;
+    at_tile[q] = d < bins ? counts[(int64_t)d * tiles + tile] : 0;
   }
   for (int d = tid; d < 2 * kBins; d += 256)
     reinterpret_cast<uint32_t*>(&cnt[0][0])[d] = 0;
@@ -779,14 +792,24 @@ __global__ __launch_bounds__(256) void segment_kernel(edl_segments a,
   };
 
   for (int64_t t = t0; t < t1; t += U) {
-    uint32_t key[U], row[U];
+    uint32_t key[U], pos[U], row[U];
     float w[U];
     V v[U];
+    // eight at once: t is a multiple of 8, and the arrays' pieces end on
+    // borders of 256 bytes
+#pragma unroll
+    for (int u = 0; u < U; u += 4) {
+      const u32x4 k = *reinterpret_cast<const u32x4*>(a.keys + t + u);
+      const u32x4 p = *reinterpret_cast<const u32x4*>(a.pos + t + u);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        key[u + q] = k[q];
+        pos[u + q] = p[q];
+      }
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t i = t + u < t1 ? t + u : t1 - 1;
-      key[u] = a.keys[i];
-      const uint32_t p = a.pos[i];
+      const uint32_t p = t + u < t1 ? pos[u] : pos[0];
       row[u] = a.L > 1 ? p / (uint32_t)a.L : p;
       w[u] = a.weights ? load_any(a.weights, p, a.w_type) : 1.f;
     }
