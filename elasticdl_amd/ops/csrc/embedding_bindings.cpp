@@ -25,10 +25,11 @@ int edl_sort_rows(const void*, int, int64_t, int64_t, uint32_t* const*,
 int edl_segment_chunk(int64_t, int, int);
 int64_t edl_sort_counts(int64_t);
 int edl_sort_rows_small(const void*, int, int64_t, int64_t, uint32_t*,
-                        uint32_t*, uint32_t*, uint32_t*, void*, int64_t,
-                        hipStream_t);
-int edl_sort_ids_small(const int64_t*, int64_t, uint32_t*, uint32_t*,
-                       uint32_t*, int64_t*, uint32_t*, hipStream_t);
+                        uint32_t*, uint32_t*, uint32_t*, uint32_t*, void*,
+                        int64_t, hipStream_t);
+int edl_sort_ids_small(const int64_t*, int64_t, uint32_t*, uint32_t*, int64_t*,
+                       uint32_t*, uint32_t*, int64_t*, uint32_t*,
+                       hipStream_t);
 int edl_ids_range(const int64_t*, int64_t, int64_t*, hipStream_t);
 int edl_sort_ids32_first(const int64_t*, int, int64_t, uint32_t* const*,
                          uint32_t* const*, uint32_t*, uint32_t*, hipStream_t);
@@ -190,13 +191,16 @@ struct SortSpace {
   }
 };
 
-struct SmallSpace {  // of a one-workgroup sort
-  uint32_t *pos = nullptr, *starts = nullptr, *runs = nullptr,
-           *rows = nullptr;
+struct SmallSpace {  // of a small sort
+  uint32_t *keys = nullptr, *pos = nullptr, *starts = nullptr,
+           *runs = nullptr, *rows = nullptr;
+  int64_t* info = nullptr;
   SmallSpace(Pieces& pieces, int64_t n, bool with_rows) {
+    pieces.add(&keys, n);
     pieces.add(&pos, n);
     pieces.add(&starts, n);
     pieces.add(&runs, 1);
+    pieces.add(&info, 2);
     if (with_rows) pieces.add(&rows, n);
   }
   void into(edl_segments& s) const {
@@ -321,8 +325,8 @@ class Lookup : public torch::autograd::Function<Lookup> {
     if (n <= EDL_SORT_SMALL) {
       SmallSpace small(pieces, n, true);
       const Tensor space = pieces.place(ids);
-      launched(edl_sort_rows_small(a.ids, a.ids64, rows, n, small.pos,
-                                   small.starts, small.runs, small.rows,
+      launched(edl_sort_rows_small(a.ids, a.ids64, rows, n, small.keys,
+                                   small.pos, small.starts, small.runs, small.rows,
                                    dt.data_ptr(), bytes, stream_of(ids)),
                "sort of ids");
       small.into(s);
@@ -406,7 +410,7 @@ std::vector<Tensor> coalesce_rows(Tensor values, Tensor ids) {
   int64_t* ids_out = unique.data_ptr<int64_t>();
   const int64_t* id = ids.data_ptr<int64_t>();
   // what the host reads, in memory that the kernels write to directly: how
-  // many ids, whether they lie too far apart for the one-workgroup sort, and
+  // many ids, whether they lie too far apart for the small sort, and
   // their smallest and largest by parts
   const Tensor host =
       torch::empty({1 + 2 * EDL_RANGE_PARTS},
@@ -453,8 +457,9 @@ std::vector<Tensor> coalesce_rows(Tensor values, Tensor ids) {
     Pieces pieces;
     SmallSpace small(pieces, n, false);
     const Tensor space = pieces.place(ids);
-    launched(edl_sort_ids_small(id, n, small.pos, small.starts, small.runs,
-                                ids_out, found_at, st),
+    launched(edl_sort_ids_small(id, n, small.keys, small.pos, small.info,
+                                small.starts, small.runs, ids_out, found_at,
+                                st),
              "sort of ids");
     mark();
     small.into(s);

@@ -45,7 +45,7 @@ struct edl_segments {
   const void* weights;  // by pos, or null
   int w_type;
   void* out;  // [limit, D] of src's type: row keys[i]
-  // where one workgroup sorted: each run's first token, how many runs there
+  // where the small sort was: each run's first token, how many runs there
   // are, and their rows (null: the run's own number); keys is not used
   const uint32_t *starts, *runs, *rows;
   // else a workspace: a row of sums for each chunk's open beginning and end

@@ -451,177 +451,138 @@ __global__ __launch_bounds__(256) void sort_move_kernel(
   }
 }
 
-// Up to EDL_SORT_SMALL items in one workgroup, all passes in LDS: one launch
-// in the place of three a pass. A wave takes a run of 64 * items of them. Out
-// come the items in order, where each run of equal keys starts, and how many
-// runs there are (runs[0]).
+// Up to EDL_SORT_SMALL items: an item's place is how many come before it, by
+// key and then by position, and it is counted. That is N^2 comparisons, but
+// two instructions each and all of the chip's at once, where a sort in one
+// workgroup waits for itself (6656 ids of 21 bits: 24 us in passes of 8 bits,
+// 12 us counted and 4 for the runs). A workgroup has 32 items, and two lanes
+// of each wave for each share those that they are compared with.
 //
-// IDS: ids of any value, taken relative to the smallest; the runs' ids go to
-// `unique`, and for the host how many there are (found[0]), or in found[1]
-// that they lie too far apart for 32 bits, and no runs. Else rows of a table:
-// the runs' go to `rows`.
+// IDS: ids of any value, less 2^31 below the first, which goes to info[0];
+// info[1]: some lie too far from it for 32 bits, and nothing is done.
+// Else rows of a table.
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallItems = EDL_SORT_SMALL / kSmallThreads;
 constexpr int kSmallWaves = kSmallThreads / 64;
+constexpr int kSmallTile = 32, kSmallShares = kSmallThreads / kSmallTile;
 
 template <typename S, bool IDS>
-__global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
-    S src, int N, int bits_all, uint32_t* pos_out, uint32_t* starts,
-    uint32_t* runs, uint32_t* rows, int64_t* unique, uint32_t* found,
-    Zeros zeros) {
-  __shared__ uint32_t s_key[EDL_SORT_SMALL];
-  __shared__ uint16_t s_pos[EDL_SORT_SMALL];
-  __shared__ __align__(16) uint16_t cnt[kSmallWaves][256];
-  __shared__ uint16_t quarters[4][256];
-  __shared__ uint32_t local[256];
-  __shared__ int64_t s_min[kSmallWaves], s_max[kSmallWaves];
-  __shared__ uint32_t s4[4];
+__global__ __launch_bounds__(kSmallThreads) void rank_small_kernel(
+    S src, int N, uint32_t* keys_out, uint32_t* pos_out, int64_t* info,
+    int tiles, Zeros zeros) {
+  __shared__ __align__(16) uint32_t s_key[EDL_SORT_SMALL];
+  __shared__ uint32_t s_rank[kSmallShares][kSmallTile];
+  if ((int)blockIdx.x >= tiles)
+    return fill_zeros<kSmallThreads>(zeros, blockIdx.x - tiles,
+                                     gridDim.x - tiles);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (blockIdx.x > 0)
-    return fill_zeros<kSmallThreads>(zeros, blockIdx.x - 1, gridDim.x - 1);
-  const int items = (N + kSmallThreads - 1) / kSmallThreads;
-  const int i0 = wave * items * 64 + lane;
-  uint32_t key[kSmallItems], pos[kSmallItems];
-  int bits = bits_all;
-  int64_t low = 0;
+  const int all = (N + 4 * kSmallShares - 1) / (4 * kSmallShares) *
+                  (4 * kSmallShares);
   if constexpr (IDS) {
-    int64_t mn = INT64_MAX, mx = INT64_MIN;
-    int64_t v[kSmallItems];
+    const uint64_t low = (uint64_t)src.ids[0] - 0x80000000ull;
+    uint32_t off = 0;
 #pragma unroll
     for (int k = 0; k < kSmallItems; ++k) {
-      const int i = i0 + k * 64;
-      const bool in = k < items && i < N;
-      v[k] = in ? src.ids[i] : 0;
-      if (in) {
-        mn = v[k] < mn ? v[k] : mn;
-        mx = v[k] > mx ? v[k] : mx;
-      }
+      const int i = k * kSmallThreads + tid;
+      const uint64_t rel = (uint64_t)src.ids[i < N ? i : 0] - low;
+      off |= (uint32_t)(rel >> 32);
+      if (i < all) s_key[i] = i < N ? (uint32_t)rel : kNone;
     }
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t a = __shfl_xor((long long)mn, o);
-      const int64_t b = __shfl_xor((long long)mx, o);
-      mn = a < mn ? a : mn;
-      mx = b > mx ? b : mx;
+    const bool far = __syncthreads_or(off != 0);
+    if (blockIdx.x == 0 && tid == 0) {
+      info[0] = (int64_t)low;
+      info[1] = far;
     }
-    if (lane == 0) {
-      s_min[wave] = mn;
-      s_max[wave] = mx;
+    if (far) return;  // all alike
+  } else {
+#pragma unroll
+    for (int k = 0; k < kSmallItems; ++k) {
+      const int i = k * kSmallThreads + tid;
+      if (i < all) s_key[i] = i < N ? (uint32_t)src(i) : kNone;
     }
-    __syncthreads();
-    for (int w = 0; w < kSmallWaves; ++w) {
-      mn = s_min[w] < mn ? s_min[w] : mn;
-      mx = s_max[w] > mx ? s_max[w] : mx;
-    }
-    const uint64_t range = (uint64_t)mx - (uint64_t)mn;
-    const bool far = range >> 32 != 0;
+  }
+  __syncthreads();
+  const int item = tid & (kSmallTile - 1), which = tid / kSmallTile;
+  const int tile0 = (int)blockIdx.x * kSmallTile, tile1 = tile0 + kSmallTile;
+  const uint32_t key = s_key[tile0 + item];
+  const int share = all / kSmallShares, j0 = which * share, j1 = j0 + share;
+  uint32_t rank = 0;
+  const auto four = [&](int j) {
+    return *reinterpret_cast<const u32x4*>(s_key + j);
+  };
+#pragma unroll 4
+  for (int j = j0; j < min(j1, tile0); j += 4) {  // equal ones come before
+    const u32x4 o = four(j);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) rank += o[q] <= key;
+  }
+  for (int j = max(j0, tile0); j < min(j1, tile1); j += 4) {
+    const u32x4 o = four(j);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      rank += o[q] < key || (o[q] == key && j + q < tile0 + item);
+  }
+#pragma unroll 4
+  for (int j = max(j0, tile1); j < j1; j += 4) {  // and behind
+    const u32x4 o = four(j);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) rank += o[q] < key;
+  }
+  s_rank[which][item] = rank;
+  __syncthreads();
+  if (tid >= kSmallTile || tile0 + item >= N) return;
+  for (int w = 1; w < kSmallShares; ++w) rank += s_rank[w][item];
+  keys_out[rank] = key;
+  pos_out[rank] = tile0 + item;
+}
+
+// Where each run of the small sort's equal keys starts, and how many there
+// are (runs[0]). IDS: the runs' ids go to `unique`, and for the host how many
+// there are (found[0]), or that there is nothing (found[1], info[1]). Else
+// the runs' rows go to `rows`.
+template <bool IDS>
+__global__ __launch_bounds__(kSmallThreads) void runs_small_kernel(
+    const uint32_t* __restrict__ keys, int N, const int64_t* info,
+    uint32_t* starts, uint32_t* runs, uint32_t* rows, int64_t* unique,
+    uint32_t* found) {
+  __shared__ uint32_t s_count[kSmallWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if constexpr (IDS) {
+    const bool far = info[1] != 0;
     if (tid == 0) found[1] = far;
     if (far) {  // all threads alike
       if (tid == 0) runs[0] = 0;
       return;
     }
-    low = mn;
-    bits = range ? 64 - __clzll((long long)range) : 1;
-#pragma unroll
-    for (int k = 0; k < kSmallItems; ++k)
-      key[k] = (uint32_t)((uint64_t)v[k] - (uint64_t)mn);
-  } else {
-#pragma unroll
-    for (int k = 0; k < kSmallItems; ++k) {
-      const int i = i0 + k * 64;
-      key[k] = k < items && i < N ? (uint32_t)src(i) : 0;
-    }
   }
+  const int items = (N + kSmallThreads - 1) / kSmallThreads;
+  const int i0 = wave * items * 64 + lane;
+  uint32_t key[kSmallItems], last[kSmallItems];
 #pragma unroll
-  for (int k = 0; k < kSmallItems; ++k) pos[k] = i0 + k * 64;
-
-  const int passes = (bits + 7) / 8;
-  int shift = 0;
-  for (int p = 0; p < passes; ++p) {
-    const int b = (bits - shift + passes - p - 1) / (passes - p);
-    const uint32_t digits = (1u << b) - 1;
-    for (int d = tid; d < kSmallWaves * 256 / 2; d += kSmallThreads)
-      reinterpret_cast<uint32_t*>(&cnt[0][0])[d] = 0;
-    __syncthreads();
-    uint32_t rank[kSmallItems];
-#pragma unroll
-    for (int k = 0; k < kSmallItems; ++k)
-      if (k < items)  // whole waves
-        rank[k] = rank_digit<8, uint16_t>(
-            cnt[wave], (key[k] >> shift) & digits, i0 + k * 64 < N);
-    __syncthreads();
-    // a digit's counts, wave by wave: four threads take four waves each
-    const int digit = tid & 255, quarter = tid >> 8;
-    uint32_t mine4[4], sum4 = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      mine4[w] = sum4;
-      sum4 += cnt[quarter * 4 + w][digit];
-    }
-    quarters[quarter][digit] = (uint16_t)sum4;
-    __syncthreads();
-    uint32_t total = 0, lead = 0;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      if (q < quarter) lead += quarters[q][digit];
-      total += quarters[q][digit];
-    }
-#pragma unroll
-    for (int w = 0; w < 4; ++w)
-      cnt[quarter * 4 + w][digit] = (uint16_t)(lead + mine4[w]);
-    // exclusive sum over the 256 digits, by the first four waves
-    uint32_t x = total;
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t y = __shfl_up(x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 63 && wave < 4) s4[wave] = x;
-    __syncthreads();
-    if (tid < 256) {
-      uint32_t before = 0;
-      for (int w = 0; w < wave; ++w) before += s4[w];
-      local[tid] = before + x - total;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kSmallItems; ++k) {
-      if (k < items && i0 + k * 64 < N) {
-        const uint32_t d = (key[k] >> shift) & digits;
-        const uint32_t at = local[d] + cnt[wave][d] + rank[k];
-        s_key[at] = key[k];
-        s_pos[at] = (uint16_t)pos[k];
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < kSmallItems; ++k) {
-      const int i = i0 + k * 64;
-      if (k < items && i < N) {
-        key[k] = s_key[i];
-        pos[k] = s_pos[i];
-      }
-    }
-    __syncthreads();
-    shift += b;
+  for (int k = 0; k < kSmallItems; ++k) {
+    const int i = i0 + k * 64;
+    const bool in = k < items && i < N;
+    key[k] = in ? keys[i] : 0;
+    last[k] = in && i > 0 ? keys[i - 1] : 0;
   }
-  // each run's number: first occurrences before it, by wave, then overall
   uint32_t here = 0, place[kSmallItems];
   bool first[kSmallItems];
 #pragma unroll
   for (int k = 0; k < kSmallItems; ++k) {
     const int i = i0 + k * 64;
-    first[k] = k < items && i < N && (i == 0 || s_key[i - 1] != key[k]);
+    first[k] = k < items && i < N && (i == 0 || last[k] != key[k]);
     const uint64_t set = __ballot(first[k]);
     place[k] = here + __builtin_amdgcn_mbcnt_hi(
                           (uint32_t)(set >> 32),
                           __builtin_amdgcn_mbcnt_lo((uint32_t)set, 0));
     here += __popcll(set);
   }
-  if (lane == 0) local[wave] = here;
+  if (lane == 0) s_count[wave] = here;
   __syncthreads();
   uint32_t before = 0, all = 0;
   for (int w = 0; w < kSmallWaves; ++w) {
-    if (w < wave) before += local[w];
-    all += local[w];
+    if (w < wave) before += s_count[w];
+    all += s_count[w];
   }
   if (tid == 0) {
     runs[0] = all;
@@ -629,17 +590,13 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small_kernel(
   }
 #pragma unroll
   for (int k = 0; k < kSmallItems; ++k) {
-    const int i = i0 + k * 64;
-    if (k < items && i < N) {
-      pos_out[i] = pos[k];
-      if (first[k]) {
-        const uint32_t at = before + place[k];
-        starts[at] = i;
-        if constexpr (IDS)
-          unique[at] = (int64_t)((uint64_t)low + (uint64_t)key[k]);
-        else
-          rows[at] = key[k];
-      }
+    if (first[k]) {
+      const uint32_t at = before + place[k];
+      starts[at] = i0 + k * 64;
+      if constexpr (IDS)
+        unique[at] = (int64_t)((uint64_t)info[0] + (uint64_t)key[k]);
+      else
+        rows[at] = key[k];
     }
   }
 }
@@ -865,7 +822,7 @@ __global__ __launch_bounds__(256) void segment_kernel(edl_segments a,
   }
 }
 
-// where one workgroup has sorted and knows the runs: a wave to a run, its
+// where the small sort has been, and the runs are known: a wave to a run, its
 // groups of lanes taking every so-many-th token; one launch in place of three
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void segment_run_kernel(edl_segments a,
@@ -1232,29 +1189,34 @@ extern "C" int64_t edl_sort_counts(int64_t N) {
 #undef EDL_COUNTS
 }
 
-// the one-workgroup sorts: see the kernel
+// the small sorts, and their runs: see the kernels
 extern "C" int edl_sort_rows_small(const void* ids, int ids64, int64_t V,
-                                   int64_t N, uint32_t* pos, uint32_t* starts,
-                                   uint32_t* runs, uint32_t* rows,
-                                   void* zeros, int64_t zero_bytes,
-                                   hipStream_t st) {
-  int bits = 1;
-  while (bits < 32 && (V >> bits) != 0) ++bits;
+                                   int64_t N, uint32_t* keys, uint32_t* pos,
+                                   uint32_t* starts, uint32_t* runs,
+                                   uint32_t* rows, void* zeros,
+                                   int64_t zero_bytes, hipStream_t st) {
+  const int tiles = (int)((N + kSmallTile - 1) / kSmallTile);
   const int64_t fill = std::min<int64_t>(
       (zero_bytes + kSmallThreads * 16 - 1) / (kSmallThreads * 16),
       kZeroBlocks * 256 / kSmallThreads);
-  sort_small_kernel<Keys32, false><<<1 + (int)fill, kSmallThreads, 0, st>>>(
-      Keys32{ids, ids64 != 0, V}, (int)N, bits, pos, starts, runs, rows,
-      nullptr, nullptr, Zeros{static_cast<uint8_t*>(zeros), zero_bytes});
+  rank_small_kernel<Keys32, false>
+      <<<tiles + (int)fill, kSmallThreads, 0, st>>>(
+          Keys32{ids, ids64 != 0, V}, (int)N, keys, pos, nullptr, tiles,
+          Zeros{static_cast<uint8_t*>(zeros), zero_bytes});
+  runs_small_kernel<false><<<1, kSmallThreads, 0, st>>>(
+      keys, (int)N, nullptr, starts, runs, rows, nullptr, nullptr);
   return (int)hipGetLastError();
 }
-extern "C" int edl_sort_ids_small(const int64_t* ids, int64_t N, uint32_t* pos,
+extern "C" int edl_sort_ids_small(const int64_t* ids, int64_t N,
+                                  uint32_t* keys, uint32_t* pos, int64_t* info,
                                   uint32_t* starts, uint32_t* runs,
                                   int64_t* unique, uint32_t* found,
                                   hipStream_t st) {
-  sort_small_kernel<Keys32Of, true><<<1, kSmallThreads, 0, st>>>(
-      Keys32Of{ids}, (int)N, 0, pos, starts, runs, nullptr, unique, found,
-      Zeros{});
+  const int tiles = (int)((N + kSmallTile - 1) / kSmallTile);
+  rank_small_kernel<Keys32Of, true><<<tiles, kSmallThreads, 0, st>>>(
+      Keys32Of{ids}, (int)N, keys, pos, info, tiles, Zeros{});
+  runs_small_kernel<true><<<1, kSmallThreads, 0, st>>>(
+      keys, (int)N, info, starts, runs, nullptr, unique, found);
   return (int)hipGetLastError();
 }
 
