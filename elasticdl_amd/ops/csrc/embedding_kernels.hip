@@ -259,8 +259,8 @@ __device__ inline uint32_t rank_digit(volatile C* count, uint32_t d, bool in) {
 }
 
 // Zeros, by workgroups beside those of a sort, whose waits they fill, and past
-// L2, which the sort uses: a whole gradient of 128 MB 157 us, 163 with a launch
-// of its own for them.
+// L2, which the sort uses: a whole gradient of 128 MB 144 us, 152 with all of
+// them beside its first kernel, 158 with a launch of their own.
 struct Zeros {
   uint8_t* to;  // on a border of 16 bytes
   int64_t bytes;
@@ -364,7 +364,7 @@ __global__ __launch_bounds__(256) void sort_move_kernel(
     S src, const uint32_t* __restrict__ pos_in, int64_t N, int shift, int bits,
     int tiles, const uint32_t* __restrict__ counts,
     const uint32_t* __restrict__ totals, typename S::K* __restrict__ keys_out,
-    uint32_t* __restrict__ pos_out) {
+    uint32_t* __restrict__ pos_out, Zeros zeros) {
   typedef typename S::K K;
   constexpr int ITEMS = P::ITEMS, kTile = ITEMS * 256, kBins = 1 << P::BITS;
   constexpr int kOwn = kBins / 256;  // neighbouring digits to a thread
@@ -374,6 +374,8 @@ __global__ __launch_bounds__(256) void sort_move_kernel(
   __shared__ uint16_t local[kBins];  // a digit's first place in the tile
   __shared__ uint32_t goal[kBins];   // where it goes, less that place
   __shared__ uint32_t s4[4];
+  if ((int)blockIdx.x >= tiles)
+    return fill_zeros<256>(zeros, blockIdx.x - tiles, gridDim.x - tiles);
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int bins = 1 << bits;
   const int tile = xcd_order(blockIdx.x, tiles);
@@ -1080,11 +1082,16 @@ int sort_pass(S src, const uint32_t* pos_in, int64_t N, int shift, int bits,
   constexpr int kTile = P::ITEMS * 256;
   const int tiles = (int)((N + kTile - 1) / kTile);
   const int bins = 1 << bits, fill = zeros.bytes ? kZeroBlocks : 0;
+  Zeros half = zeros;  // a part beside each of the two that wait most
+  half.bytes = zeros.bytes / 32 * 16;
+  zeros.to += half.bytes;
+  zeros.bytes -= half.bytes;
   sort_count_kernel<S, P><<<tiles + fill, 256, 0, st>>>(src, N, shift, bits,
-                                                        tiles, counts, zeros);
+                                                        tiles, counts, half);
   sort_offsets_kernel<<<bins, 256, 0, st>>>(counts, tiles, totals);
-  sort_move_kernel<S, FIRST, P><<<tiles, 256, 0, st>>>(
-      src, pos_in, N, shift, bits, tiles, counts, totals, keys_out, pos_out);
+  sort_move_kernel<S, FIRST, P><<<tiles + fill, 256, 0, st>>>(
+      src, pos_in, N, shift, bits, tiles, counts, totals, keys_out, pos_out,
+      zeros);
   return (int)hipGetLastError();
 }
 

@@ -1216,27 +1216,47 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_rows_kernel(
   const int kbs = (int)(g.ld / kBlk);
   const uint8_t* pb = g.b + n * g.ld + q4 * 32;
   const uint8_t* ps = g.sb + scale_slot(n);
+  // what the end needs and what the next block does are fetched ahead
+  float bias[4] = {0.f, 0.f, 0.f, 0.f};
+  if (wave == 0 && g.bias) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (n0 + q4 * 4 + q < g.N)
+        bias[q] = load_any(g.bias, n0 + q4 * 4 + q, g.bias_type);
+  }
+  constexpr bool kHalf = sizeof(T) == 2;
+  i32x8 b_next;
+  int sb_next;
+  u32x4 w_next[4] = {};
+  auto fetch = [&](int kb) {
+    b_next = *reinterpret_cast<const i32x8*>(pb + (int64_t)kb * kBlk);
+    sb_next = ps[(int64_t)kb * g.b_rp];
+    if (kHalf && wide && (kb + 1) * kBlk <= K) {  // the wave alike
+      const T* p = x + (row < g.M ? row : 0) * x_ld + (int64_t)kb * kBlk +
+                   q4 * 32;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        w_next[k] = *reinterpret_cast<const u32x4*>(p + k * 8);
+    }
+  };
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
+  if (wave < kbs) fetch(wave);
   for (int kb = wave; kb < kbs; kb += kFewWaves) {
-    const i32x8 b = *reinterpret_cast<const i32x8*>(pb + (int64_t)kb * kBlk);
-    const int sb = ps[(int64_t)kb * g.b_rp];
+    const i32x8 b = b_next;
+    const int sb = sb_next;
+    u32x4 w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = w_next[k];
+    if (kb + kFewWaves < kbs) fetch(kb + kFewWaves);
     const int64_t k0 = (int64_t)kb * kBlk + q4 * 32;
     i32x8 a;
     int sa;
     bool done = false;
-    if constexpr (sizeof(T) == 2) {
-      if (wide && (kb + 1) * kBlk <= K) {  // the wave alike
-        u32x4 w[4];
-        const T* p = x + (row < g.M ? row : 0) * x_ld + k0;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          w[k] = *reinterpret_cast<const u32x4*>(p + k * 8);
-        done = round32_fast<T>(w, &sa, &a);
-      }
+    if constexpr (kHalf) {
+      if (wide && (kb + 1) * kBlk <= K) done = round32_fast<T>(w, &sa, &a);
     }
     if (!done) a = round32<T>(x, x_ld, g.M, K, row, k0, wide, &sa);
-    if (sizeof(T) == 4)  // the result is in 32 bits
+    if (!kHalf)  // the result is in 32 bits
       acc = mfma_wide(widen(b, scale_value(sb, 0)),
                       widen(a, scale_value(sa, 0)), acc);
     else
@@ -1258,9 +1278,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_rows_kernel(
   for (int q = 0; q < 4; ++q) {
     int64_t c = n0 + q4 * 4 + q;
     if (c >= g.N) continue;
-    float z = t[q];
-    if (g.bias) z += load_any(g.bias, c, g.bias_type);
-    store_any(g.c, row * g.N + c, activate(z, g.act), g.c_type);
+    store_any(g.c, row * g.N + c, activate(t[q] + bias[q], g.act), g.c_type);
   }
 }
 
