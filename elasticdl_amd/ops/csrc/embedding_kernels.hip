@@ -55,6 +55,48 @@ __device__ inline int64_t load_id(const void* ids, bool wide, int64_t i) {
               : (int64_t)static_cast<const int32_t*>(ids)[i];
 }
 
+// U neighbours at `at`, of which n are there: wide loads where all are, as a
+// load costs its instruction for every row of lanes, not its bytes
+template <typename T, int U, int ALIGN>
+__device__ inline void load_run(const void* p, int64_t at, T* to) {
+  constexpr int W = 16 / sizeof(T) < U ? 16 / sizeof(T) : U;
+  typedef T vec __attribute__((ext_vector_type(W), aligned(ALIGN)));
+#pragma unroll
+  for (int u = 0; u < U; u += W) {
+    const vec v = *reinterpret_cast<const vec*>(static_cast<const T*>(p) + at + u);
+#pragma unroll
+    for (int q = 0; q < W; ++q) to[u + q] = v[q];
+  }
+}
+template <int U>
+__device__ inline void load_ids(const void* ids, bool wide, int64_t at, int n,
+                                int64_t* id) {
+  if (n < U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = u < n ? load_id(ids, wide, at + u) : -1;
+  } else if (wide) {
+    load_run<int64_t, U, 8>(ids, at, id);
+  } else {
+    int32_t v[U];
+    load_run<int32_t, U, 4>(ids, at, v);
+#pragma unroll
+    for (int u = 0; u < U; ++u) id[u] = v[u];
+  }
+}
+template <int U>
+__device__ inline void load_weights(const void* p, int type, int64_t at, int n,
+                                    float* w) {
+  if (p == nullptr) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = 1.f;
+  } else if (type == EDL_T_F32 && n >= U) {
+    load_run<float, U, 4>(p, at, w);
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = u < n ? load_any(p, at + u, type) : 0.f;
+  }
+}
+
 // lanes that share a row: a power of two, at most a wave
 __host__ __device__ inline int lanes_of(int D, int vec) {
   int n = (D + vec - 1) / vec, l = 1;
@@ -94,13 +136,13 @@ __global__ __launch_bounds__(256) void lookup_kernel(edl_bag a, int subs,
   int count = 0;
   for (int l0 = sub * U; l0 < a.L; l0 += subs * U) {
     int64_t id[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      id[u] = l0 + u < a.L ? load_id(a.ids, a.ids64, bag * a.L + l0 + u) : -1;
+    load_ids<U>(a.ids, a.ids64, bag * a.L + l0, a.L - l0, id);
     bool any = false;
 #pragma unroll
     for (int u = 0; u < U; ++u) any |= id[u] >= 0;
     if (!__any(any)) continue;  // behind the ends of short bags
+    float weight[U];
+    load_weights<U>(a.weights, a.w_type, bag * a.L + l0, a.L - l0, weight);
     V row[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -110,8 +152,7 @@ __global__ __launch_bounds__(256) void lookup_kernel(edl_bag a, int subs,
     for (int u = 0; u < U; ++u) {
       if (id[u] < 0) continue;
       ++count;
-      const float w =
-          a.weights ? load_any(a.weights, bag * a.L + l0 + u, a.w_type) : 1.f;
+      const float w = weight[u];
       const float bad = id[u] < a.V ? 0.f : __uint_as_float(0x7fc00000u);
 #pragma unroll
       for (int k = 0; k < VEC; ++k)
@@ -158,11 +199,9 @@ __global__ __launch_bounds__(256) void weight_grad_kernel(edl_bag a,
   for (int l = l0; l < l0 + 8 && l < a.L; l += U) {
     int64_t id[U];
     float dot[U];
+    load_ids<U>(a.ids, a.ids64, bag * a.L + l, a.L - l, id);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      id[u] = l + u < a.L ? load_id(a.ids, a.ids64, bag * a.L + l + u) : -1;
-      dot[u] = 0.f;
-    }
+    for (int u = 0; u < U; ++u) dot[u] = 0.f;
     for (int col = l_lane * VEC; col < a.D; col += lanes * VEC) {
       V g, row[U];
       g.v = *reinterpret_cast<const decltype(g.v)*>(dy + col);

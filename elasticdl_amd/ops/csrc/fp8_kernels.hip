@@ -1116,9 +1116,9 @@ __global__ __launch_bounds__(256) void finish_kernel(edl_fp8_finish f) {
 // registers of the wave that multiplies it and the weights go from memory
 // straight to the matrix instruction, so that a layer is one launch. A
 // workgroup takes 16 columns; its 16 waves share the blocks of 128 between
-// them and join through LDS in order. Bound by the read of the weights.
+// them and join through LDS in order, with a block's loads ahead of its turn
+// (16 x 4096 x 4096 9.2 us, 10.1 without). Bound by the read of the weights.
 constexpr int kFewWaves = 16;
-
 
 // 32 neighbours of a row as e4m3 bytes, and the scale's byte of the 128 that
 // the four lanes of a row hold together
@@ -1146,7 +1146,7 @@ __device__ inline i32x8 round32(const T* x, int64_t ld, int64_t M, int K,
 // The same for 16-bit inputs of 32 whole neighbours: the largest by packed
 // 16-bit integers and two values a conversion, a fifth of the instructions.
 // Every workgroup rounds all of x, so they are what 16 rows cost: 16 x 4096 x
-// 4096 12.3 us without this.
+// 4096 2.2 us more without this.
 template <typename T>
 struct Halves;
 template <>
