@@ -178,8 +178,8 @@ __global__ __launch_bounds__(256) void lookup_kernel(edl_bag a, int subs,
       o.v;
 }
 
-// the weights' gradient: a group of lanes keeps its bag's dy (its first
-// piece; wider rows read the rest again) and goes over the ids
+// the weights' gradient: a group of lanes goes over a bag's ids, which lie
+// in its lanes' registers four at a time
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void weight_grad_kernel(edl_bag a,
                                                           int64_t block0) {
@@ -202,7 +202,10 @@ __global__ __launch_bounds__(256) void weight_grad_kernel(edl_bag a,
     load_ids<U>(a.ids, a.ids64, bag * a.L + l, a.L - l, id);
 #pragma unroll
     for (int u = 0; u < U; ++u) dot[u] = 0.f;
-    for (int col = l_lane * VEC; col < a.D; col += lanes * VEC) {
+    bool any = false;  // not behind the end of a short bag
+#pragma unroll
+    for (int u = 0; u < U; ++u) any |= id[u] >= 0;
+    for (int col = l_lane * VEC; any && col < a.D; col += lanes * VEC) {
       V g, row[U];
       g.v = *reinterpret_cast<const decltype(g.v)*>(dy + col);
 #pragma unroll
