@@ -781,6 +781,10 @@ __global__ __launch_bounds__(256) void segment_kernel(edl_segments a,
 #pragma unroll
   for (int k = 0; k < VEC; ++k) acc[k] = 0.f;
   uint32_t cur = a.keys[t0];
+  if (cur >= a.limit) {  // padding, which is sorted behind the rest
+    if (col == 0) a.head[c] = a.tail[c] = kNone;
+    return;
+  }
   bool open = t0 > 0 && a.keys[t0 - 1] == cur;  // begun in a chunk before
   uint32_t head = kNone, tail = kNone;
 
