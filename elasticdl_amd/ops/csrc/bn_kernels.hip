@@ -227,12 +227,20 @@ __global__ __launch_bounds__(BN_THREADS) void bn_bwd_reduce_kernel(
         *reinterpret_cast<const bn_bf16x8*>(x + (r + step) * C + c0);
     bn_bf16x8 vd1 =
         *reinterpret_cast<const bn_bf16x8*>(dy + (r + step) * C + c0);
+    // the mask by 8 as well: seven layers of 512 images 237 us in the mean, 324
+    // element by element
+    bn_bf16x8 vr0 = {}, vr1 = {};
+    if (relu_out != nullptr) {
+      vr0 = *reinterpret_cast<const bn_bf16x8*>(relu_out + r * C + c0);
+      vr1 =
+          *reinterpret_cast<const bn_bf16x8*>(relu_out + (r + step) * C + c0);
+    }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       float d0 = (float)vd0[k], d1 = (float)vd1[k];
       if (relu_out != nullptr) {
-        d0 = (float)relu_out[r * C + c0 + k] > 0.f ? d0 : 0.f;
-        d1 = (float)relu_out[(r + step) * C + c0 + k] > 0.f ? d1 : 0.f;
+        d0 = (float)vr0[k] > 0.f ? d0 : 0.f;
+        d1 = (float)vr1[k] > 0.f ? d1 : 0.f;
       }
       s1[k] += d0 + d1;
       s2[k] += d0 * ((float)vx0[k] - m[k]) * rs[k] +
@@ -353,13 +361,19 @@ __global__ __launch_bounds__(BN_THREADS) void bn_bwd_apply_kernel(
         *reinterpret_cast<const bn_bf16x8*>(x + (r + step) * C + c0);
     bn_bf16x8 vd1 =
         *reinterpret_cast<const bn_bf16x8*>(dy + (r + step) * C + c0);
+    bn_bf16x8 vr0 = {}, vr1 = {};
+    if (relu_out != nullptr) {
+      vr0 = *reinterpret_cast<const bn_bf16x8*>(relu_out + r * C + c0);
+      vr1 =
+          *reinterpret_cast<const bn_bf16x8*>(relu_out + (r + step) * C + c0);
+    }
     bn_bf16x8 o0, o1;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       float d0 = (float)vd0[k], d1 = (float)vd1[k];
       if (relu_out != nullptr) {
-        d0 = (float)relu_out[r * C + c0 + k] > 0.f ? d0 : 0.f;
-        d1 = (float)relu_out[(r + step) * C + c0 + k] > 0.f ? d1 : 0.f;
+        d0 = (float)vr0[k] > 0.f ? d0 : 0.f;
+        d1 = (float)vr1[k] > 0.f ? d1 : 0.f;
       }
       o0[k] = (__bf16)(a[k] * d0 - b[k] * (float)vx0[k] + c[k]);
       o1[k] = (__bf16)(a[k] * d1 - b[k] * (float)vx1[k] + c[k]);
