@@ -113,6 +113,8 @@ __host__ __device__ inline int pieces_of(int D, int vec) {
 // A row is read by the few lanes that its width takes, 8 ids at a time so
 // that 8 rows are in flight; `subs` such groups share a bag, each taking
 // every so-many-th eight, where bags alone are too few to fill the chip.
+// Bound by random rows: 16384 bags of up to 50 rows of 128 bytes 15.6 us, 3.0
+// TB/s with the padding's ids.
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void lookup_kernel(edl_bag a, int subs,
                                                      int64_t block0) {
@@ -179,7 +181,8 @@ __global__ __launch_bounds__(256) void lookup_kernel(edl_bag a, int subs,
 }
 
 // the weights' gradient: a group of lanes goes over a bag's ids, which lie
-// in its lanes' registers four at a time
+// in its lanes' registers four at a time (16384 bags of up to 50 ids, 64
+// columns of bf16 19 us; eight at a time 24)
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void weight_grad_kernel(edl_bag a,
                                                           int64_t block0) {
@@ -758,7 +761,9 @@ __global__ __launch_bounds__(256) void unique_place_kernel(
 // begins and ends in the chunk is written at once. One that goes on past an
 // end of the chunk leaves its sum in the workspace, and where it begins the
 // join collects the sums of those behind: short runs by a group of lanes of
-// a workgroup's first wave, long ones (over kShort chunks) by all of it.
+// a workgroup's first wave, long ones (over kShort chunks) by all of it. Bound
+// by the gather: 2.6 million rows of 64 bytes 73 us, 3.6 TB/s (89 with keys
+// and positions read one by one), and 13 for the join.
 constexpr int kShort = 8;
 
 template <typename T, int VEC>
