@@ -419,6 +419,38 @@ def test_coalesce_of_strided_values():
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,d", [(400_000, 16), (70_000, 130), (300_000, 1)])
+def test_runs_of_most_of_the_tokens(n, d):
+    # whole numbers: every sum is exact
+    values = torch.randint(-3, 4, (n, d), generator=gen(n)).float().cuda()
+    for ids in (torch.full((n,), 12345), torch.arange(n) % 2 * 7,
+                torch.where(torch.arange(n) < n - 9, 5, torch.arange(n))):
+        rows, unique = coalesce_rows(values, ids.cuda())
+        want, back = torch.unique(ids, return_inverse=True)
+        assert torch.equal(unique.cpu(), want)
+        sums = torch.zeros(want.numel(), d, dtype=torch.float64)
+        sums.index_add_(0, back, values.cpu().double())
+        assert torch.equal(rows.cpu().double(), sums)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v,d", [(7, 3), (1000, 16), (1, 1)])
+@pytest.mark.parametrize("bags", [30, 4000])
+def test_gradient_of_padding_alone_is_zero(v, d, bags):
+    for dtype in TYPES:
+        table = randn(v, d, dtype=dtype).cuda().requires_grad_(True)
+        ids = torch.full((bags, 3), -1, device="cuda")
+        for last in (-1, v - 1):
+            ids[-1, -1] = last
+            out = embedding_lookup(table, ids, None, "sum")
+            g, = torch.autograd.grad(out, table, torch.full_like(out, 2.0))
+            want = torch.zeros_like(g)
+            if last >= 0:
+                want[last] = 2.0
+            assert torch.equal(g, want)
+
+
 # ------------------------------- refusals ---------------------------------
 def test_refusals():
     table, ids = randn(6, 4), torch.zeros(2, 3, dtype=torch.int64)
