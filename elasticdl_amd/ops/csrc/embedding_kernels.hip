@@ -506,7 +506,9 @@ __global__ __launch_bounds__(256) void sort_move_kernel(
 // of each wave for each share those that they are compared with.
 //
 // IDS: ids of any value, less 2^31 below the first, which goes to info[0];
-// info[1]: some lie too far from it for 32 bits, and nothing is done.
+// info[1]: some lie too far from it for 32 bits, and nothing is done. The
+// difference wraps at 2^64, so that ids at one end of int64 look near to the
+// other's: their order and the keys' disagree, which is too far as well.
 // Else rows of a table.
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallItems = EDL_SORT_SMALL / kSmallThreads;
@@ -526,13 +528,15 @@ __global__ __launch_bounds__(kSmallThreads) void rank_small_kernel(
   const int all = (N + 4 * kSmallShares - 1) / (4 * kSmallShares) *
                   (4 * kSmallShares);
   if constexpr (IDS) {
-    const uint64_t low = (uint64_t)src.ids[0] - 0x80000000ull;
+    const int64_t first = src.ids[0];
+    const uint64_t low = (uint64_t)first - 0x80000000ull;
     uint32_t off = 0;
 #pragma unroll
     for (int k = 0; k < kSmallItems; ++k) {
       const int i = k * kSmallThreads + tid;
-      const uint64_t rel = (uint64_t)src.ids[i < N ? i : 0] - low;
-      off |= (uint32_t)(rel >> 32);
+      const int64_t id = src.ids[i < N ? i : 0];
+      const uint64_t rel = (uint64_t)id - low;
+      off |= (uint32_t)(rel >> 32) | ((id < first) != (rel < 0x80000000ull));
       if (i < all) s_key[i] = i < N ? (uint32_t)rel : kNone;
     }
     const bool far = __syncthreads_or(off != 0);

@@ -399,6 +399,27 @@ def test_deduplicate(n, d, low, high, device):
     check(rows, want, (count.unsqueeze(1) + 8) * 2.0 ** -24 * size, dtype)
 
 
+LOW, HIGH = -(1 << 63), (1 << 63) - 1
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("ids", [
+    [HIGH, LOW], [LOW, HIGH], [HIGH - 5, LOW + 3, HIGH, LOW, HIGH - 5],
+    [LOW + (1 << 31) - 1, HIGH, LOW], [HIGH - (1 << 31) + 2, LOW, HIGH],
+    [LOW, LOW + (1 << 31), HIGH], [LOW + 1, LOW, LOW + 1], [HIGH, HIGH - 1]])
+@pytest.mark.parametrize("times", [1, 700])
+def test_deduplicate_at_the_ends_of_int64(ids, times, device):
+    """The two ends are neighbours modulo 2^64, and far apart."""
+    ids = torch.tensor(ids).repeat(times)
+    values = torch.arange(1.0, 2 * ids.numel() + 1).view(-1, 2) % 64
+    rows, unique = deduplicate_indexed_slices(values.to(device), ids.to(device))
+    want, place = torch.unique(ids, return_inverse=True)
+    assert torch.equal(unique.cpu(), want)
+    # whole numbers below 2^24: every sum is exact
+    sums = torch.zeros(want.numel(), 2).index_add_(0, place, values)
+    assert torch.equal(rows.cpu(), sums)
+
+
 @pytest.mark.gpu
 def test_deduplicate_keeps_a_gradient_where_one_is_asked_for():
     values = randn(50, 3).cuda().requires_grad_(True)
