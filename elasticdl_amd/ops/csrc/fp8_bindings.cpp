@@ -208,6 +208,7 @@ Tensor product_of(edl_fp8_gemm& g, const Blocks& a, const Blocks& b,
   g.c = c.data_ptr();
   g.c_type = type_code(type, "output");
   g.c_wide = aligned(c, b.rows);
+  g.wide = g.c_type == EDL_T_F32;
   return c;
 }
 void bias_into(edl_fp8_gemm& g, const Tensor& bias) {
@@ -324,6 +325,7 @@ class Fp8Dense : public torch::autograd::Function<Fp8Dense> {
     f.g[0].act = (int)act;
     bias_into(f.g[0], bias);
     f.g[0].mask_ld = mask_row(n);
+    f.g[0].wide |= bits;
     if (!few && m > 0) plan_into(f, 1, passing);
     Tensor held;
     if (need_x || need_w || bits) held = kept.place(x);

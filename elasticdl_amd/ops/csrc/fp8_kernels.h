@@ -51,6 +51,7 @@ struct edl_fp8_gemm {
   void* c;  // [M, N], contiguous
   int c_type;
   bool c_wide;    // 16-byte stores of 16 neighbours are aligned
+  bool wide;      // sums in 32 bits: c is of 32 bits, or there is a mask
   uint8_t* mask;  // relu: bits of c > 0, rows mask_ld bytes apart; may be null
   int64_t mask_ld;
   int tile;     // EDL_TILE_*

@@ -14,11 +14,13 @@
 // neighbouring products with about 16 bits below the largest of them (32
 // only between such groups): 1.6e-5 of a result's norm, measured over random
 // e4m3. That is far below e4m3's and a 16-bit result's own rounding, but not
-// 32 bits. So where a result is returned in 32 bits the bytes are widened to
-// bf16 in registers on the way (exactly, scale included) and multiplied by
-// the bf16 instruction, whose sums hold 24 bits (8e-9 measured), at half the
-// rate. And where the sign of a 16-bit result decides a relu's gradient, the
-// few sums that lie near zero are added up once more in 32 bits (settle).
+// 32 bits. So where a result is returned in 32 bits, or the sign of a sum
+// decides a relu's gradient, the bytes are widened to bf16 in registers on the
+// way (exactly from 2^-126 up, scale included) and multiplied by the bf16
+// instruction, whose sums hold 24 bits (8e-9 measured), at half the rate. The error of a sum is
+// in proportion to its largest products, not to its own size or its
+// neighbours', so a result says nothing of how near to zero is too near, and
+// all of a relu's sums are taken in 32 bits.
 //
 // Layout. A matrix [R, C] that is contracted over C is stored as bytes
 // [R, Cp], Cp = C rounded up to 128 (zeros behind C), with scales
@@ -36,7 +38,6 @@ typedef __attribute__((ext_vector_type(8))) int i32x8;
 typedef __attribute__((ext_vector_type(4))) int i32x4;
 typedef __attribute__((ext_vector_type(2))) int i32x2;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
-typedef __attribute__((ext_vector_type(2))) float f32x2;
 typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
@@ -483,123 +484,9 @@ __device__ inline f32x4 mfma_wide(const Wide& a, const Wide& b, f32x4 c) {
   return c;
 }
 
-// one element of A B^T by a whole wave, in 32 bits
-__device__ inline float dot_of(const edl_fp8_gemm& g, int64_t m, int64_t n,
-                               int lane) {
-  const uint8_t *pa = g.a + m * g.ld, *pb = g.b + n * g.ld;
-  const uint8_t *ps = g.sa + scale_slot(m), *pt = g.sb + scale_slot(n);
-  constexpr int U = 4;  // loads in flight: a wave waits here for nothing else
-  float t = 0.f;
-  for (int64_t k0 = lane * 16; k0 < g.ld; k0 += 1024 * U) {
-    i32x4 a[U], b[U];
-    float s[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = k0 + u * 1024 < g.ld;
-      const int64_t k = in ? k0 + u * 1024 : k0, kb = k / kBlk;
-      a[u] = *reinterpret_cast<const i32x4*>(pa + k);
-      b[u] = *reinterpret_cast<const i32x4*>(pb + k);
-      const float sa = scale_value(ps[kb * g.a_rp], 0);
-      s[u] = in ? sa * scale_value(pt[kb * g.b_rp], 0) : 0.f;
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float d = 0.f;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x2 a0 = __builtin_amdgcn_cvt_pk_f32_fp8(a[u][q], false);
-        const f32x2 a1 = __builtin_amdgcn_cvt_pk_f32_fp8(a[u][q], true);
-        const f32x2 b0 = __builtin_amdgcn_cvt_pk_f32_fp8(b[u][q], false);
-        const f32x2 b1 = __builtin_amdgcn_cvt_pk_f32_fp8(b[u][q], true);
-        d = __builtin_fmaf(a0[0], b0[0], d);
-        d = __builtin_fmaf(a0[1], b0[1], d);
-        d = __builtin_fmaf(a1[0], b1[0], d);
-        d = __builtin_fmaf(a1[1], b1[1], d);
-      }
-      t = __builtin_fmaf(d, s[u], t);
-    }
-  }
-  for (int o = 1; o < 64; o <<= 1) t += __shfl_xor(t, o);
-  return t;
-}
-
-// sum over the 16 lanes of a row of lanes; those that are off add nothing
-template <int CTRL>
-__device__ inline float add_ror(float v) {
-  return v + __int_as_float(__builtin_amdgcn_update_dpp(
-                 0, __float_as_int(v), CTRL, 0xf, 0xf, false));
-}
-__device__ inline float sum16(float v) {
-  return add_ror<0x121>(add_ror<0x122>(add_ror<0x124>(add_ror<0x128>(v))));
-}
-
-// Of a lane's 16 sums v (bias apart), those that with their bias lie within
-// 2^-12 of their neighbours' size from zero are replaced by dot_of. The size
-// is a mean, and of the means of every other neighbour the smaller, which one
-// large value does not move; at C's right edge, over 16 rows. 2^-12 of it is
-// 11 times the usual error of a sum (with 2^-13 a few in 67 million signs were
-// still other than in 64 bits). One value in 8000 is met; each takes the wave
-// some 3 us, and a wave stops after 32 of its 1024.
-__device__ inline void settle(const edl_fp8_gemm& g, int64_t m, int64_t n,
-                              float* v, const float* bias, bool live) {
-  const int lane = threadIdx.x & 63;
-  float sum[2] = {0.f, 0.f}, count[2] = {8.f, 8.f};
-#pragma unroll
-  for (int k = 0; k < 16; ++k)
-    sum[k & 1] += n + k < g.N ? __builtin_fabsf(v[k]) : 0.f;
-  if (g.N & 15) {  // all lanes alike
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int in = n >= g.N || !live ? 0
-                     : n + 16 <= g.N   ? 8
-                                       : (int)(g.N - n + 1 - h) / 2;
-      const float rows = sum16(live ? sum[h] : 0.f);
-      const float of = sum16((float)in);
-      if (n + 16 > g.N) {
-        sum[h] = rows;
-        count[h] = of;
-      }
-    }
-  }
-  const float a = count[0] > 0.f ? sum[0] / count[0] : 0.f;
-  const float b = count[1] > 0.f ? sum[1] / count[1] : a;
-  const float size = (a < b ? a : b) * (1.f / 4096);
-  uint32_t near = 0;
-#pragma unroll
-  for (int k = 0; k < 16; ++k)
-    near |= (n + k < g.N && __builtin_fabsf(v[k] + bias[k]) < size ? 1u : 0u)
-            << k;
-  if (!live || !(size < 3e38f)) near = 0;
-  for (int met = 0; met < 32; ++met) {
-    const uint64_t who = __ballot(near != 0);
-    if (who == 0) break;
-    const int at = __builtin_ctzll(who);
-    const int k = __builtin_ctz(__builtin_amdgcn_readlane((int)near, at));
-    const int64_t row = __builtin_amdgcn_readlane((int)m, at);
-    const int64_t col = __builtin_amdgcn_readlane((int)n, at) + k;
-    const float z = dot_of(g, row, col, lane);
-    if (lane == at) {
-      near &= near - 1;
-#pragma unroll
-      for (int q = 0; q < 16; ++q) v[q] = q == k ? z : v[q];
-    }
-  }
-}
-
+// results of 32 bits have sums of 32 bits
 template <typename T>
-struct TypeOf;
-template <>
-struct TypeOf<float> {
-  static constexpr bool wide = true;  // sums in 32 bits
-};
-template <>
-struct TypeOf<__bf16> {
-  static constexpr bool wide = false;
-};
-template <>
-struct TypeOf<_Float16> {
-  static constexpr bool wide = false;
-};
+constexpr bool is_f32 = sizeof(T) == 4;
 
 __device__ inline void load_bias16(const edl_fp8_gemm& g, int64_t n,
                                    float* bias) {
@@ -609,13 +496,10 @@ __device__ inline void load_bias16(const edl_fp8_gemm& g, int64_t n,
                                     : 0.f;
 }
 
-// 16 neighbours of a row of C, from column n; live: the row and column n are
-// C's. Whole waves call it.
+// 16 neighbours of a row of C, from column n
 template <typename T>
 __device__ inline void epilogue16(const edl_fp8_gemm& g, int64_t m, int64_t n,
-                                  float* v, const float* bias, bool live) {
-  if (!TypeOf<T>::wide && g.mask) settle(g, m, n, v, bias, live);
-  if (!live) return;
+                                  float* v, const float* bias) {
   uint32_t bits = 0;
 #pragma unroll
   for (int k = 0; k < 16; ++k) {
@@ -832,7 +716,7 @@ __device__ inline void write_tile(const edl_fp8_gemm& g, const Spot& s,
                 (f32x4){v[k], v[k + 1], v[k + 2], v[k + 3]};
         }
       } else {
-        epilogue16<T>(g, m, n, v, bias, live);
+        if (live) epilogue16<T>(g, m, n, v, bias);
       }
     }
   }
@@ -844,10 +728,9 @@ struct GemmLds {  // two buffers each: A's, B's, scales (256 of A's and B's)
   __align__(1024) uint8_t m[4 * BM * kBlk + 1024];
 };
 
-template <int WM, int WN, int FM, int FN, typename T>
+template <int WM, int WN, int FM, int FN, typename T, bool WIDE>
 __device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
                                  uint8_t* smem) {
-  constexpr bool WIDE = TypeOf<T>::wide;
   constexpr int BM = WM * FM * 16, BN = WN * FN * 16, NW = WM * WN;
   static_assert(BM == BN && (BM == 128 || BM == 256), "buffers' toggle");
   constexpr uint32_t kTile = GemmLds<BM>::kTile, kB = GemmLds<BM>::kB,
@@ -966,11 +849,11 @@ __device__ inline void gemm_tile(const edl_fp8_gemm& g, int block, int blocks,
   write_tile<T, FM, FN>(g, s, h, smem, wave, lane, fA0, wB, BM == 128);
 }
 
-template <int WM, int WN, int FM, int FN, typename T>
+template <int WM, int WN, int FM, int FN, typename T, bool WIDE>
 __global__ __launch_bounds__(WM* WN * 64, 2) void gemm_kernel(
     edl_fp8_gemm g) {
   __shared__ GemmLds<WM * FM * 16> lds;
-  gemm_tile<WM, WN, FM, FN, T>(g, blockIdx.x, gridDim.x, lds.m);
+  gemm_tile<WM, WN, FM, FN, T, WIDE>(g, blockIdx.x, gridDim.x, lds.m);
 }
 
 // Products too small to fill the chip with the tiles above wait for memory,
@@ -986,10 +869,9 @@ struct RingLds {
   __align__(1024) uint8_t m[kBuffers * kOne];
 };
 
-template <typename T>
+template <typename T, bool WIDE>
 __device__ inline void gemm_ring(const edl_fp8_gemm& g, int block, int blocks,
                                  uint8_t* smem) {
-  constexpr bool WIDE = TypeOf<T>::wide;
   constexpr int FM = 2, FN = 4;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1041,19 +923,21 @@ __device__ inline void gemm_ring(const edl_fp8_gemm& g, int block, int blocks,
   write_tile<T, FM, FN>(g, s, h, smem, wave, lane, fA0, wB, true);
 }
 
-template <typename T>
+template <typename T, bool WIDE>
 __global__ __launch_bounds__(256, 2) void gemm_ring_kernel(edl_fp8_gemm g) {
   __shared__ RingLds lds;
-  gemm_ring<T>(g, blockIdx.x, gridDim.x, lds.m);
+  gemm_ring<T, WIDE>(g, blockIdx.x, gridDim.x, lds.m);
 }
+// a backward pass's products, of which none decides a sign
 template <typename T0, typename T1>
 __global__ __launch_bounds__(256, 2) void gemm_ring_pair_kernel(
     edl_fp8_gemm g0, edl_fp8_gemm g1, int blocks0) {
   __shared__ RingLds lds;
   if ((int)blockIdx.x < blocks0)
-    gemm_ring<T0>(g0, blockIdx.x, blocks0, lds.m);
+    gemm_ring<T0, is_f32<T0>>(g0, blockIdx.x, blocks0, lds.m);
   else
-    gemm_ring<T1>(g1, blockIdx.x - blocks0, gridDim.x - blocks0, lds.m);
+    gemm_ring<T1, is_f32<T1>>(g1, blockIdx.x - blocks0, gridDim.x - blocks0,
+                              lds.m);
 }
 
 // the two products of a backward pass in one launch, each of 128 x 128
@@ -1063,10 +947,10 @@ __global__ __launch_bounds__(256, 2) void gemm_pair_kernel(edl_fp8_gemm g0,
                                                            int blocks0) {
   __shared__ GemmLds<128> lds;
   if ((int)blockIdx.x < blocks0)
-    gemm_tile<2, 2, 4, 4, T0>(g0, blockIdx.x, blocks0, lds.m);
+    gemm_tile<2, 2, 4, 4, T0, is_f32<T0>>(g0, blockIdx.x, blocks0, lds.m);
   else
-    gemm_tile<2, 2, 4, 4, T1>(g1, blockIdx.x - blocks0, gridDim.x - blocks0,
-                              lds.m);
+    gemm_tile<2, 2, 4, 4, T1, is_f32<T1>>(g1, blockIdx.x - blocks0,
+                                          gridDim.x - blocks0, lds.m);
 }
 
 // joins a product's splits in order; a thread takes 16 neighbours of a row
@@ -1074,8 +958,8 @@ template <typename T>
 __device__ inline void gemm_join_as(const edl_fp8_gemm& g, int64_t block) {
   const int64_t each = g.part_ld / 16;
   const int64_t id = block * 256 + threadIdx.x;
-  const bool live = id < g.M * each;
-  const int64_t m = live ? id / each : 0, n = live ? (id % each) * 16 : 0;
+  if (id >= g.M * each) return;
+  const int64_t m = id / each, n = (id % each) * 16;
   float v[16], bias[16];
 #pragma unroll
   for (int k = 0; k < 16; ++k) v[k] = 0.f;
@@ -1089,7 +973,7 @@ __device__ inline void gemm_join_as(const edl_fp8_gemm& g, int64_t block) {
     }
   }
   load_bias16(g, n, bias);
-  epilogue16<T>(g, m, n, v, bias, live);
+  epilogue16<T>(g, m, n, v, bias);
 }
 __device__ inline void gemm_join(const edl_fp8_gemm& g, int64_t block) {
   if (g.c_type == EDL_T_F32)
@@ -1375,7 +1259,7 @@ extern "C" void edl_fp8_gemm_plan(edl_fp8_gemm* g, int n, int finish) {
   bool ring = true;
   for (int i = 0; i < n; ++i) {
     g[i].splits = 1;
-    g[i].tile = g[i].c_type != EDL_T_F32 && tiles_of(g[i], 256, 256) >= 256
+    g[i].tile = !g[i].wide && tiles_of(g[i], 256, 256) >= 256
                     ? EDL_TILE_256
                     : EDL_TILE_128;
     if (g[i].tile == EDL_TILE_256 || tiles_of(g[i], 128, 128) >= 256)
@@ -1396,23 +1280,30 @@ extern "C" void edl_fp8_gemm_plan(edl_fp8_gemm* g, int n, int finish) {
   }
 }
 
-template <typename T>
+template <typename T, bool WIDE>
 static void launch_as(const edl_fp8_gemm& g, hipStream_t st) {
   dim3 grid((unsigned)(tiles_of(g) * g.splits));
   if (g.tile == EDL_TILE_RING)
-    gemm_ring_kernel<T><<<grid, dim3(256), 0, st>>>(g);
+    gemm_ring_kernel<T, WIDE><<<grid, dim3(256), 0, st>>>(g);
   else if (g.tile == EDL_TILE_128)
-    gemm_kernel<2, 2, 4, 4, T><<<grid, dim3(256), 0, st>>>(g);
-  else if constexpr (!TypeOf<T>::wide)
-    gemm_kernel<2, 4, 8, 4, T><<<grid, dim3(512), 0, st>>>(g);
+    gemm_kernel<2, 2, 4, 4, T, WIDE><<<grid, dim3(256), 0, st>>>(g);
+  else if constexpr (!WIDE)
+    gemm_kernel<2, 4, 8, 4, T, false><<<grid, dim3(512), 0, st>>>(g);
+}
+template <typename T>
+static void launch_half(const edl_fp8_gemm& g, hipStream_t st) {
+  if (g.wide)
+    launch_as<T, true>(g, st);
+  else
+    launch_as<T, false>(g, st);
 }
 static int launch_one(const edl_fp8_gemm& g, hipStream_t st) {
   if (g.c_type == EDL_T_F32)
-    launch_as<float>(g, st);
+    launch_as<float, true>(g, st);
   else if (g.c_type == EDL_T_BF16)
-    launch_as<__bf16>(g, st);
+    launch_half<__bf16>(g, st);
   else
-    launch_as<_Float16>(g, st);
+    launch_half<_Float16>(g, st);
   return (int)hipGetLastError();
 }
 template <typename T0, typename T1>

@@ -320,6 +320,82 @@ def test_gradients_against_the_formula(m, k, n, act, device):
           dtype)
 
 
+# ----------------------------- relu's gates -------------------------------
+def gates(x, w, b, rows):
+    """Which outputs of these rows let a gradient through. The bias's gradient
+    of 2^i in the i-th of 24 rows is their bits, exact in 32 bits."""
+    b = b.requires_grad_(True)
+    y = fp8_dense(x, w, b, "relu")
+    found = []
+    for at in range(0, len(rows), 24):
+        part = rows[at:at + 24]
+        powers = 2.0 ** torch.arange(-9, len(part) - 9)
+        dy = torch.zeros_like(y)
+        dy[part] = powers.to(y.dtype).to(y.device).unsqueeze(1)
+        db, = torch.autograd.grad(y, b, dy, retain_graph=True)
+        bits = (db.cpu() * 512).long().unsqueeze(0)
+        found.append((bits >> torch.arange(len(part)).unsqueeze(1)) & 1)
+    return torch.cat(found).bool()
+
+
+GATE_SIZES = [(1, 64, 17), (33, 136, 40), (300, 640, 130),
+              (130, 4096, 72),      # a split contraction
+              (2041, 512, 2053),    # many tiles, and edges of them
+              (4100, 192, 4097)]
+
+
+def some(m):
+    return torch.arange(0, m, max(1, m // 200))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", GATE_SIZES)
+def test_relu_gates_of_products_that_cancel(m, k, n, dtype, device):
+    """In eight groups of eight neighbours two products of 448^2 cancel beside
+    six of up to 1/4, and some columns have no weights. Every sum is a multiple
+    of 1/4 below 2^21, so exact in 32 bits in any order, and the gates are
+    those of 64 bits."""
+    g = torch.Generator().manual_seed(m + n)
+    x, w = torch.zeros(m, k), torch.zeros(n, k)
+    for at in range(0, 8 * (k // 64) * 8, (k // 64) * 8):
+        for t in (x, w):
+            t[:, at:at + 6] = torch.randint(-1, 2, (len(t), 6), generator=g) / 2
+        x[:, at + 6:at + 8] = 448.0
+        w[:, at + 6] = 448.0 - 896.0 * torch.randint(0, 2, (n,), generator=g)
+        w[:, at + 7] = -w[:, at + 6]
+    b = torch.randint(-1, 2, (n,), generator=g) / 4
+    w[3::7], b[3::7] = 0.0, 0.0
+    assert torch.equal(values(w, True), w.double())  # e4m3 holds them
+    rows = some(m)
+    z = x[rows].double() @ w.double().t() + b.double()
+    got = gates(x.to(dtype).to(device), w.to(dtype).to(device), b.to(device),
+                rows)
+    assert torch.equal(got, z > 0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", GATE_SIZES)
+def test_relu_gates_of_columns_of_unlike_size(m, k, n, dtype, device):
+    """Columns between 2^-8 and 2^8 times the others' size; a gate may differ
+    where the sum is within its 32 bits' error of zero."""
+    x = randn(m, k, seed=m, dtype=dtype)
+    size = 2.0 ** torch.randint(-8, 9, (n, 1),
+                                generator=torch.Generator().manual_seed(n))
+    w = (randn(n, k, seed=1) * size / k ** 0.5).to(dtype)
+    b = randn(n, seed=2) * size.view(-1) * 0.1
+    b[3::7] = 0.0
+    w[3::7] = 0.0
+    rows = some(m)
+    xq, wq = values(x[rows]), values(w, True)
+    z = xq @ wq.t() + b.double()
+    bound = product_bound(xq, wq, k, b.double().abs(), torch.float32)
+    got = gates(x.to(device), w.to(device), b.to(device), rows)
+    assert bool(((got == (z > 0)) | (z.abs() <= bound)).all())
+    assert bool((z.abs() > bound).float().mean() > 0.8)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_only_what_is_asked_for_is_kept(device):
     x = randn(200, 128, dtype=torch.bfloat16, device=device)
