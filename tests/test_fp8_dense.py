@@ -527,6 +527,29 @@ def test_outputs_and_checkpoints_past_32_bit_offsets():
 
 
 @pytest.mark.gpu
+def test_gradients_of_more_rows_than_can_be_transposed():
+    """Only x^T's form has a limit of rows; x's and the bias's gradients do
+    not use it."""
+    m, k, n = (1 << 24) - 128, 8, 3
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x = torch.randint(-2, 3, (m, k), generator=g, device="cuda",
+                      dtype=torch.int8).bfloat16().requires_grad_(True)
+    w = whole_numbers(n, k, seed=1, most=2, device="cuda", dtype=torch.bfloat16)
+    b = whole_numbers(n, seed=2, device="cuda").requires_grad_(True)
+    y = fp8_dense(x, w, b, "relu")
+    dy = torch.randint(-1, 2, (m, n), generator=g, device="cuda",
+                       dtype=torch.int8).bfloat16()
+    dx, db = torch.autograd.grad(y, (x, b), dy)
+    z = x.detach().float() @ w.float().t() + b.detach()
+    dz = dy.float() * (z > 0)
+    # whole numbers below 2^24, and below 2^8 in dx: exact
+    assert torch.equal(dx, (dz @ w.float()).bfloat16())
+    assert torch.equal(db.double(), dz.double().sum(0))
+    with pytest.raises(RuntimeError, match="too many rows"):
+        fp8_dense(x, w.requires_grad_(True))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m", [4, 300])
 def test_two_graphs_of_a_laid_out_weight(m):
     layers = []
