@@ -11,6 +11,7 @@ import pickle
 
 import pytest
 import torch
+from torch.nn.utils import prune
 
 from elasticdl_amd.common.tensor_utils import deduplicate_indexed_slices
 from elasticdl_amd.layers.embedding import bind_local_engine
@@ -171,6 +172,88 @@ def test_sparse_embedding_scale_and_weights(device):
     w = torch.tensor([[1.0, 0.5, 7.0]], device=device)
     t = se.bag.weight.detach()
     assert torch.equal(se(ids, w), ((t[1] + t[2] * 0.5) * 2).unsqueeze(0))
+
+
+SOME_IDS = torch.tensor([[1, 2, -1], [3, 3, 9], [-1, -1, -1]])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("combiner", ["sum", "mean", "sqrtn"])
+def test_sparse_embedding_runs_a_hooked_bag(combiner, device):
+    """What a user hangs on the bag runs: pruning and weight norms are such
+    hooks, which make the weight before each call."""
+    ids = SOME_IDS.to(device)
+    se = SparseEmbedding(10, 4, combiner, scale=2.0).to(device)
+    want = se(ids)
+    calls = []
+    hook = se.bag.register_forward_hook(
+        lambda m, i, o: (calls.append("out"), o * 4)[1])
+    assert torch.allclose(se(ids), want * 4, rtol=1e-6, atol=0)
+    hook.remove()
+    for add in (se.bag.register_forward_pre_hook,
+                se.bag.register_full_backward_pre_hook,
+                se.bag.register_full_backward_hook):
+        hook = add(lambda m, *a: calls.append("hook"))
+        se(ids).sum().backward()
+        hook.remove()
+    assert calls == ["out", "hook", "hook", "hook"]
+    every = torch.nn.modules.module.register_module_forward_hook(
+        lambda m, i, o: calls.append(type(m).__name__))
+    se(ids)
+    every.remove()
+    assert calls[4:] == ["EmbeddingBag", "SparseEmbedding"]
+    # a pruned weight is made from weight_orig by a hook before each call
+    prune.random_unstructured(se.bag, "weight", amount=0.5)
+    with torch.no_grad():
+        se.bag.weight_orig.mul_(2.0)
+    kept = se.bag.weight_orig.detach() * se.bag.weight_mask
+    want = embedding_lookup(kept, ids, None, combiner, 2.0)
+    got = se(ids)
+    assert torch.allclose(got, want, rtol=1e-6, atol=1e-6)
+    g, = torch.autograd.grad(got.sum(), se.bag.weight_orig)
+    assert not g[se.bag.weight_mask == 0].any() and g.any()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sparse_embedding_runs_another_bag(device):
+    ids = SOME_IDS.to(device)
+    se = SparseEmbedding(10, 4, "sum").to(device)
+    se.bag = torch.nn.EmbeddingBag(10, 4, mode="max").to(device)
+    rows = se.bag.weight.detach()
+    assert torch.equal(se(ids)[:2], torch.stack(
+        [rows[[1, 2]].amax(0), rows[[3, 9]].amax(0)]))
+    se.bag = torch.nn.EmbeddingBag(10, 4, mode="sum", padding_idx=3).to(device)
+    rows = se.bag.weight.detach()
+    assert torch.equal(se(ids)[1], rows[9])
+    se.bag = torch.nn.EmbeddingBag(10, 4, mode="sum", sparse=True).to(device)
+    g, = torch.autograd.grad(se(ids).sum(), se.bag.weight)
+    assert g.is_sparse
+    se.bag = torch.nn.EmbeddingBag(10, 4, mode="sum", max_norm=0.1).to(device)
+    se(ids)
+    assert float(se.bag.weight.detach()[3].norm()) <= 0.1001
+
+    class Twice(torch.nn.EmbeddingBag):
+        def forward(self, *args, **kwargs):
+            return 2 * super().forward(*args, **kwargs)
+
+    se.bag = Twice(10, 4, mode="sum").to(device)
+    rows = se.bag.weight.detach()
+    assert torch.equal(se(ids)[0], 2 * (rows[1] + rows[2]))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sparse_embedding_weights_of_a_bag_that_runs(device):
+    ids = SOME_IDS.to(device)
+    weights = torch.rand(3, 3, device=device)
+    for combiner in ("sum", "sqrtn"):
+        se = SparseEmbedding(10, 4, combiner, scale=2.0).to(device)
+        want = se(ids, weights)
+        se.bag.register_forward_hook(lambda m, i, o: None)
+        assert torch.allclose(se(ids, weights), want, rtol=1e-6, atol=1e-6)
+    se = SparseEmbedding(10, 4, "mean").to(device)
+    se.bag.register_forward_hook(lambda m, i, o: None)
+    with pytest.raises(ValueError, match="weights of a mean"):
+        se(ids, weights)
 
 
 # -------------------------------- serving ---------------------------------
