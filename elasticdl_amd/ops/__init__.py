@@ -40,3 +40,14 @@ def use_native(device) -> bool:
         require_native()
         return True
     return False
+
+
+def reads_directly(*tensors: torch.Tensor) -> bool:
+    """Whether kernels may read these tensors' memory. Not while torch traces,
+    compiles or transforms the call, which sees its own operators alone, and
+    not where a subclass stands for a tensor that lies elsewhere."""
+    return (all(type(t) in (torch.Tensor, torch.nn.Parameter)
+                for t in tensors)
+            and not torch.jit.is_tracing()
+            and not torch.compiler.is_compiling()
+            and not torch._C._are_functorch_transforms_active())

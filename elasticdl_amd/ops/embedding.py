@@ -22,10 +22,23 @@ from typing import Optional, Tuple
 
 import torch
 
-from elasticdl_amd.ops import reference, require_native
+from elasticdl_amd.ops import reads_directly, reference, require_native
 
 _COMBINERS = {None: -1, "sum": 0, "mean": 1, "sqrtn": 2}
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+_MOST = 2 ** 31 - 4097  # positions and rows are 32-bit
+
+
+def takes(table: torch.Tensor, ids: torch.Tensor,
+          weights: Optional[torch.Tensor] = None) -> bool:
+    """Whether ``embedding_lookup`` has these sizes and types; for callers
+    that have another way."""
+    given = (table, ids) if weights is None else (table, ids, weights)
+    return (reads_directly(*given) and table.dtype in _DTYPES
+            and ids.dtype in (torch.int64, torch.int32)
+            and (weights is None or weights.dtype in _DTYPES)
+            and table.shape[0] < _MOST and table.shape[1] < 2 ** 20
+            and ids.numel() < _MOST)
 
 
 def embedding_lookup(table: torch.Tensor, ids: torch.Tensor,

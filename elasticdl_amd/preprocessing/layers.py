@@ -308,7 +308,8 @@ class SparseEmbedding(nn.Module):
 
     ``bag`` itself runs where there is more to it than its weight: hooks
     (pruning and weight norms are such), another class, mode or option of
-    EmbeddingBag, 64 bits. Weights of a mean are refused then, as EmbeddingBag
+    EmbeddingBag, tracing and torch.func transforms, sizes and types that the
+    kernels do not take. Weights of a mean are refused then, as EmbeddingBag
     has none."""
 
     scale = 1.0
@@ -335,13 +336,13 @@ class SparseEmbedding(nn.Module):
 
     def forward(self, ids: torch.Tensor,
                 weights: Optional[torch.Tensor] = None) -> torch.Tensor:
-        if ((ids.is_cuda or weights is not None or self.scale != 1.0)
-                and self.bag.weight.dtype != torch.float64
-                and self._bag_is_its_weight()):
-            from elasticdl_amd.ops.embedding import embedding_lookup
+        if ids.is_cuda or weights is not None or self.scale != 1.0:
+            from elasticdl_amd.ops import embedding
 
-            return embedding_lookup(self.bag.weight, ids, weights,
-                                    self.combiner, self.scale)
+            if (self._bag_is_its_weight()
+                    and embedding.takes(self.bag.weight, ids, weights)):
+                return embedding.embedding_lookup(
+                    self.bag.weight, ids, weights, self.combiner, self.scale)
         mask = ids >= 0
         flat = ids[mask]
         offsets = torch.zeros(ids.shape[0] + 1, dtype=torch.int64,
@@ -351,7 +352,7 @@ class SparseEmbedding(nn.Module):
             out = self.bag(flat, offsets[:-1])
         elif self.combiner == "mean":
             raise ValueError("weights of a mean need a bag without hooks or "
-                             "options")
+                             "options, outside of transforms")
         else:
             out = self.bag(flat, offsets[:-1],
                            weights[mask].to(self.bag.weight.dtype))

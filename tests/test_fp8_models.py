@@ -256,6 +256,33 @@ def test_sparse_embedding_weights_of_a_bag_that_runs(device):
         se(ids, weights)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("combiner", ["sum", "mean", "sqrtn"])
+def test_sparse_embedding_under_transforms(combiner, device):
+    """Tracing and torch.func see torch's own operators."""
+    ids = SOME_IDS.to(device)
+    se = SparseEmbedding(10, 4, combiner).to(device)
+    params = dict(se.named_parameters())
+    got = torch.func.grad(lambda p: torch.func.functional_call(
+        se, p, (ids,)).square().sum())(params)["bag.weight"]
+    want, = torch.autograd.grad(se(ids).square().sum(), se.bag.weight)
+    assert torch.allclose(got, want, rtol=1e-5, atol=1e-6)
+    with torch.no_grad():
+        traced = torch.jit.trace(se, ids)
+        other = ids.flip(1) % 5
+        assert torch.allclose(traced(other), se(other), rtol=1e-6, atol=1e-6)
+        exported = torch.export.export(se, (ids,), strict=False).module()
+        assert torch.allclose(exported(other), se(other), rtol=1e-6, atol=1e-6)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sparse_embedding_wider_than_the_kernels(device):
+    se = SparseEmbedding(4, 1 << 20, "sum").to(device)
+    ids = torch.tensor([[1, 2, -1]], device=device)
+    rows = se.bag.weight.detach()
+    assert torch.equal(se(ids)[0], rows[1] + rows[2])
+
+
 # -------------------------------- serving ---------------------------------
 @pytest.mark.parametrize("device", DEVICES)
 def test_serving_runner_in_fp8(device):
