@@ -83,6 +83,13 @@ int type_code(torch::ScalarType t, const char* name) {
   }
 }
 
+// what stands for a tensor (a traced call's, a subclass's) has no memory, and
+// a kernel would read from address 0
+void check_memory(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.numel() == 0 || t.data_ptr() != nullptr, name,
+              " has no memory of its own");
+}
+
 // the largest load of neighbours, up to 16 bytes, that every row allows
 int vec_of(const Tensor& t, int64_t d, int64_t row_stride) {
   const int64_t size = t.element_size();
@@ -254,6 +261,7 @@ class Lookup : public torch::autograd::Function<Lookup> {
     const int64_t need = ctx->saved_data["need"].toInt();
     torch::autograd::variable_list out(6);
     if (!grads[0].defined()) return out;
+    check_memory(grads[0], "gradient");
     {
       at::NoGradGuard none;
       run(grads[0].contiguous(), saved[0], saved[1], saved[2], saved[3],
@@ -375,7 +383,10 @@ Tensor embedding_lookup(const Tensor& table_, const Tensor& ids,
                           weights->device() == ids.device(),
                       "weights must have the ids' shape and device");
     check_type(*weights, "weights");
+    check_memory(*weights, "weights");
   }
+  check_memory(table, "table");
+  check_memory(ids, "ids");
   if (table.size(1) > 1 && table.stride(1) != 1) table = table.contiguous();
   Tensor out = Lookup::apply(table, weights, ids, combiner, scale,
                              at::GradMode::is_enabled());
@@ -397,6 +408,8 @@ std::vector<Tensor> coalesce_rows(Tensor values, Tensor ids) {
               "values must be contiguous [ids, dim]");
   const int64_t n = ids.size(0), d = values.size(1);
   TORCH_CHECK(n < kMost, "too many ids: ", n);
+  check_memory(values, "values");
+  check_memory(ids, "ids");
   c10::DeviceGuard guard(ids.device());
   TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() ==
                   c10::hip::CaptureStatus::None,

@@ -53,6 +53,13 @@ int type_code(torch::ScalarType t, const char* name) {
   }
 }
 
+// what stands for a tensor (a traced call's, a subclass's) has no memory, and
+// a kernel would read from address 0
+void check_memory(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.numel() == 0 || t.data_ptr() != nullptr, name,
+              " has no memory of its own");
+}
+
 bool aligned(const Tensor& t, int64_t row_stride) {
   return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
          row_stride * t.element_size() % 16 == 0;
@@ -234,6 +241,7 @@ std::vector<OptTensor> fp8_quantize(Tensor x, bool tile, bool rows,
   TORCH_CHECK(x.size(0) < (1 << 24) - 128 || !cols,
               "x has too many rows to be transposed: ", x.size(0));
   TORCH_CHECK(rows || cols, "nothing asked for");
+  check_memory(x, "x");
   c10::DeviceGuard guard(x.device());
   x = row_major(x);
   edl_fp8_quant a = quant_of(x, "x");
@@ -270,12 +278,14 @@ void check_layer(const Tensor& x, int64_t n, int64_t k, c10::Device w_device,
   TORCH_CHECK_VALUE(w_device == x.device(), "x is on ", x.device(),
                     ", and the weight on ", w_device);
   TORCH_CHECK_VALUE(n > 0, "the weight has no rows");
+  check_memory(x, "x");
   if (!bias.defined()) return;
   TORCH_CHECK_VALUE(bias.dim() == 1 && bias.size(0) == n, "bias is ",
                     bias.sizes(), ", not (", n, ")");
   check_type(bias, "bias");
   TORCH_CHECK_VALUE(bias.device() == x.device(), "x is on ", x.device(),
                     ", and the bias on ", bias.device());
+  check_memory(bias, "bias");
 }
 Tensor rows_of(const Tensor& x) {
   return row_major(x.dim() == 2 ? x : x.reshape({-1, x.size(-1)}));
@@ -375,6 +385,7 @@ class Fp8Dense : public torch::autograd::Function<Fp8Dense> {
     const int64_t b_type = ctx->saved_data["b"].toInt();
     torch::autograd::variable_list out(5);
     if (!grads[0].defined()) return out;
+    check_memory(grads[0], "gradient");
     {
       at::NoGradGuard none;
       run(saved[0], saved[1], need, grads[0],
@@ -487,6 +498,7 @@ Tensor fp8_dense(const Tensor& x, const Tensor& w, const OptTensor& bias_,
                     w.dim());
   check_type(w, "w");
   TORCH_CHECK_VALUE(w.size(1) > 0, "w has no columns");
+  check_memory(w, "w");
   check_layer(x, w.size(0), w.size(1), w.device(), bias);
   return shaped_like(
       Fp8Dense::apply(rows_of(x), w, bias_, act, at::GradMode::is_enabled()),
@@ -499,6 +511,8 @@ Tensor fp8_dense_frozen(const Tensor& x, const Tensor& wq, const Tensor& ws,
   Tensor bias = bias_.has_value() ? *bias_ : Tensor();
   const int64_t n = wq.size(0);
   check_layer(x, n, k, wq.device(), bias);
+  check_memory(wq, "weight");
+  check_memory(ws, "weight");
   TORCH_CHECK(!at::GradMode::is_enabled() ||
                   !(x.requires_grad() ||
                     (bias.defined() && bias.requires_grad())),

@@ -12,6 +12,7 @@ import pytest
 import torch
 
 from elasticdl_amd.common.tensor_utils import deduplicate_indexed_slices
+from elasticdl_amd.ops import native_available, require_native
 from elasticdl_amd.ops.embedding import coalesce_rows, embedding_lookup
 
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
@@ -495,6 +496,32 @@ def test_refusals():
         embedding_lookup(table, ids, torch.ones(2, 3).double(), "sum")
     with pytest.raises(ValueError, match="GPU"):
         coalesce_rows(table, ids[0])
+
+
+class Elsewhere(torch.Tensor):
+    """Stands for a tensor on a GPU, without memory of its own."""
+
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_wrapper_subclass(
+            cls, t.shape, dtype=t.dtype, device="cuda:0")
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise RuntimeError(f"{func} is not what is tested")
+
+
+@pytest.mark.skipif(not native_available(), reason="needs the extension")
+def test_tensors_without_memory_are_refused():
+    """Before a kernel would read from address 0; no GPU takes part."""
+    table, ids = Elsewhere(randn(5, 4)), Elsewhere(torch.zeros(2, 3).long())
+    weights = Elsewhere(randn(2, 3))
+    for args in ((table, ids), (table, ids, weights, "sum")):
+        with pytest.raises(RuntimeError, match="no memory"):
+            embedding_lookup(*args)
+    with pytest.raises(RuntimeError, match="no memory"):
+        require_native().coalesce_rows(Elsewhere(randn(3, 4)),
+                                       Elsewhere(torch.zeros(3).long()))
 
 
 @pytest.mark.gpu

@@ -14,8 +14,14 @@ import threading
 import pytest
 import torch
 
-from elasticdl_amd.ops import fp8, reference
+from elasticdl_amd.ops import (
+    fp8,
+    native_available,
+    reference,
+    require_native,
+)
 from elasticdl_amd.ops.fp8 import fp8_dense, quantize_fp8, quantize_fp8_weight
+from test_embedding_ops import Elsewhere
 
 TYPES = [torch.float32, torch.bfloat16, torch.float16]
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
@@ -643,6 +649,17 @@ def test_refusals():
     with pytest.raises(RuntimeError):
         g.sum().backward()
     assert repr(fp8.quantize_fp8(x)).startswith("Fp8Blocks")
+
+
+@pytest.mark.skipif(not native_available(), reason="needs the extension")
+def test_tensors_without_memory_are_refused():
+    x, w, b = (Elsewhere(randn(*s)) for s in ((4, 32), (8, 32), (8,)))
+    frozen = quantize_fp8_weight(randn(8, 32))
+    frozen = fp8.Fp8Blocks(Elsewhere(frozen.data), Elsewhere(frozen.scale), 32)
+    for call in (lambda: fp8_dense(x, w, b), lambda: fp8_dense(x, frozen),
+                 lambda: require_native().fp8_quantize(x, False, True, False)):
+        with pytest.raises(RuntimeError, match="no memory"):
+            call()
 
 
 @pytest.mark.gpu
