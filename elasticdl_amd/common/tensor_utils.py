@@ -47,18 +47,23 @@ def deduplicate_indexed_slices(
     (common/tensor_utils.py:39-60): unique ids in sorted order, gradient
     rows summed per id. On a GPU the sorted segmented sum of
     ``ops.embedding.coalesce_rows``, whose order of addition (and so its
-    bits) the inputs alone decide; else, and where the rows need a gradient,
-    vectorized via sort + index_add (no Python loop).
+    bits) the inputs alone decide; else, where the rows need a gradient, and
+    where torch traces or transforms the call, vectorized via sort + index_add
+    (no Python loop).
     """
     ids = ids.to(torch.int64)
-    if (values.is_cuda and ids.device == values.device
-            and values.dim() == 2 and ids.dim() == 1
-            and ids.numel() < 2 ** 31 - 8192 and values.shape[1] < 2 ** 20
-            and values.dtype in (torch.float32, torch.bfloat16, torch.float16)
-            and not (torch.is_grad_enabled() and values.requires_grad)):
+    if values.is_cuda:
+        from elasticdl_amd.ops import reads_directly
         from elasticdl_amd.ops.embedding import coalesce_rows
 
-        return coalesce_rows(values, ids)
+        if (reads_directly(values, ids) and ids.device == values.device
+                and values.dim() == 2 and ids.dim() == 1
+                and ids.numel() < 2 ** 31 - 8192
+                and values.shape[1] < 2 ** 20
+                and values.dtype in (torch.float32, torch.bfloat16,
+                                     torch.float16)
+                and not (torch.is_grad_enabled() and values.requires_grad)):
+            return coalesce_rows(values, ids)
     unique_ids, inverse = torch.unique(ids, sorted=True, return_inverse=True)
     summed = torch.zeros(
         (unique_ids.numel(), values.shape[1]),

@@ -432,6 +432,22 @@ def test_deduplicate_keeps_a_gradient_where_one_is_asked_for():
         assert not deduplicate_indexed_slices(values, ids)[0].requires_grad
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_deduplicate_under_transforms(device):
+    """Tracing and torch.func see torch's own operators."""
+    values = torch.arange(1.0, 13.0).view(6, 2).to(device)
+    ids = torch.tensor([4, 1, 4, 0, 1, 4], device=device)
+    other = torch.tensor([2, 2, 2, 7, 2, 3], device=device)
+    traced = torch.jit.trace(deduplicate_indexed_slices, (values, ids))
+    for a, b in zip(traced(values * 2, other),
+                    deduplicate_indexed_slices(values * 2, other)):
+        assert torch.equal(a, b)
+    weight = torch.tensor([[1.0], [2.0], [3.0]], device=device)
+    g = torch.func.grad(lambda v: (
+        deduplicate_indexed_slices(v, ids)[0] * weight).sum())(values)
+    assert torch.equal(g[:, 0].cpu(), torch.tensor([3.0, 2, 3, 1, 2, 3]))
+
+
 @pytest.mark.gpu
 def test_coalesce_of_strided_values():
     base = randn(100, 20).cuda()
