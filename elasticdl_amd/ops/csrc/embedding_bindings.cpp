@@ -423,8 +423,7 @@ std::vector<Tensor> coalesce_rows(Tensor values, Tensor ids) {
   int64_t* ids_out = unique.data_ptr<int64_t>();
   const int64_t* id = ids.data_ptr<int64_t>();
   // what the host reads, in memory that the kernels write to directly: how
-  // many ids, whether they lie too far apart for the small sort, and
-  // their smallest and largest by parts
+  // many ids, and their smallest and largest by parts
   const Tensor host =
       torch::empty({1 + 2 * EDL_RANGE_PARTS},
                    torch::TensorOptions().dtype(torch::kInt64).pinned_memory(
@@ -478,12 +477,9 @@ std::vector<Tensor> coalesce_rows(Tensor values, Tensor ids) {
     small.into(s);
     if (early) sum_into(n);
     wait();
-    if (found_at[1] == 0) {
-      found = found_at[0];
-      if (!early) sum_into(found);
-      return {rows.narrow(0, 0, found), unique.narrow(0, 0, found)};
-    }
-    s.starts = s.runs = nullptr;  // too far apart
+    found = found_at[0];
+    if (!early) sum_into(found);
+    return {rows.narrow(0, 0, found), unique.narrow(0, 0, found)};
   }
   uint32_t* place = nullptr;
   Pieces pieces;

@@ -17,6 +17,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <type_traits>
 
 #include "embedding_kernels.h"
 
@@ -506,27 +507,63 @@ __global__ __launch_bounds__(256) void sort_move_kernel(
 // of each wave for each share those that they are compared with.
 //
 // IDS: ids of any value, less 2^31 below the first, which goes to info[0];
-// info[1]: some lie too far from it for 32 bits, and nothing is done. The
-// difference wraps at 2^64, so that ids at one end of int64 look near to the
-// other's: their order and the keys' disagree, which is too far as well.
+// info[1]: some lie too far from it for 32 bits, and all are compared in 64
+// (8192 ids in 15 us, 13.5 in 32 bits; the whole call 48 us and 38, and 144
+// where they went to the radix sort). The difference wraps at 2^64, so that
+// ids at one end of int64 look near to the other's: their order and the keys'
+// disagree, which is too far as well.
 // Else rows of a table.
 constexpr int kSmallThreads = 1024;
 constexpr int kSmallItems = EDL_SORT_SMALL / kSmallThreads;
 constexpr int kSmallWaves = kSmallThreads / 64;
 constexpr int kSmallTile = 32, kSmallShares = kSmallThreads / kSmallTile;
 
+// how many keys of places j0 to j1 come before the one at `place`
+template <typename K>
+__device__ inline uint32_t rank_among(const K* s_key, int place, int j0,
+                                      int j1) {
+  typedef K k4 __attribute__((ext_vector_type(4), aligned(16)));
+  const int tile0 = place / kSmallTile * kSmallTile, tile1 = tile0 + kSmallTile;
+  const K key = s_key[place];
+  uint32_t rank = 0;
+  const auto four = [&](int j) {
+    return *reinterpret_cast<const k4*>(s_key + j);
+  };
+#pragma unroll 4
+  for (int j = j0; j < min(j1, tile0); j += 4) {  // equal ones come before
+    const k4 o = four(j);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) rank += o[q] <= key;
+  }
+  for (int j = max(j0, tile0); j < min(j1, tile1); j += 4) {
+    const k4 o = four(j);
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      rank += o[q] < key || (o[q] == key && j + q < place);
+  }
+#pragma unroll 4
+  for (int j = max(j0, tile1); j < j1; j += 4) {  // and behind
+    const k4 o = four(j);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) rank += o[q] < key;
+  }
+  return rank;
+}
+
 template <typename S, bool IDS>
 __global__ __launch_bounds__(kSmallThreads) void rank_small_kernel(
     S src, int N, uint32_t* keys_out, uint32_t* pos_out, int64_t* info,
     int tiles, Zeros zeros) {
-  __shared__ __align__(16) uint32_t s_key[EDL_SORT_SMALL];
+  __shared__ __align__(16) uint64_t s_room[EDL_SORT_SMALL / (IDS ? 1 : 2)];
   __shared__ uint32_t s_rank[kSmallShares][kSmallTile];
+  uint32_t* s_key = reinterpret_cast<uint32_t*>(s_room);
   if ((int)blockIdx.x >= tiles)
     return fill_zeros<kSmallThreads>(zeros, blockIdx.x - tiles,
                                      gridDim.x - tiles);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x;
   const int all = (N + 4 * kSmallShares - 1) / (4 * kSmallShares) *
                   (4 * kSmallShares);
+  bool far = false;
   if constexpr (IDS) {
     const int64_t first = src.ids[0];
     const uint64_t low = (uint64_t)first - 0x80000000ull;
@@ -539,12 +576,20 @@ __global__ __launch_bounds__(kSmallThreads) void rank_small_kernel(
       off |= (uint32_t)(rel >> 32) | ((id < first) != (rel < 0x80000000ull));
       if (i < all) s_key[i] = i < N ? (uint32_t)rel : kNone;
     }
-    const bool far = __syncthreads_or(off != 0);
+    far = __syncthreads_or(off != 0);  // all alike
     if (blockIdx.x == 0 && tid == 0) {
       info[0] = (int64_t)low;
       info[1] = far;
     }
-    if (far) return;  // all alike
+    if (far) {
+#pragma unroll
+      for (int k = 0; k < kSmallItems; ++k) {
+        const int i = k * kSmallThreads + tid;
+        if (i < all)
+          s_room[i] = i < N ? (uint64_t)src.ids[i] ^ 0x8000000000000000ull
+                            : ~0ull;
+      }
+    }
   } else {
 #pragma unroll
     for (int k = 0; k < kSmallItems; ++k) {
@@ -554,67 +599,51 @@ __global__ __launch_bounds__(kSmallThreads) void rank_small_kernel(
   }
   __syncthreads();
   const int item = tid & (kSmallTile - 1), which = tid / kSmallTile;
-  const int tile0 = (int)blockIdx.x * kSmallTile, tile1 = tile0 + kSmallTile;
-  const uint32_t key = s_key[tile0 + item];
+  const int place = (int)blockIdx.x * kSmallTile + item;
   const int share = all / kSmallShares, j0 = which * share, j1 = j0 + share;
-  uint32_t rank = 0;
-  const auto four = [&](int j) {
-    return *reinterpret_cast<const u32x4*>(s_key + j);
-  };
-#pragma unroll 4
-  for (int j = j0; j < min(j1, tile0); j += 4) {  // equal ones come before
-    const u32x4 o = four(j);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) rank += o[q] <= key;
-  }
-  for (int j = max(j0, tile0); j < min(j1, tile1); j += 4) {
-    const u32x4 o = four(j);
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      rank += o[q] < key || (o[q] == key && j + q < tile0 + item);
-  }
-#pragma unroll 4
-  for (int j = max(j0, tile1); j < j1; j += 4) {  // and behind
-    const u32x4 o = four(j);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) rank += o[q] < key;
-  }
+  uint32_t rank = far ? rank_among(s_room, place, j0, j1)
+                      : rank_among(s_key, place, j0, j1);
   s_rank[which][item] = rank;
   __syncthreads();
-  if (tid >= kSmallTile || tile0 + item >= N) return;
+  if (tid >= kSmallTile || place >= N) return;
   for (int w = 1; w < kSmallShares; ++w) rank += s_rank[w][item];
-  keys_out[rank] = key;
-  pos_out[rank] = tile0 + item;
+  if (!far) keys_out[rank] = s_key[place];
+  pos_out[rank] = place;
 }
 
 // Where each run of the small sort's equal keys starts, and how many there
-// are (runs[0]). IDS: the runs' ids go to `unique`, and for the host how many
-// there are (found[0]), or that there is nothing (found[1], info[1]). Else
-// the runs' rows go to `rows`.
+// are (runs[0]). IDS: the runs' ids go to `unique`, and how many there are to
+// found[0], for the host. Ids that lie far apart have no keys: they are read
+// where the sort took them from. Else the runs' rows go to `rows`.
 template <bool IDS>
 __global__ __launch_bounds__(kSmallThreads) void runs_small_kernel(
     const uint32_t* __restrict__ keys, int N, const int64_t* info,
+    const int64_t* __restrict__ ids, const uint32_t* __restrict__ pos,
     uint32_t* starts, uint32_t* runs, uint32_t* rows, int64_t* unique,
     uint32_t* found) {
+  typedef typename std::conditional<IDS, uint64_t, uint32_t>::type K;
   __shared__ uint32_t s_count[kSmallWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  bool far = false;
+  uint64_t low = 0;
   if constexpr (IDS) {
-    const bool far = info[1] != 0;
-    if (tid == 0) found[1] = far;
-    if (far) {  // all threads alike
-      if (tid == 0) runs[0] = 0;
-      return;
-    }
+    far = info[1] != 0;  // all threads alike
+    low = far ? 0 : (uint64_t)info[0];
   }
   const int items = (N + kSmallThreads - 1) / kSmallThreads;
   const int i0 = wave * items * 64 + lane;
-  uint32_t key[kSmallItems], last[kSmallItems];
+  K key[kSmallItems], last[kSmallItems];
 #pragma unroll
   for (int k = 0; k < kSmallItems; ++k) {
     const int i = i0 + k * 64;
     const bool in = k < items && i < N;
-    key[k] = in ? keys[i] : 0;
-    last[k] = in && i > 0 ? keys[i - 1] : 0;
+    if (IDS && far) {
+      key[k] = in ? ids[pos[i]] : 0;
+      last[k] = in && i > 0 ? ids[pos[i - 1]] : 0;
+    } else {
+      key[k] = in ? keys[i] : 0;
+      last[k] = in && i > 0 ? keys[i - 1] : 0;
+    }
   }
   uint32_t here = 0, place[kSmallItems];
   bool first[kSmallItems];
@@ -645,7 +674,7 @@ __global__ __launch_bounds__(kSmallThreads) void runs_small_kernel(
       const uint32_t at = before + place[k];
       starts[at] = i0 + k * 64;
       if constexpr (IDS)
-        unique[at] = (int64_t)((uint64_t)info[0] + (uint64_t)key[k]);
+        unique[at] = (int64_t)(low + key[k]);
       else
         rows[at] = key[k];
     }
@@ -1266,7 +1295,8 @@ extern "C" int edl_sort_rows_small(const void* ids, int ids64, int64_t V,
           Keys32{ids, ids64 != 0, V}, (int)N, keys, pos, nullptr, tiles,
           Zeros{static_cast<uint8_t*>(zeros), zero_bytes});
   runs_small_kernel<false><<<1, kSmallThreads, 0, st>>>(
-      keys, (int)N, nullptr, starts, runs, rows, nullptr, nullptr);
+      keys, (int)N, nullptr, nullptr, nullptr, starts, runs, rows, nullptr,
+      nullptr);
   return (int)hipGetLastError();
 }
 extern "C" int edl_sort_ids_small(const int64_t* ids, int64_t N,
@@ -1278,7 +1308,7 @@ extern "C" int edl_sort_ids_small(const int64_t* ids, int64_t N,
   rank_small_kernel<Keys32Of, true><<<tiles, kSmallThreads, 0, st>>>(
       Keys32Of{ids}, (int)N, keys, pos, info, tiles, Zeros{});
   runs_small_kernel<true><<<1, kSmallThreads, 0, st>>>(
-      keys, (int)N, info, starts, runs, nullptr, unique, found);
+      keys, (int)N, info, ids, pos, starts, runs, nullptr, unique, found);
   return (int)hipGetLastError();
 }
 

@@ -421,6 +421,23 @@ def test_deduplicate_at_the_ends_of_int64(ids, times, device):
     assert torch.equal(rows.cpu(), sums)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n", [2, 31, 33, 1024, 4095, 8191, 8192])
+def test_deduplicate_of_few_ids_far_apart(n, device):
+    known = torch.cat([torch.randint(LOW, HIGH, (n // 3 + 1,), generator=gen(n)),
+                       torch.tensor([LOW, HIGH, 0, -1, 1 << 32, 1 << 31])])
+    at = torch.randint(0, len(known), (n,), generator=gen(n + 1))
+    at[torch.rand(n, generator=gen(n + 2)) < 0.3] = 0  # one of them often
+    values = torch.randint(-8, 9, (n, 3), generator=gen(n + 3)).float()
+    rows, unique = deduplicate_indexed_slices(values.to(device),
+                                              known[at].to(device))
+    want, place = torch.unique(known[at], return_inverse=True)
+    assert torch.equal(unique.cpu(), want)
+    # whole numbers below 2^24: every sum is exact
+    sums = torch.zeros(want.numel(), 3).index_add_(0, place, values)
+    assert torch.equal(rows.cpu(), sums)
+
+
 @pytest.mark.gpu
 def test_deduplicate_keeps_a_gradient_where_one_is_asked_for():
     values = randn(50, 3).cuda().requires_grad_(True)
