@@ -6,6 +6,8 @@ The built elasticdl_amd/ops/_C*.so travels with the repo snapshot to GPU
 boxes (it is git-ignored but not gpurun-ignored).
 """
 
+import glob
+import hashlib
 import os
 
 from setuptools import find_packages, setup
@@ -15,6 +17,15 @@ os.environ.setdefault("PYTORCH_ROCM_ARCH", "gfx950")
 from torch.utils.cpp_extension import BuildExtension, CUDAExtension  # noqa: E402
 
 ROOT = os.path.dirname(os.path.abspath(__file__))
+
+# ninja follows a source's headers only where the compiler lists them, which
+# it does not for HIP: a flag that changes with them makes it compile again
+HEADERS = hashlib.sha256()
+for header in sorted(glob.glob(
+        os.path.join(ROOT, "elasticdl_amd", "ops", "csrc", "*.h"))):
+    with open(header, "rb") as f:
+        HEADERS.update(f.read())
+HEADERS = "-DEDL_HEADERS=0x" + HEADERS.hexdigest()[:16]
 
 ext = CUDAExtension(
     name="elasticdl_amd.ops._C",
@@ -30,10 +41,10 @@ ext = CUDAExtension(
         "elasticdl_amd/ops/csrc/embedding_kernels.hip",
     ],
     extra_compile_args={
-        "cxx": ["-O3", "-std=c++17"],
+        "cxx": ["-O3", "-std=c++17", HEADERS],
         # no packed 32-bit float instructions: some forms of them have given
         # wrong results on this hardware
-        "nvcc": ["-O3", "-std=c++17", "-Xclang", "-target-feature",
+        "nvcc": ["-O3", "-std=c++17", HEADERS, "-Xclang", "-target-feature",
                  "-Xclang", "-packed-fp32-ops"],
     },
 )
