@@ -57,3 +57,4 @@ struct edl_segments {
 #define EDL_SORT_TILE 4096
 #define EDL_SORT_BINS 2048  // most of a pass
 #define EDL_SORT_SMALL 8192
+#define EDL_SORT_FAR (192 * 1024)

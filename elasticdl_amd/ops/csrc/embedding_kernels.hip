@@ -519,11 +519,11 @@ constexpr int kSmallWaves = kSmallThreads / 64;
 constexpr int kSmallTile = 32, kSmallShares = kSmallThreads / kSmallTile;
 
 // how many keys of places j0 to j1 come before the one at `place`
-template <typename K>
+template <typename K, int kTile = kSmallTile>
 __device__ inline uint32_t rank_among(const K* s_key, int place, int j0,
                                       int j1) {
   typedef K k4 __attribute__((ext_vector_type(4), aligned(16)));
-  const int tile0 = place / kSmallTile * kSmallTile, tile1 = tile0 + kSmallTile;
+  const int tile0 = place / kTile * kTile, tile1 = tile0 + kTile;
   const K key = s_key[place];
   uint32_t rank = 0;
   const auto four = [&](int j) {
@@ -679,6 +679,85 @@ __global__ __launch_bounds__(kSmallThreads) void runs_small_kernel(
         rows[at] = key[k];
     }
   }
+}
+
+// Ids over more than 32 bits, up to EDL_SORT_FAR of them. Six passes of the
+// radix sort wait for their 18 launches. So chunks of 2048 are sorted as above,
+// all at once, and an id's place is the one in its chunk and, for each of the
+// other chunks, how many of its ids come before, found by bisection. That grows
+// with the square of their number (whole calls by chunks and by passes: 8193
+// ids 70 us and 128, 50 thousand 79 and 137, 160 thousand 134 and 154, 200
+// thousand 162 and 160).
+constexpr int kChunk = 2048, kChunkTile = 128, kChunkGroup = 8;
+constexpr int kChunkShares = kSmallThreads / kChunkTile;
+
+__global__ __launch_bounds__(kSmallThreads) void chunk_rank_kernel(
+    Keys64 src, int N, uint64_t* __restrict__ keys, uint32_t* __restrict__ pos,
+    uint32_t* __restrict__ place) {
+  __shared__ __align__(16) uint64_t s_key[kChunk];
+  __shared__ uint32_t s_rank[kChunkShares][kChunkTile];
+  const int tid = threadIdx.x;
+  constexpr int kTiles = kChunk / kChunkTile;
+  const int chunk0 = (int)blockIdx.x / kTiles * kChunk;
+#pragma unroll
+  for (int i = tid; i < kChunk; i += kSmallThreads)
+    s_key[i] = chunk0 + i < N ? src(chunk0 + i) : ~0ull;
+  __syncthreads();
+  const int item = tid % kChunkTile, which = tid / kChunkTile;
+  const int at = (int)blockIdx.x % kTiles * kChunkTile + item;
+  constexpr int kShare = kChunk / kChunkShares;
+  uint32_t rank = rank_among<uint64_t, kChunkTile>(
+      s_key, at, which * kShare, (which + 1) * kShare);
+  s_rank[which][item] = rank;
+  __syncthreads();
+  if (tid >= kChunkTile || chunk0 + at >= N) return;
+#pragma unroll
+  for (int w = 1; w < kChunkShares; ++w) rank += s_rank[w][item];
+  keys[chunk0 + rank] = s_key[at];
+  pos[chunk0 + rank] = chunk0 + at;
+  place[chunk0 + rank] = rank;
+}
+
+// places among kChunkGroup chunks, added to those so far: whole numbers, whose
+// sum does not depend on the order
+__global__ __launch_bounds__(kSmallThreads) void chunk_merge_kernel(
+    const uint64_t* __restrict__ keys, int N, uint32_t* place) {
+  __shared__ uint64_t s_key[kChunk];
+  const int i = (int)blockIdx.x * kSmallThreads + threadIdx.x;
+  const int own = (int)blockIdx.x * kSmallThreads / kChunk;
+  const int chunks = (N + kChunk - 1) / kChunk;
+  const int c0 = (int)blockIdx.y * kChunkGroup;
+  const uint64_t key = i < N ? keys[i] : 0;
+  uint32_t before = 0;
+  for (int c = c0; c < c0 + kChunkGroup && c < chunks; ++c) {
+    if (c == own) continue;  // the workgroup alike
+    __syncthreads();
+#pragma unroll
+    for (int k = threadIdx.x; k < kChunk; k += kSmallThreads)
+      s_key[k] = c * kChunk + k < N ? keys[c * kChunk + k] : ~0ull;
+    __syncthreads();
+    const bool first = c < own;  // equal ones of chunks before come before
+    int at = 0;
+#pragma unroll
+    for (int step = kChunk / 2; step > 0; step /= 2) {
+      const uint64_t o = s_key[at + step - 1];
+      if (o < key || (first && o == key)) at += step;
+    }
+    const uint64_t o = s_key[at];
+    before += at + (o < key || (first && o == key));
+  }
+  if (i < N && before) atomicAdd(place + i, before);
+}
+
+__global__ __launch_bounds__(256) void chunk_move_kernel(
+    const uint64_t* __restrict__ keys, const uint32_t* __restrict__ pos,
+    const uint32_t* __restrict__ place, int N, uint64_t* __restrict__ keys_out,
+    uint32_t* __restrict__ pos_out) {
+  const int i = (int)blockIdx.x * 256 + threadIdx.x;
+  if (i >= N) return;
+  const uint32_t to = place[i];
+  keys_out[to] = keys[i];
+  pos_out[to] = pos[i];
 }
 
 // each workgroup's smallest and largest of ids, for the host: no atomics,
@@ -1347,7 +1426,20 @@ extern "C" int edl_sort_ids64(const int64_t* ids, int64_t N,
                               uint64_t* const* keys, uint32_t* const* pos,
                               uint32_t* counts, uint32_t* totals,
                               hipStream_t st) {
-  return sort_all(Keys64{ids}, N, 64, keys, pos, counts, totals, st);
+  if (N > EDL_SORT_FAR)
+    return sort_all(Keys64{ids}, N, 64, keys, pos, counts, totals, st);
+  static_assert(EDL_SORT_FAR < 256 * 1024, "counts have room for the places");
+  const int n = (int)N, chunks = (n + kChunk - 1) / kChunk;
+  uint32_t* place = counts;
+  chunk_rank_kernel<<<(n + kChunkTile - 1) / kChunkTile, kSmallThreads, 0,
+                      st>>>(Keys64{ids}, n, keys[0], pos[0], place);
+  chunk_merge_kernel<<<dim3((n + kSmallThreads - 1) / kSmallThreads,
+                            (chunks + kChunkGroup - 1) / kChunkGroup),
+                       kSmallThreads, 0, st>>>(keys[0], n, place);
+  chunk_move_kernel<<<(n + 255) / 256, 256, 0, st>>>(keys[0], pos[0], place, n,
+                                                     keys[1], pos[1]);
+  const int rc = (int)hipGetLastError();
+  return rc ? -1 - rc : 1;
 }
 
 extern "C" int edl_unique32(const uint32_t* keys, int64_t N, uint32_t* counts,

@@ -438,6 +438,42 @@ def test_deduplicate_of_few_ids_far_apart(n, device):
     assert torch.equal(rows.cpu(), sums)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n", [8193, 10240, 12289, 65536, 100_001, 196_608,
+                               196_609, 250_000])
+@pytest.mark.parametrize("known", [2, 700, 100_000])
+def test_deduplicate_of_many_ids_far_apart(n, known, device):
+    """Chunks that are merged, whole and not, and behind them all 64 bits."""
+    known = torch.randint(LOW, HIGH, (known,), generator=gen(known))
+    known[:2] = torch.tensor([LOW, HIGH])
+    at = torch.randint(0, len(known), (n,), generator=gen(n))
+    at[torch.rand(n, generator=gen(n + 1)) < 0.2] = 1  # the last, often
+    values = torch.randint(-8, 9, (n, 3), generator=gen(n + 2)).float()
+    rows, unique = deduplicate_indexed_slices(values.to(device),
+                                              known[at].to(device))
+    want, place = torch.unique(known[at], return_inverse=True)
+    assert torch.equal(unique.cpu(), want)
+    # whole numbers below 2^24: every sum is exact
+    sums = torch.zeros(want.numel(), 3).index_add_(0, place, values)
+    assert torch.equal(rows.cpu(), sums)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [8192, 50_000])
+def test_sums_of_ids_far_apart_have_the_same_bits_each_time(n):
+    ids = torch.randint(LOW, HIGH, (n // 9,), generator=gen(0)).cuda()
+    ids = ids[torch.randint(0, n // 9, (n,), generator=gen(1)).cuda()]
+    values = randn(n, 5, seed=2).cuda()
+    want = coalesce_rows(values, ids)
+    # the order of equal ids is theirs: near ids with the same order agree
+    near = torch.unique(ids, return_inverse=True)[1]
+    same = coalesce_rows(values, near)
+    assert torch.equal(want[0], same[0])
+    for _ in range(5):
+        for a, b in zip(coalesce_rows(values, ids), want):
+            assert torch.equal(a, b)
+
+
 @pytest.mark.gpu
 def test_deduplicate_keeps_a_gradient_where_one_is_asked_for():
     values = randn(50, 3).cuda().requires_grad_(True)
