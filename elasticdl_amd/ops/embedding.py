@@ -55,10 +55,13 @@ def embedding_lookup(table: torch.Tensor, ids: torch.Tensor,
     output is NaN and it has no gradient.
 
     ``weights`` [bags, length] multiply each id's row; the mean's and
-    sqrtn's divisor counts ids, not weights. The result has the table's type
-    (float32, bfloat16 or float16), rounded once from a sum in 32 bits. The
-    table's gradient is dense, in the table's type; weights have one too.
-    Rows of the table may be strided; ids are fewer than 2^31 - 4096.
+    sqrtn's divisor counts ids, not weights. (tf.nn.embedding_lookup_sparse
+    divides by the weights' sum and the root of their squares' sum: for its
+    results divide the weights by these first and take "sum".) The result has
+    the table's type (float32, bfloat16 or float16), rounded once from a sum
+    in 32 bits. The table's gradient is dense, in the table's type; weights
+    have one too. Rows of the table may be strided; ids are fewer than
+    2^31 - 4096.
 
     In code that is captured into a graph, take gradients with
     ``torch.autograd.grad`` (or drop eager graphs of the same leaves first):

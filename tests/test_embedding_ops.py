@@ -154,6 +154,39 @@ def test_no_ids(combiner, device):
         assert g.shape == (6, 4) and not g.any()
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("combiner", ["mean", "sqrtn"])
+def test_weighted_norms_count_ids_and_weights_divide_before(combiner, device):
+    """The documented way to norms by weights, with their gradient's term."""
+    t = randn(9, 5, seed=1).to(device)
+    ids = torch.tensor([[1, 4, 7, 4], [2, -1, -1, -1]], device=device)
+    w = (torch.rand(2, 4, generator=gen(2)) + 0.5).to(device)
+    live = ids >= 0
+    n = live.sum(1, keepdim=True).float()
+    want = torch.where(live.unsqueeze(2), t[ids.clamp(min=0)]
+                       * w.unsqueeze(2), 0.0).sum(1)
+    want = want / (n if combiner == "mean" else n.sqrt())
+    got = embedding_lookup(t, ids, w, combiner)
+    assert torch.allclose(got, want, rtol=1e-6, atol=1e-6)
+
+    def normed(w):
+        w = torch.where(live, w, 0.0)
+        sums = w if combiner == "mean" else w.square()
+        norm = sums.sum(1, keepdim=True)
+        return w / (norm if combiner == "mean" else norm.sqrt())
+
+    w.requires_grad_(True)
+    a = embedding_lookup(t, ids, normed(w), "sum")
+    b = (t[ids.clamp(min=0)].double() * normed(w.double()).unsqueeze(2)).sum(1)
+    # a few roundings of 2^-24 of sums of at most 4 terms of size 3
+    assert torch.allclose(a.double(), b, rtol=0, atol=64 * 2.0 ** -24)
+    ga, = torch.autograd.grad(a.square().sum(), w)
+    gb, = torch.autograd.grad(b.square().sum(), w)
+    # 5 columns of products of such, and a quotient's two terms
+    assert torch.allclose(ga, gb.float(), rtol=0, atol=2048 * 2.0 ** -24)
+
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("bags", [2, 20000])
 def test_ids_past_the_table_show_and_reach_nothing(bags):
