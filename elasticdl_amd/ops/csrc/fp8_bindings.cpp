@@ -30,7 +30,9 @@ namespace {
 using torch::Tensor;
 using OptTensor = c10::optional<Tensor>;
 
-constexpr int64_t kFewRows = 16;
+// rows that take one launch, and the outputs from which on it would have 2^32
+// threads, 64 to each
+constexpr int64_t kFewRows = 16, kFewOutputs = 1 << 26;
 
 int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
@@ -533,7 +535,7 @@ Tensor fp8_dense_frozen(const Tensor& x, const Tensor& wq, const Tensor& ws,
   bias_into(f.g[0], bias);
   if (m > 0) {
     edl_fp8_quant a = quant_of(x2, "x");
-    if (m <= kFewRows) {
+    if (m <= kFewRows && n < kFewOutputs) {
       Fp8Dense::few_rows(x2, a, f.g[0]);
     } else {
       Pieces passing;

@@ -556,6 +556,16 @@ def test_gradients_of_more_rows_than_can_be_transposed():
 
 
 @pytest.mark.gpu
+def test_one_row_of_more_outputs_than_a_launch_has_threads_for():
+    n = 1 << 26
+    w = (torch.arange(n, device="cuda") % 17 - 8).bfloat16().view(n, 1)
+    x = torch.full((1, 1), 3.0, device="cuda", dtype=torch.bfloat16)
+    with torch.no_grad():  # whole numbers: exact
+        y = fp8_dense(x, quantize_fp8_weight(w))
+    assert torch.equal(y, (w * 3).view(1, n))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("m", [4, 300])
 def test_two_graphs_of_a_laid_out_weight(m):
     layers = []
