@@ -456,7 +456,9 @@ std::vector<Tensor> coalesce_rows(Tensor values, Tensor ids) {
   s.scale = 1.f;
   s.limit = (uint32_t)n;
   // small results are summed into room for n rows before the host knows how
-  // many there are, which takes it longer than the sums take
+  // many there are, which takes it longer than the sums take (20 thousand rows
+  // of 16 columns 57 us, 62 where it waits first; 400 thousand, 73 and 80).
+  // The limit is for memory: the result keeps the room
   const bool early = n * d * values.element_size() <= (4 << 20);
   Tensor rows;
   const auto sum_into = [&](int64_t most) {

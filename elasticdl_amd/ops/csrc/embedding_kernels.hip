@@ -17,7 +17,6 @@
 
 #include <algorithm>
 #include <cstdint>
-#include <type_traits>
 
 #include "embedding_kernels.h"
 
@@ -503,7 +502,9 @@ __global__ __launch_bounds__(256) void sort_move_kernel(
 // key and then by position, and it is counted. That is N^2 comparisons, but
 // two instructions each and all of the chip's at once, where a sort in one
 // workgroup waits for itself (6656 ids of 21 bits: 24 us in passes of 8 bits,
-// 12 us counted and 4 for the runs). A workgroup has 32 items, and two lanes
+// 12 us counted and 4 for the runs). Sums of 8192 rows by id take 36 us so
+// and 69 by the radix sort; of 16384, whose keys would take 128 KB of LDS, 62
+// and 68. A workgroup has 32 items, and two lanes
 // of each wave for each share those that they are compared with.
 //
 // IDS: ids of any value, less 2^31 below the first, which goes to info[0];
@@ -621,36 +622,45 @@ __global__ __launch_bounds__(kSmallThreads) void runs_small_kernel(
     const int64_t* __restrict__ ids, const uint32_t* __restrict__ pos,
     uint32_t* starts, uint32_t* runs, uint32_t* rows, int64_t* unique,
     uint32_t* found) {
-  typedef typename std::conditional<IDS, uint64_t, uint32_t>::type K;
   __shared__ uint32_t s_count[kSmallWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  bool far = false;
-  uint64_t low = 0;
-  if constexpr (IDS) {
-    far = info[1] != 0;  // all threads alike
-    low = far ? 0 : (uint64_t)info[0];
-  }
+  const bool far = IDS && info[1] != 0;  // all threads alike
   const int items = (N + kSmallThreads - 1) / kSmallThreads;
   const int i0 = wave * items * 64 + lane;
-  K key[kSmallItems], last[kSmallItems];
+  uint32_t key[kSmallItems];
+  bool first[kSmallItems];
+  if (far) {
+    int64_t id[kSmallItems], last[kSmallItems];
 #pragma unroll
-  for (int k = 0; k < kSmallItems; ++k) {
-    const int i = i0 + k * 64;
-    const bool in = k < items && i < N;
-    if (IDS && far) {
-      key[k] = in ? ids[pos[i]] : 0;
+    for (int k = 0; k < kSmallItems; ++k) {
+      const int i = i0 + k * 64;
+      const bool in = k < items && i < N;
+      id[k] = in ? ids[pos[i]] : 0;
       last[k] = in && i > 0 ? ids[pos[i - 1]] : 0;
-    } else {
+    }
+#pragma unroll
+    for (int k = 0; k < kSmallItems; ++k) {
+      const int i = i0 + k * 64;
+      first[k] = k < items && i < N && (i == 0 || last[k] != id[k]);
+    }
+  } else {
+    uint32_t last[kSmallItems];
+#pragma unroll
+    for (int k = 0; k < kSmallItems; ++k) {
+      const int i = i0 + k * 64;
+      const bool in = k < items && i < N;
       key[k] = in ? keys[i] : 0;
       last[k] = in && i > 0 ? keys[i - 1] : 0;
     }
+#pragma unroll
+    for (int k = 0; k < kSmallItems; ++k) {
+      const int i = i0 + k * 64;
+      first[k] = k < items && i < N && (i == 0 || last[k] != key[k]);
+    }
   }
   uint32_t here = 0, place[kSmallItems];
-  bool first[kSmallItems];
 #pragma unroll
   for (int k = 0; k < kSmallItems; ++k) {
-    const int i = i0 + k * 64;
-    first[k] = k < items && i < N && (i == 0 || last[k] != key[k]);
     const uint64_t set = __ballot(first[k]);
     place[k] = here + __builtin_amdgcn_mbcnt_hi(
                           (uint32_t)(set >> 32),
@@ -674,7 +684,8 @@ __global__ __launch_bounds__(kSmallThreads) void runs_small_kernel(
       const uint32_t at = before + place[k];
       starts[at] = i0 + k * 64;
       if constexpr (IDS)
-        unique[at] = (int64_t)(low + key[k]);
+        unique[at] = far ? ids[pos[i0 + k * 64]]
+                         : (int64_t)((uint64_t)info[0] + (uint64_t)key[k]);
       else
         rows[at] = key[k];
     }
@@ -1226,10 +1237,14 @@ void launch_segments(const edl_segments& a, hipStream_t st) {
   }
 
 // Up to 256 thousand items, a pass less counts for more than the runs in
-// which it writes (160 thousand of 21 bits: 77 us for a whole gradient with 2
-// passes of 11 bits, 92 with 3 of 7), and tiles of 1024 fill the chip until
-// there are a million (820 thousand: 167 us with 9 bits, 177 with 11, 204
-// with tiles of 4096).
+// which it writes, and tiles of 1024 fill the chip until there are a million.
+// Whole gradients of a table of 2^20 - 1 rows, and sums by ids of 27 bits, us:
+//   items      Plan4x11   Plan4x9    Plan16x9
+//   200,000    61   86    69   82    73  100
+//   400,000    60  100    67   98    75  107
+//   800,000    85  134    76  130    81  122
+//   1,500,000 128  189   107  180   109  161
+// The key's width moves where they cross; the borders are between the two.
 int sort_plan(int64_t N) {
   return N < 256 * 1024 ? 0 : N < 1024 * 1024 ? 1 : 2;
 }
