@@ -1250,7 +1250,9 @@ extern "C" int edl_fp8_quantize_pair(const edl_fp8_quant* x,
 // it takes the products that give each of the 256 CUs one. (In 32 bits a
 // wave's fragments take twice the registers: no.) Where 128 x 128 leaves CUs
 // without work, the ring of 64 x 128 is in time what its loads take: 4096 x
-// 624 x 400 17.7 us in 128 tiles of 128, 13.3 in 256 of the ring.
+// 624 x 400 10.8 us in 128 tiles of 128, 7.6 in 256 of the ring, and in 32
+// bits 14.0 and 9.9. Large products in 32 bits reach 1.18 PFLOP/s (16384 x
+// 4096 x 4096 465 us, in 8 bits 240).
 //
 // Splits, up to 512 workgroups in all (two a CU): a join is a launch more,
 // so a split has at least 8 blocks to do, or 4 where something else needs
