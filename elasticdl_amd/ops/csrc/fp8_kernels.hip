@@ -17,10 +17,10 @@
 // 32 bits. So where a result is returned in 32 bits, or the sign of a sum
 // decides a relu's gradient, the bytes are widened to bf16 in registers on the
 // way (exactly from 2^-126 up, scale included) and multiplied by the bf16
-// instruction, whose sums hold 24 bits (8e-9 measured), at half the rate. The error of a sum is
-// in proportion to its largest products, not to its own size or its
-// neighbours', so a result says nothing of how near to zero is too near, and
-// all of a relu's sums are taken in 32 bits.
+// instruction, whose sums hold 24 bits (8e-9 measured), at half the rate. The
+// error of a sum is in proportion to its largest products, not to its own size
+// or its neighbours', so a result says nothing of how near to zero is too
+// near, and all of a relu's sums are taken in 32 bits.
 //
 // Layout. A matrix [R, C] that is contracted over C is stored as bytes
 // [R, Cp], Cp = C rounded up to 128 (zeros behind C), with scales
