@@ -16,7 +16,7 @@
 // e4m3. That is far below e4m3's and a 16-bit result's own rounding, but not
 // 32 bits. So where a result is returned in 32 bits, or the sign of a sum
 // decides a relu's gradient, the bytes are widened to bf16 in registers on the
-// way (exactly from 2^-126 up, scale included) and multiplied by the bf16
+// way (exactly, scale included, from 2^-133 up) and multiplied by the bf16
 // instruction, whose sums hold 24 bits (8e-9 measured), at half the rate. The
 // error of a sum is in proportion to its largest products, not to its own size
 // or its neighbours', so a result says nothing of how near to zero is too
